@@ -114,7 +114,7 @@ def _run_two_ranks(tmp_path, backend, mt, world=2):
     perr = (r0["flat"] - flat).abs().max().item()
     # (no retry: ranks sharing one GPU run each other's kernels side by side, and round 3 tolerated one repetition here because
     # a packed-fp32 operand form misbehaves beside f16 MFMAs of another process -- tests/test_isa_audit.py now covers every
-    # kernel source and RCCL's code object, so a wrong sum is a failure)
+    # kernel source, so a wrong sum is a failure)
     assert gerr < 1e-6, gerr
     assert perr < (1e-6 if world == 2 else 2.1e-3), perr          # Adam's first step is +-lr: a rounding may flip a ~0 entry
     # BatchNorm statistics stay rank-local (DataParallel: per-replica statistics)

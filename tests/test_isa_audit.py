@@ -2,8 +2,7 @@
 of src1 while src0 reads its low half (op_sel[src1] = 1, op_sel[src0] = 0).  On MI355X such an instruction returns wrong values
 now and then while a wave of another kernel on the same CU executes v_mfma_f32_32x32x16_f16 (tools/pk_f32_beside_mfma_probe.hip,
 DESIGN.md section 7) -- and with side-stream weight gradients, RCCL reductions beside the backward pass or ranks sharing a GPU,
-any kernel can end up beside one.  The same scan over RCCL's own gfx950 code object (`python tools/isa_audit.py --rccl`) is
-committed per round under profiles/ (clean: 0 of its 325 packed-fp32 instructions use op_sel at all)."""
+any kernel can end up beside one."""
 import importlib.util
 import os
 import shutil

@@ -3,12 +3,11 @@
 tools/pk_f32_beside_mfma_probe.hip): a `v_pk_*_f32` whose LOW lane reads the HIGH half of src1 while src0 reads its low half
 (op_sel[src1] = 1, op_sel[src0] = 0).
 
-    python tools/isa_audit.py file.s [...]            # hipcc -S output or llvm-objdump -d output
-    python tools/isa_audit.py --rccl                  # extract the gfx950 code object of torch's librccl.so and audit it
+    python tools/isa_audit.py file.s [...]            # hipcc -S output of a source of this repository
     python tools/isa_audit.py --csrc                  # compile every csrc/*.hip to gfx950 assembly and audit it
 
 Prints one line per input: packed-fp32 instructions, op_sel histogram, fragile count (+ the kernels that hold them).
-tests/test_isa_audit.py imports scan() for the csrc files; the RCCL result of the round is kept under profiles/."""
+tests/test_isa_audit.py imports scan() for the csrc files.  Only code built here from source is read: installed libraries stay closed."""
 import collections
 import os
 import re
@@ -17,10 +16,9 @@ import sys
 import tempfile
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-LLVM = "/opt/rocm/lib/llvm/bin"
 PK = re.compile(r"\b(v_pk_\w+_f32)\b(.*)")
 SEL = re.compile(r"op_sel:\[([01,]+)\]")
-LABEL = re.compile(r"^(?:[0-9a-f]+ <)?([A-Za-z_][\w.$]*)>?:\s*$")
+LABEL = re.compile(r"^([A-Za-z_][\w.$]*):\s*$")
 
 
 def scan(path):
@@ -59,18 +57,6 @@ def report(name, r, out=sys.stdout):
         out.write("        %s\n" % l)
 
 
-def rccl_asm(workdir):
-    import torch
-    lib = os.path.join(os.path.dirname(torch.__file__), "lib", "librccl.so")
-    fat, co, asm = (os.path.join(workdir, n) for n in ("rccl_fatbin.bin", "rccl_gfx950.co", "rccl_gfx950.s"))
-    subprocess.run([os.path.join(LLVM, "llvm-objcopy"), "--dump-section", ".hip_fatbin=" + fat, lib], check=True)
-    subprocess.run([os.path.join(LLVM, "clang-offload-bundler"), "--unbundle", "--type=o", "--input=" + fat,
-                    "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", "--output=" + co], check=True)
-    with open(asm, "w") as f:
-        subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", "--mcpu=gfx950", co], check=True, stdout=f)
-    return lib, asm
-
-
 def csrc_asm(src, workdir):
     from sound_event_detection_dcase2017_task4_amd import build
     out = os.path.join(workdir, os.path.basename(src) + ".s")
@@ -84,11 +70,6 @@ def main(argv):
     sys.path.insert(0, REPO)
     bad = 0
     with tempfile.TemporaryDirectory() as wd:
-        if "--rccl" in argv:
-            lib, asm = rccl_asm(wd)
-            r = scan(asm)
-            report("%s [gfx950 code object, %d bytes of disassembly]" % (lib, os.path.getsize(asm)), r)
-            bad += len(r["fragile"])
         if "--csrc" in argv:
             from sound_event_detection_dcase2017_task4_amd import build
             for s in build.SOURCES:
