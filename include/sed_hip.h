@@ -28,6 +28,11 @@ extern "C" {
 
 const char* sed_version(void);
 
+/* element types of the entry points that take more than one */
+#define SED_F32 0
+#define SED_F16 1
+#define SED_BF16 2
+
 /* ---- K1 log-mel front-end -------------------------------------------------------------------------------
  * Replaces torchlibrosa Spectrogram + LogmelFilterBank as constructed at pytorch/models.py:251-258 and called
  * at :284-285 (reflect pad 512, Hann-windowed 1024-point DFT, hop 320, power, 513x64 Slaney mel matrix,
@@ -472,6 +477,23 @@ int sed_adam_amsgrad(float* p, const float* g, float* m, float* v, float* vmax, 
  * the gradient bucket it all-reduces last and hands it to sed_adam_amsgrad as rank_flag (nullable): a non-zero / NaN word
  * after the sum means SOME rank met a non-finite operand, and every rank refuses the same step. */
 int sed_guard_publish(const int* err_dev, float* flag_out, sed_stream_t stream);
+
+/* ---- AdamW over many tensors in one launch, moments in 32 or in 8 bits ------------------------------------------------
+ * m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+ * rows (device): per tensor six longs {parameter address, gradient address (0: the tensor is left as it is), first element of its
+ * moments (a multiple of 256), first element of its 32-bit copy in `master` (16-bit parameters; a multiple of 256), elements,
+ * hyper-parameter group | element type << 32}.  chunks (device): nchunks pairs {tensor, chunk}: every sed_adamw_chunk() elements of
+ * every tensor once.  Moments: flat buffers padded to 256 elements per tensor -- float (state_bits 32), or signed / unsigned bytes
+ * (state_bits 8) with one float of m_scale / v_scale per 256 elements: m = sign(q) (|q| / 127)^2 scale, v = (q / 255)^4 scale.
+ * hyper (HOST): per group five doubles {lr, beta1, beta2, eps, weight_decay}, at most 16 groups; grad_scale multiplies the gradient.
+ * skip_flag (nullable, device): non-zero leaves everything untouched and adds 1 to *skipped, as in sed_adam_amsgrad.
+ * sed_adamw_moments: the values that 8-bit moments stand for, n elements (a multiple of 256). */
+int sed_adamw_chunk(void);
+int sed_adamw(const long* rows, const int* chunks, long nchunks, void* m, void* v, float* m_scale, float* v_scale, float* master,
+              int state_bits, const double* hyper, int ngroups, int step, float grad_scale, const int* skip_flag, int* skipped,
+              sed_stream_t stream);
+int sed_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, long n, float* out_m, float* out_v,
+                      sed_stream_t stream);
 
 #ifdef __cplusplus
 }

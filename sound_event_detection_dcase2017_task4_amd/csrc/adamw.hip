@@ -1,0 +1,232 @@
+// AdamW over many tensors in one launch, moments held in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g^2      p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// The work is a list of chunks of 4096 elements, each inside one tensor: a 28-tensor model and a single 240-million-element matrix
+// fill the chip alike, and no tensor costs a launch.  Bound by HBM: 28 bytes an element with 32-bit moments (parameter, gradient, two
+// moments in; parameter, two moments out; a 16-bit parameter adds its 32-bit copy and saves as much), 16 bytes with 8-bit ones.
+//
+// 8-bit moments: a block of 256 elements -- one wave, four elements a lane -- shares one scale, the block's largest magnitude, held
+// in 32 bits.  The codes are powers of a linear grid, because the moments of one block spread over decades and a relative error
+// is what the update sees:
+//   m = sign(q) (|q| / 127)^2 scale, q = rint(127 sqrt(|m| / scale))       half a step = 0.8 % at the scale, 8 % at a hundredth of it
+//   v = (q / 255)^4 scale,           q = rint(255 (v / scale)^(1/4))       half a step of sqrt(v) = 0.4 % at the scale
+// A positive v never decodes to 0 (its code is at least 1): m / (0 + eps) would be a step of any size.  The update itself uses the
+// new moments in 32 bits; only what the next step reads is rounded.  A NaN or an infinity in a block makes its scale NaN or infinite,
+// and the block reads back as NaN: as with 32-bit moments, nothing hides it.
+#include "common.h"
+#include "sed_hip.h"
+
+SED_OBJECT_FLAGS(adamw)
+
+namespace {
+
+constexpr int BLK = 256;            // elements of one 8-bit block; every tensor's state begins at a multiple of it
+constexpr int CHUNK = 4096;         // elements of one workgroup
+constexpr int MAX_GROUPS = 16;
+constexpr int ROW = 6;              // longs per tensor: parameter, gradient, first element of its moments, of its copy, elements, group | type << 32
+
+struct Hyper {
+    float decay, step_size, b1, omb1, b2, omb2, inv_c2, eps;
+};
+struct AdamwP {
+    const long* rows;
+    const int2* chunks;             // (tensor, chunk inside it)
+    void* m;
+    void* v;
+    float* ms;
+    float* vs;
+    float* master;
+    const int* skip_flag;
+    int* skipped;
+    float grad_scale;
+    Hyper h[MAX_GROUPS];
+};
+
+template <typename T> struct Vec4;
+template <> struct Vec4<float> { typedef float type __attribute__((ext_vector_type(4))); };
+template <> struct Vec4<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
+template <> struct Vec4<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
+
+// four elements at e of a tensor of n; wide when the base address allows it
+template <typename T> __device__ __forceinline__ void load4(const T* p, long e, long n, bool wide, float (&f)[4]) {
+    if (wide && e + 4 <= n) {
+        const auto q = *reinterpret_cast<const typename Vec4<T>::type*>(p + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = (float)q[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = e + j < n ? (float)p[e + j] : 0.f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, long e, long n, bool wide, const float (&f)[4]) {
+    if (wide && e + 4 <= n) {
+        typename Vec4<T>::type q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = (T)f[j];
+        *reinterpret_cast<typename Vec4<T>::type*>(p + e) = q;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (e + j < n) p[e + j] = (T)f[j];
+    }
+}
+
+// largest of non-negative floats over the wave, compared as bits: a NaN is the largest of all and is not lost
+__device__ __forceinline__ float wave_max_bits(float a, float b, float c, float d) {
+    unsigned m = max(max(__float_as_uint(a), __float_as_uint(b)), max(__float_as_uint(c), __float_as_uint(d)));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+    return __uint_as_float(m);
+}
+
+// The codes and the sums below are formed with one rounding per operation (no fused multiply-add): a code is then the same wherever
+// it is formed, and a value next to the border of two codes does not depend on how the compiler groups the terms.
+__device__ __forceinline__ float decode_m(int q, float scale) {
+#pragma clang fp contract(off)
+    const float u = (float)q * (float)(1.0 / 127.0);
+    return u * fabsf(u) * scale;
+}
+__device__ __forceinline__ float decode_v(int q, float scale) {
+#pragma clang fp contract(off)
+    float u = (float)q * (float)(1.0 / 255.0);
+    u = u * u;
+    return u * u * scale;
+}
+__device__ __forceinline__ int encode_m(float m, float scale) {
+    const int q = (int)rintf(sqrtf(fabsf(m) / scale) * 127.f);
+    return m < 0.f ? -q : q;
+}
+__device__ __forceinline__ int encode_v(float v, float scale) {
+    const int q = (int)rintf(sqrtf(sqrtf(v / scale)) * 255.f);
+    return v > 0.f ? max(q, 1) : q;
+}
+
+template <typename T, bool EIGHT> __device__ __forceinline__ void adamw_chunk(const AdamwP& a, const long* row, long c0) {
+    T* const p = reinterpret_cast<T*>(row[0]);
+    const T* const g = reinterpret_cast<const T*>(row[1]);
+    const long n = row[4], off = row[2], padded = (n + BLK - 1) / BLK * BLK;
+    float* const copy = sizeof(T) == 4 ? nullptr : a.master + row[3];
+    const Hyper h = a.h[(int)(row[5] & 0xffffffff)];
+    const bool wide = ((row[0] | row[1]) & (4 * sizeof(T) - 1)) == 0;
+    float pv[4][4], gv[4][4], mv[4][4], vv[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long e = c0 + i * 1024 + threadIdx.x * 4;
+        if (e >= padded) continue;
+        load4(g, e, n, wide, gv[i]);
+        if (sizeof(T) == 4) load4(p, e, n, wide, pv[i]);
+        else load4(copy, e, padded, true, pv[i]);
+        if (EIGHT) {
+            const char4 qm = reinterpret_cast<const char4*>(a.m)[(off + e) >> 2];
+            const uchar4 qv = reinterpret_cast<const uchar4*>(a.v)[(off + e) >> 2];
+            const float sm = a.ms[(off + e) / BLK], sv = a.vs[(off + e) / BLK];
+            mv[i][0] = decode_m(qm.x, sm); mv[i][1] = decode_m(qm.y, sm); mv[i][2] = decode_m(qm.z, sm); mv[i][3] = decode_m(qm.w, sm);
+            vv[i][0] = decode_v(qv.x, sv); vv[i][1] = decode_v(qv.y, sv); vv[i][2] = decode_v(qv.z, sv); vv[i][3] = decode_v(qv.w, sv);
+        } else {
+            load4(reinterpret_cast<const float*>(a.m) + off, e, padded, true, mv[i]);
+            load4(reinterpret_cast<const float*>(a.v) + off, e, padded, true, vv[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long e = c0 + i * 1024 + threadIdx.x * 4;
+        if (e >= padded) continue;                 // whole waves: a wave's 256 elements are one block
+        {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float gj = gv[i][j] * a.grad_scale;
+                mv[i][j] = mv[i][j] * h.b1 + gj * h.omb1;
+                vv[i][j] = vv[i][j] * h.b2 + gj * gj * h.omb2;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pv[i][j] = pv[i][j] * h.decay - h.step_size * mv[i][j] / fmaf(sqrtf(vv[i][j]), h.inv_c2, h.eps);
+        if (e < n) {
+            store4(p, e, n, wide, pv[i]);
+            if (sizeof(T) != 4) store4(copy, e, n, true, pv[i]);
+        }
+        if (EIGHT) {
+            const float sm = wave_max_bits(fabsf(mv[i][0]), fabsf(mv[i][1]), fabsf(mv[i][2]), fabsf(mv[i][3]));
+            const float sv = wave_max_bits(fabsf(vv[i][0]), fabsf(vv[i][1]), fabsf(vv[i][2]), fabsf(vv[i][3]));
+            const float dm = sm > 0.f ? sm : 1.f, dv = sv > 0.f ? sv : 1.f;
+            reinterpret_cast<char4*>(a.m)[(off + e) >> 2] =
+                make_char4(encode_m(mv[i][0], dm), encode_m(mv[i][1], dm), encode_m(mv[i][2], dm), encode_m(mv[i][3], dm));
+            reinterpret_cast<uchar4*>(a.v)[(off + e) >> 2] =
+                make_uchar4(encode_v(vv[i][0], dv), encode_v(vv[i][1], dv), encode_v(vv[i][2], dv), encode_v(vv[i][3], dv));
+            if ((threadIdx.x & 63) == 0) {
+                a.ms[(off + e) / BLK] = sm;
+                a.vs[(off + e) / BLK] = sv;
+            }
+        } else {
+            store4(reinterpret_cast<float*>(a.m) + off, e, n, true, mv[i]);
+            store4(reinterpret_cast<float*>(a.v) + off, e, n, true, vv[i]);
+        }
+    }
+}
+
+template <bool EIGHT> __global__ __launch_bounds__(256) void adamw_kernel(AdamwP a) {
+    if (a.skip_flag && __hip_atomic_load(a.skip_flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicAdd(a.skipped, 1);
+        return;
+    }
+    const int2 c = a.chunks[blockIdx.x];
+    const long* const row = a.rows + (long)c.x * ROW;
+    if (row[1] == 0) return;                       // no gradient in this step: the tensor and its moments stay
+    const int type = (int)(row[5] >> 32);
+    const long c0 = (long)c.y * CHUNK;
+    if (type == SED_F32) adamw_chunk<float, EIGHT>(a, row, c0);
+    else if (type == SED_F16) adamw_chunk<_Float16, EIGHT>(a, row, c0);
+    else adamw_chunk<__bf16, EIGHT>(a, row, c0);
+}
+
+__global__ __launch_bounds__(256) void adamw_moments_kernel(const char4* m, const float* ms, const uchar4* v, const float* vs, long n4,
+                                                            float4* om, float4* ov) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long)gridDim.x * 256) {
+        const char4 q = m[i];
+        const uchar4 r = v[i];
+        const float sm = ms[i / (BLK / 4)], sv = vs[i / (BLK / 4)];
+        om[i] = make_float4(decode_m(q.x, sm), decode_m(q.y, sm), decode_m(q.z, sm), decode_m(q.w, sm));
+        ov[i] = make_float4(decode_v(r.x, sv), decode_v(r.y, sv), decode_v(r.z, sv), decode_v(r.w, sv));
+    }
+}
+
+}  // namespace
+
+SED_API int sed_adamw_chunk(void) { return CHUNK; }
+
+SED_API int sed_adamw(const long* rows, const int* chunks, long nchunks, void* m, void* v, float* m_scale, float* v_scale,
+                      float* master, int state_bits, const double* hyper, int ngroups, int step, float grad_scale, const int* skip_flag,
+                      int* skipped, sed_stream_t stream) {
+    if (!rows || !chunks || !m || !v || !hyper || nchunks < 1 || nchunks > 0x7fffffffL || ngroups < 1 || ngroups > MAX_GROUPS || step < 1)
+        return SED_EINVAL;
+    if (state_bits != 32 && (state_bits != 8 || !m_scale || !v_scale)) return SED_EINVAL;
+    if (skip_flag && !skipped) return SED_EINVAL;
+    AdamwP a;
+    a.rows = rows; a.chunks = reinterpret_cast<const int2*>(chunks);
+    a.m = m; a.v = v; a.ms = m_scale; a.vs = v_scale; a.master = master;
+    a.skip_flag = skip_flag; a.skipped = skipped; a.grad_scale = grad_scale;
+    for (int k = 0; k < ngroups; ++k) {
+        const double *q = hyper + 5 * k, lr = q[0], b1 = q[1], b2 = q[2], eps = q[3], wd = q[4];
+        if (!(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1 && eps >= 0)) return SED_EINVAL;
+        // formed in double and rounded once: 1.f - 0.999f is 5e-5 off
+        a.h[k] = {(float)(1.0 - lr * wd), (float)(lr / (1.0 - pow(b1, step))), (float)b1, (float)(1.0 - b1), (float)b2, (float)(1.0 - b2),
+                  (float)(1.0 / sqrt(1.0 - pow(b2, step))), (float)eps};
+    }
+    if (state_bits == 8) hipLaunchKernelGGL(adamw_kernel<true>, dim3((unsigned)nchunks), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(adamw_kernel<false>, dim3((unsigned)nchunks), dim3(256), 0, stream, a);
+    SED_LAUNCH_CHECK();
+    return 0;
+}
+
+SED_API int sed_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, long n, float* out_m,
+                              float* out_v, sed_stream_t stream) {
+    if (!m || !m_scale || !v || !v_scale || !out_m || !out_v || n < 1 || n % BLK) return SED_EINVAL;
+    const long nb = (n / 4 + 255) / 256;
+    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)(nb > 16384 ? 16384 : nb)), dim3(256), 0, stream,
+                       reinterpret_cast<const char4*>(m), m_scale, reinterpret_cast<const uchar4*>(v), v_scale, n / 4,
+                       reinterpret_cast<float4*>(out_m), reinterpret_cast<float4*>(out_v));
+    SED_LAUNCH_CHECK();
+    return 0;
+}

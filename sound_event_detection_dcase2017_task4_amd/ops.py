@@ -1933,3 +1933,47 @@ def adam_amsgrad_(p, g, m, v, vmax, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, 
 def guard_publish(flag_out):
     """flag_out[0] = NaN if this rank's found-non-finite word is set, else 0 (see include/sed_hip.h: sed_guard_publish)."""
     _call("sed_guard_publish", _sf16_err_dev_ptr(flag_out.device), _ptr(flag_out), _stream())
+
+
+# ------------------------------------------------------------------------------------------------------------
+# operators on float32 / float16 / bfloat16 tensors
+
+DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}       # SED_F32, SED_F16, SED_BF16
+
+
+class _on_device(object):
+    """Makes the device of `t` the current one around a launch (its current stream is then the one that is used)."""
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def adamw_(rows, chunks, nchunks, m, v, m_scale, v_scale, master, state_bits, hyper, step, grad_scale=1.0, guard=None, skipped=None):
+    """One AdamW step over the tensors of `rows` (device int64 (tensors, 6)) in one launch: see include/sed_hip.h, sed_adamw.
+    hyper: host float64 array (groups, 5).  guard (default: on while the split-f16 kernels are in use): the step is refused when a
+    split-f16 kernel met a NaN / inf operand; see NonFiniteOperand.  optim.FusedAdamW keeps the tables."""
+    _chk_dev(rows, chunks, m, v)
+    if guard is None:
+        guard = USE_SF16 and skipped is not None
+    invalidate_weight_caches()                     # parameters change through raw pointers: `_version` does not see it
+    _call("sed_adamw", _ptr(rows), _ptr(chunks), nchunks, _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), _ptr(master), state_bits,
+          hyper.ctypes.data, hyper.shape[0], step, grad_scale, _sf16_err_dev_ptr(m.device) if guard else None,
+          _ptr(skipped) if guard else None, _stream())
+
+
+def adamw_moments(m, m_scale, v, v_scale):
+    """The float32 values that 8-bit moments stand for (sed_adamw_moments)."""
+    _chk_dev(m, v)
+    om, ov = (torch.empty((m.numel(),), dtype=torch.float32, device=m.device) for _ in range(2))
+    _call("sed_adamw_moments", _ptr(m), _ptr(m_scale), _ptr(v), _ptr(v_scale), m.numel(), _ptr(om), _ptr(ov), _stream())
+    return om, ov

@@ -15,6 +15,7 @@ several backward passes into one step needs `direct_grads=False` (plain autograd
 """
 import collections
 
+import numpy as np
 import torch
 
 from . import ops, parallel
@@ -328,3 +329,219 @@ class FusedAdamAmsgrad(object):
         for k, m in zip(("exp_avg", "exp_avg_sq", "max_exp_avg_sq"), moments):
             getattr(self, k).copy_(m.reshape(-1))
         ops.invalidate_weight_caches()
+
+
+STATE_BLOCK = 256      # elements that share one scale of an 8-bit moment; every tensor's moments begin at a multiple of it
+
+
+class FusedAdamW(object):
+    """AdamW (decoupled weight decay) over many separate tensors in ONE launch (sed_adamw), float32 / float16 / bfloat16 ones together.
+
+    params: a module, an iterable of tensors, or a list of groups {'params': [...], 'lr' / 'betas' / 'eps' / 'weight_decay': ...} as
+    torch.optim.AdamW takes them (at most 16 groups); `param_groups` may be changed between steps.  Gradients are read from `p.grad`
+    wherever they lie; a tensor whose gradient is None is left as it is in that step (weight decay and moments too).  One step
+    counter serves all tensors, as in FusedAdamAmsgrad.
+
+    state_bits: 32 -- the two moments as float32; 8 -- as 8-bit codes with one float32 scale per 256 elements (csrc/adamw.hip), a
+    quarter of the memory.  The update itself is computed in 32 bits either way.  16-bit parameters get a 32-bit copy (`master`, flat,
+    in the order of those parameters) that the step updates and rounds once into the parameter; a parameter that torch changes in
+    place (`load_state_dict` of its model, clipping) is copied back into it at the next step.
+
+    `exp_avg`, `exp_avg_sq` (and `exp_avg_scale`, `exp_avg_sq_scale`) are flat buffers in which every tensor begins at a multiple of
+    256 elements (`offsets`).  In a data-parallel job reduce the gradients first and pass `step(grad_scale=1 / world_size)`.  The step
+    number is an argument of the launch, so step() refuses to be captured into a graph: it belongs behind the graph.
+
+    Found-non-finite guard: as FusedAdamAmsgrad, the kernel refuses a step behind a split-f16 kernel that met a NaN / inf operand;
+    the gradients themselves are not scanned (a NaN gradient makes a NaN parameter, as in torch)."""
+
+    DEFAULTS = ("lr", "betas", "eps", "weight_decay")
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32, got %r" % (state_bits,))
+        if hasattr(params, "parameters"):
+            params = [p for p in params.parameters() if p.requires_grad]
+        params = list(params)
+        if params and not isinstance(params[0], dict):
+            params = [{"params": params}]
+        defaults = {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay}
+        self.param_groups = []
+        for g in params:
+            extra = set(g) - set(self.DEFAULTS) - {"params"}
+            if extra:
+                raise ValueError("unknown parameter group option(s) %s" % sorted(extra))
+            ps = [g["params"]] if torch.is_tensor(g["params"]) else list(g["params"])
+            self.param_groups.append(dict(defaults, **{k: v for k, v in g.items() if k != "params"}, params=ps))
+        self.params = [p for g in self.param_groups for p in g["params"]]
+        if not self.params:
+            raise ValueError("no trainable parameters")
+        if len(self.param_groups) > 16:
+            raise ValueError("at most 16 parameter groups, got %d" % len(self.param_groups))
+        self._hyper()                                       # refuses bad values now, not at the first step
+        self._check_params()
+        dev = self.params[0].device
+        self.device, self.state_bits = dev, state_bits
+        self.offsets, self._copy_at = [], []
+        total = copied = 0
+        for p in self.params:
+            n = -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+            self.offsets.append(total)
+            self._copy_at.append(copied)
+            total += n
+            copied += n if p.dtype != torch.float32 else 0
+        total = max(total, STATE_BLOCK)
+        zeros = lambda n, t: torch.zeros((n,), dtype=t, device=dev)  # noqa: E731
+        self.exp_avg = zeros(total, torch.float32 if state_bits == 32 else torch.int8)
+        self.exp_avg_sq = zeros(total, torch.float32 if state_bits == 32 else torch.uint8)
+        self.exp_avg_scale = zeros(total // STATE_BLOCK, torch.float32) if state_bits == 8 else None
+        self.exp_avg_sq_scale = zeros(total // STATE_BLOCK, torch.float32) if state_bits == 8 else None
+        self.master = zeros(copied, torch.float32) if copied else None
+        self._versions = [None] * len(self.params)
+        self.step_count = 0
+        self.skipped_steps = 0
+        self._skipped = zeros(1, torch.int32)
+        ops._GUARDED.add(self)
+        # the table of tensors: gradient addresses change from step to step, the rest only when a parameter moves
+        self._rows = np.zeros((len(self.params), 6), dtype=np.int64)
+        group = [k for k, g in enumerate(self.param_groups) for _ in g["params"]]
+        self._rows[:, 2], self._rows[:, 3] = self.offsets, self._copy_at
+        self._rows[:, 4] = [p.numel() for p in self.params]
+        self._rows[:, 5] = [k | ops.DTYPE_CODES[p.dtype] << 32 for k, p in zip(group, self.params)]
+        self._sent = self._dev_rows = self._sent_on = None
+        per = int(ops._lib.lib().sed_adamw_chunk())
+        count = -(-self._rows[:, 4] // per)
+        first = np.repeat(np.cumsum(count) - count, count)
+        chunks = np.stack([np.repeat(np.arange(len(count)), count), np.arange(len(first)) - first], axis=1).astype(np.int32)
+        self._chunks = torch.from_numpy(chunks).to(dev)     # complete when this returns: any stream may read it
+
+    def _hyper(self):
+        rows = []
+        for g in self.param_groups:
+            lr, (b1, b2), eps, wd = float(g["lr"]), g["betas"], float(g["eps"]), float(g["weight_decay"])
+            if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and wd >= 0.0):
+                raise ValueError("invalid lr / betas / eps / weight_decay: %r" % ((lr, (b1, b2), eps, wd),))
+            rows.append((lr, b1, b2, eps, wd))
+        return np.array(rows, dtype=np.float64)
+
+    def _check_params(self):
+        dev, spans = self.params[0].device, []
+        for p in self.params:
+            if not torch.is_tensor(p) or p.device.type != "cuda":
+                raise RuntimeError("FusedAdamW: move the model to the GPU first (HIP kernel, no CPU path)")
+            if p.device != dev:
+                raise ValueError("FusedAdamW: all parameters must be on one device, got %s and %s" % (dev, p.device))
+            if p.dtype not in ops.DTYPE_CODES:
+                raise ValueError("FusedAdamW: parameters must be float32, float16 or bfloat16, got %s" % p.dtype)
+            if not p.is_contiguous():
+                raise ValueError("FusedAdamW: parameters must be contiguous, got strides %s for shape %s" % (p.stride(), tuple(p.shape)))
+            if getattr(p, "_sed_sink", None) is not None:
+                raise ValueError("FusedAdamW: a parameter belongs to a FusedAdamAmsgrad (its gradient sinks point there)")
+            spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        spans = sorted(s for s in spans if s[0] != s[1])
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("FusedAdamW: a parameter appears twice, or two overlap in memory")
+
+    def zero_grad(self, set_to_none=True):
+        ops.drop_pending_wgrads()          # a backward pass that raised may have left side-stream work behind
+        for p in self.params:
+            if p.grad is not None:
+                if set_to_none:
+                    p.grad = None
+                else:
+                    p.grad.detach_().zero_()
+
+    def _refresh_copies(self):
+        """Take parameters that torch wrote since the last step (or never seen) into their 32-bit copies."""
+        for i, p in enumerate(self.params):
+            if p.dtype != torch.float32 and self._versions[i] != (p._version, p.data_ptr()):
+                self.master[self._copy_at[i]:self._copy_at[i] + p.numel()].copy_(p.detach().reshape(-1))
+                self._versions[i] = (p._version, p.data_ptr())
+
+    def _table(self):
+        """Device table of this step's tensors; the gradients it points to are returned with it and stay alive until the launch."""
+        grads = [p.grad for p in self.params]
+        if not all(g is None or g.is_contiguous() for g in grads):
+            grads = [g if g is None else g.contiguous() for g in grads]
+        rows = self._rows
+        where = [p.data_ptr() for p in self.params]
+        if where != self._sent_params():
+            self._check_params()
+            if [p.numel() for p in self.params] != rows[:, 4].tolist() or [ops.DTYPE_CODES[p.dtype] for p in self.params] != (rows[:, 5] >> 32).tolist():
+                raise ValueError("FusedAdamW: a parameter changed its size or type since the optimiser was made")
+            rows[:, 0] = where
+        rows[:, 1] = [0 if g is None else g.data_ptr() for g in grads]
+        for p, g in zip(self.params, grads):
+            if g is not None and (g.dtype != p.dtype or g.device != p.device or g.layout != torch.strided):
+                raise ValueError("FusedAdamW: a gradient of type %s on %s for a parameter of type %s on %s" % (g.dtype, g.device, p.dtype, p.device))
+        stream = ops._stream()
+        if self._sent is None or self._sent_on != stream or not np.array_equal(self._sent, rows):
+            # uploaded on the stream that reads it, into new memory: a step still in flight keeps the table it was given
+            self._dev_rows = ops.upload_small(rows, self.device, torch.int64)
+            self._sent, self._sent_on = rows.copy(), stream
+        return grads
+
+    def _sent_params(self):
+        return None if self._sent is None else self._sent[:, 0].tolist()
+
+    @torch.no_grad()
+    def step(self, grad_scale=1.0):
+        """One update of every tensor that has a gradient, multiplied by grad_scale first."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW.step() cannot be captured into a graph (the step number is an argument of the launch): "
+                               "capture forward and backward, and call step() behind the replay")
+        hyper = self._hyper()
+        with ops._on_device(self.exp_avg):
+            if self.master is not None:
+                self._refresh_copies()
+            grads = self._table()
+            self.step_count += 1
+            if len(self._chunks):
+                ops.adamw_(self._dev_rows, self._chunks, len(self._chunks), self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
+                           self.exp_avg_sq_scale, self.master, self.state_bits, hyper, self.step_count, float(grad_scale),
+                           skipped=self._skipped)
+        del grads
+        ops.check_device_errors()
+
+    def moments(self):
+        """(exp_avg, exp_avg_sq) as flat float32 buffers: the state itself with 32 bits, the values that the codes stand for with 8."""
+        if self.state_bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        with ops._on_device(self.exp_avg):
+            return ops.adamw_moments(self.exp_avg, self.exp_avg_scale, self.exp_avg_sq, self.exp_avg_sq_scale)
+
+    _STATE = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")
+
+    def state_dict(self):
+        if self.master is not None:
+            self._refresh_copies()
+        return dict({"step": self.step_count, "state_bits": self.state_bits, "numels": [p.numel() for p in self.params],
+                     "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]},
+                    **{k: getattr(self, k) for k in self._STATE})
+
+    def load_state_dict(self, sd):
+        """Takes over the step counter, the moments and the 32-bit copies of a state_dict() of the same tensors and state_bits; a
+        'master' of None (or none at all) takes the copies from the parameters.  lr / betas / eps / weight_decay stay those of this
+        optimiser.  Anything that does not fit is refused (ValueError) before anything is changed."""
+        if "step" not in sd or "exp_avg" not in sd or "exp_avg_sq" not in sd:
+            raise ValueError("unknown optimiser state layout (keys: %s): expected a FusedAdamW.state_dict()" % sorted(sd.keys()))
+        if sd.get("state_bits", 32) != self.state_bits:
+            raise ValueError("the state holds %r-bit moments, this optimiser %d-bit ones" % (sd.get("state_bits", 32), self.state_bits))
+        if "numels" in sd and list(sd["numels"]) != self._rows[:, 4].tolist():
+            raise ValueError("the state belongs to tensors of other sizes")
+        step = int(sd["step"])
+        if step < 0:
+            raise ValueError("a negative step number: %d" % step)
+        new = {}
+        for k in self._STATE:
+            have, want = sd.get(k), getattr(self, k)
+            if want is None or (k == "master" and have is None):
+                continue
+            have = None if have is None else torch.as_tensor(have)
+            if have is None or have.numel() != want.numel() or have.dtype != want.dtype:
+                raise ValueError("optimiser state '%s': expected %d values of %s" % (k, want.numel(), want.dtype))
+            new[k] = have
+        with torch.no_grad():
+            for k, have in new.items():
+                getattr(self, k).copy_(have.reshape(-1))
+        self.step_count = step
+        self._versions = [(p._version, p.data_ptr()) if "master" in new else None for p in self.params]
