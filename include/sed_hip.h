@@ -32,6 +32,11 @@ const char* sed_version(void);
 #define SED_F32 0
 #define SED_F16 1
 #define SED_BF16 2
+/* activations of sed_group_norm_* and sed_linear_* */
+#define SED_ACT_NONE 0
+#define SED_ACT_RELU 1
+#define SED_ACT_SILU 2
+#define SED_ACT_GELU 3 /* z Phi(z) */
 
 /* ---- K1 log-mel front-end -------------------------------------------------------------------------------
  * Replaces torchlibrosa Spectrogram + LogmelFilterBank as constructed at pytorch/models.py:251-258 and called
@@ -477,6 +482,21 @@ int sed_adam_amsgrad(float* p, const float* g, float* m, float* v, float* vmax, 
  * the gradient bucket it all-reduces last and hands it to sed_adam_amsgrad as rank_flag (nullable): a non-zero / NaN word
  * after the sum means SOME rank met a non-finite operand, and every rank refuses the same step. */
 int sed_guard_publish(const int* err_dev, float* flag_out, sed_stream_t stream);
+
+/* ---- group normalisation with an activation, channels last -----------------------------------------------------------
+ * x, y, gy, gx [N][S][C] of `dtype` (SED_F32 / SED_F16 / SED_BF16); group g = channels [g C/G, (g+1) C/G).
+ *   mean, rstd [N][G] (float): over the S rows and C/G channels of a group, rstd = 1 / sqrt(variance + eps), variance / count
+ *   z = (x - mean) rstd weight + bias;  y = act(z);  weight, bias [C] of wdtype, nullable (1 and 0)
+ *   gz = gy act'(z);  gweight = sum gz xhat;  gbias = sum gz  (float [C], nullable)
+ *   gx = rstd (gz weight - mean_g(gz weight) - xhat mean_g(gz weight xhat))  (nullable)
+ * ws: sed_group_norm_ws_floats(N, S, C, G, backward) floats of scratch.  No pointer needs more than its element's alignment.
+ * N, S, C >= 1, C % G == 0. */
+long sed_group_norm_ws_floats(long N, long S, int C, int G, int backward);
+int sed_group_norm_fwd(const void* x, const void* weight, const void* bias, int dtype, int wdtype, long N, long S, int C, int G,
+                       float eps, int act, void* y, float* mean, float* rstd, float* ws, sed_stream_t stream);
+int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const void* bias, int dtype, int wdtype, long N, long S,
+                       int C, int G, int act, const float* mean, const float* rstd, void* gx, float* gweight, float* gbias, float* ws,
+                       sed_stream_t stream);
 
 /* ---- AdamW over many tensors in one launch, moments in 32 or in 8 bits ------------------------------------------------
  * m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).

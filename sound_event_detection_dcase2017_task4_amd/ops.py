@@ -1958,6 +1958,107 @@ class _on_device(object):
         return False
 
 
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}                  # SED_ACT_*; gelu is z Phi(z)
+
+
+def _act_code(activation):
+    if activation not in ACTIVATIONS:
+        raise ValueError("activation must be one of %s, got %r" % (sorted(ACTIVATIONS), activation))
+    return ACTIVATIONS[activation]
+
+
+def _chk_operand(name, t, shape, dtypes, device):
+    """A further operand of an operator whose first one fixes device and sizes."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if t.dtype not in dtypes:
+        raise ValueError("%s must be %s, got %s" % (name, " or ".join(str(d) for d in dtypes), t.dtype))
+    if t.device != device:
+        raise ValueError("%s is on %s, the input on %s" % (name, t.device, device))
+
+
+def _group_norm_fwd(x, weight, bias, groups, eps, act):
+    C = x.shape[-1]
+    N, S = x.shape[0], x.numel() // (x.shape[0] * C)
+    y = torch.empty_like(x)
+    stats = torch.empty((2, N, groups), dtype=torch.float32, device=x.device)
+    ws = torch.empty((int(_lib.lib().sed_group_norm_ws_floats(N, S, C, groups, 0)),), dtype=torch.float32, device=x.device)
+    _call("sed_group_norm_fwd", _ptr(x), _ptr(weight), _ptr(bias), DTYPE_CODES[x.dtype],
+          DTYPE_CODES[weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32], N, S, C, groups, eps,
+          act, _ptr(y), stats.data_ptr(), stats.data_ptr() + 4 * N * groups, _ptr(ws), _stream())
+    return y, stats
+
+
+class GroupNormActFn(torch.autograd.Function):
+    """Parameter gradients go to autograd, not into a gradient sink: a layer may be applied several times in one pass."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        with _on_device(x):
+            y, stats = _group_norm_fwd(x, weight, bias, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, stats = ctx.saved_tensors
+        gy = gy.contiguous()
+        C, G = x.shape[-1], ctx.groups
+        N, S = x.shape[0], x.numel() // (x.shape[0] * C)
+        par = weight if weight is not None else bias
+        want = ctx.needs_input_grad
+        with _on_device(x):
+            gx = torch.empty_like(x) if want[0] else None
+            gp = torch.empty((2, C), dtype=torch.float32, device=x.device) if want[1] or want[2] else None
+            ws = torch.empty((int(_lib.lib().sed_group_norm_ws_floats(N, S, C, G, 1)),), dtype=torch.float32, device=x.device)
+            _call("sed_group_norm_bwd", _ptr(x), _ptr(gy), _ptr(weight), _ptr(bias), DTYPE_CODES[x.dtype],
+                  DTYPE_CODES[par.dtype if par is not None else torch.float32], N, S, C, G, ctx.act, stats.data_ptr(),
+                  stats.data_ptr() + 4 * N * G, _ptr(gx), gp[0].data_ptr() if want[1] else None, gp[1].data_ptr() if want[2] else None,
+                  _ptr(ws), _stream())
+            gw = gp[0].to(weight.dtype) if want[1] else None
+            gb = gp[1].to(bias.dtype) if want[2] else None
+        return gx, gw, gb, None, None, None
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
+    """y = act(weight * (x - mean) * rstd + bias) on channels-last activations x (B, ..., C): mean and rstd = 1 / sqrt(var + eps) of each
+    sample over all its positions and the C / groups channels of a group, as nn.GroupNorm on (B, C, ...).
+
+    x: float32, float16 or bfloat16 (any strides; a non-contiguous one is copied); weight, bias (C,): float32 or x's type, both the
+    same.  activation: 'none', 'relu', 'silu', 'gelu' (z Phi(z)).  Statistics and sums are held in 32 bits, y and the gradients are
+    rounded once.  Every position counts: a padded batch is normalised with its padding.  An empty x gives an empty y."""
+    act = _act_code(activation)
+    if x.dtype not in DTYPE_CODES:
+        raise ValueError("x must be float32, float16 or bfloat16, got %s" % x.dtype)
+    if x.dim() < 2:
+        raise ValueError("x must be (batch, ..., channels), got shape %s" % (tuple(x.shape),))
+    groups, C = int(groups), x.shape[-1]
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError("groups must divide the channels: %d channels, %d groups" % (C, groups))
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative, got %r" % (eps,))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _chk_operand(name, t, (C,), (torch.float32, x.dtype), x.device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must have one type, got %s and %s" % (weight.dtype, bias.dtype))
+    _chk_dev(x)
+    if x.numel() == 0:
+        y = torch.zeros_like(x)
+        for t in (x, weight, bias):                       # stays part of the graph, with gradients of zero
+            y = y if t is None or not (torch.is_grad_enabled() and t.requires_grad) else y + t.sum().to(x.dtype) * 0
+        return y
+    weight = weight if weight is None else weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    x = x.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return GroupNormActFn.apply(x, weight, bias, groups, float(eps), act)
+    with _on_device(x):
+        return _group_norm_fwd(x, weight, bias, groups, float(eps), act)[0]
+
+
 def adamw_(rows, chunks, nchunks, m, v, m_scale, v_scale, master, state_bits, hyper, step, grad_scale=1.0, guard=None, skipped=None):
     """One AdamW step over the tensors of `rows` (device int64 (tensors, 6)) in one launch: see include/sed_hip.h, sed_adamw.
     hyper: host float64 array (groups, 5).  guard (default: on while the split-f16 kernels are in use): the step is refused when a
