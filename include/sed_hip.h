@@ -498,6 +498,25 @@ int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const 
                        int C, int G, int act, const float* mean, const float* rstd, void* gx, float* gweight, float* gbias, float* ws,
                        sed_stream_t stream);
 
+/* ---- matrix product with bias, activation and residual in its epilogue -----------------------------------------------
+ * z = x W^T + b;  y = act(z) + residual:  x [M][K], weight [N][K], residual (nullable), y [M][N] of `dtype` (SED_F32 / SED_F16 /
+ * SED_BF16), bias (nullable) [N] of bdtype.  Products are summed in 32 bits and rounded once; 32-bit ones run on the fp32 matrix
+ * instructions.  z (nullable): what the backward pass needs of z, sed_linear_kept_elements(M, N) floats (SED_F32) or 16-bit values.
+ * sed_linear_bwd: gz = gy act'(z) (z nullable without an activation);  gx = gz W [M][K];  gweight = gz^T x [N][K];  gbias = sum gz [N]
+ * of bdtype; each nullable (x only serves gweight, weight only gx).  gz is rounded to `dtype` for the two products, gbias is summed
+ * before that.
+ * ws: 16-byte aligned scratch of sed_linear_*_ws_bytes bytes (0: none).  M, N, K >= 1; N, K <= 2^21.  The tensors need no more than
+ * their element's alignment; lines of a multiple of 16 bytes at 16-byte addresses are read in place, others are copied into ws first
+ * (not where M <= 64 in the forward product). */
+long sed_linear_kept_elements(long M, long N);
+long sed_linear_fwd_ws_bytes(const void* x, const void* weight, int dtype, long M, long N, long K);
+int sed_linear_fwd(const void* x, const void* weight, const void* bias, const void* residual, int dtype, int bdtype, long M, long N,
+                   long K, int act, void* y, void* z, void* ws, long ws_bytes, sed_stream_t stream);
+long sed_linear_bwd_ws_bytes(const void* x, const void* weight, const void* gy, int dtype, long M, long N, long K, int act, int gx,
+                             int gweight, int gbias);
+int sed_linear_bwd(const void* x, const void* weight, const void* gy, const void* z, int dtype, int bdtype, long M, long N, long K,
+                   int act, void* gx, void* gweight, void* gbias, void* ws, long ws_bytes, sed_stream_t stream);
+
 /* ---- AdamW over many tensors in one launch, moments in 32 or in 8 bits ------------------------------------------------
  * m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
  * rows (device): per tensor six longs {parameter address, gradient address (0: the tensor is left as it is), first element of its

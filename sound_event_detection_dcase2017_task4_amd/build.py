@@ -13,14 +13,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsed_hip.so")
 SOURCES = ["logmel.hip", "bn.hip", "conv.hip", "conv_wino2.hip", "conv_sf16.hip", "gemm_sf16.hip", "heads.hip", "attention.hip", "gru.hip",
-           "adamw.hip", "groupnorm.hip"]
+           "adamw.hip", "groupnorm.hip", "linear.hip"]
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 BASE_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-I", INCLUDE]
 # Sources compiled without packed-fp32 instructions (the compiler forms them by itself from ordinary float code, and some of their
 # operand forms return wrong values beside other kernels' MFMAs); the older sources are scanned for those forms instead
 # (tests/test_isa_audit.py), two of them are written with packed instructions of the safe form.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {"adamw.hip": NO_PACKED_FP32, "groupnorm.hip": NO_PACKED_FP32}
+SOURCE_FLAGS = {s: NO_PACKED_FP32 for s in ("adamw.hip", "groupnorm.hip", "linear.hip")}
 # SED_HIPCC_FLAGS: extra flags for kernel experiments (tools/ablate.sh, tools/experiments/*.patch).  A library built with them
 # carries a different flags hash in sed_version(), and _lib.lib() refuses it unless SED_ALLOW_EXPERIMENT=1.
 FLAGS = BASE_FLAGS + os.environ.get("SED_HIPCC_FLAGS", "").split()

@@ -1,0 +1,618 @@
+// Matrix products with bias, activation and residual in their epilogue, forward and backward, for 32- and 16-bit tensors.
+//
+//   z = x W^T + b;  y = act(z) + r          x [M][K], W [N][K], y, r [M][N]
+//   gz = gy act'(z);  gx = gz W;  gW = gz^T x;  gb = sum_m gz;  gr = gy
+//
+// All three products are out[m][n] = sum_k Q(m, k) P(n, k).  An operand lies in memory with k contiguous (x and W of the forward
+// product, gz of gx) or with its rows contiguous (W of gx, both operands of gW).  Either is staged into LDS as it lies, 16 bytes a lane
+// straight from memory, and read from there as the matrix instructions want it: 16 bytes of one row, or by transposing reads.
+// The matrix instruction takes P as its first operand: a lane then holds four consecutive n of one row m, which it can store together.
+// Products of 32-bit tensors run on the fp32 matrix instructions; sums are held in 32 bits for all types.
+#include "common.h"
+#include "sed_hip.h"
+
+SED_OBJECT_FLAGS(linear)
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef short short4t __attribute__((__vector_size__(4 * sizeof(short))));
+typedef short short8t __attribute__((ext_vector_type(8)));
+
+constexpr unsigned OUTSIDE = 0x80000000u;          // a byte offset behind every descriptor: such a lane receives zeros
+
+struct Epilogue {
+    const void* bias;                              // nullable, [N]
+    const void* res;                               // nullable, [M][N]
+    void* y;                                       // [M][N]
+    void* z;                                       // nullable: what the backward pass needs of z, [M][ldz]
+    long ldz;
+    int btype, act, wide;                          // wide: y and res can be accessed four elements at a time
+};
+
+__device__ __forceinline__ float load_typed(const void* p, int type, long i) {
+    if (type == SED_F32) return reinterpret_cast<const float*>(p)[i];
+    if (type == SED_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+    return (float)reinterpret_cast<const __bf16*>(p)[i];
+}
+__device__ __forceinline__ void store_typed(void* p, int type, long i, float v) {
+    if (type == SED_F32) reinterpret_cast<float*>(p)[i] = v;
+    else if (type == SED_F16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
+    else reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
+}
+
+// What is kept of z for the backward pass, which reads nothing but act'(z) from it.  16-bit tensors keep it as float16 whatever
+// their type: its 11 bits lose a sixteenth of what gz loses when it is rounded to bfloat16, and beyond +-60000 every derivative has
+// long been 0 or 1.  ReLU keeps 1 or 0, so that a z below the smallest float16 is not lost.
+template <typename T> struct Kept { typedef _Float16 type; };
+template <> struct Kept<float> { typedef float type; };
+template <typename T> __device__ __forceinline__ typename Kept<T>::type keep_z(float z, int act) {
+    if (act == SED_ACT_RELU) return (typename Kept<T>::type)(z > 0.f ? 1.f : 0.f);
+    if (sizeof(T) == 4) return (typename Kept<T>::type)z;
+    return (typename Kept<T>::type)(z > 60000.f ? 60000.f : (z < -60000.f ? -60000.f : z));
+}
+__device__ __forceinline__ float act_of(float z, int act) {
+    switch (act) {
+        case SED_ACT_RELU: return sed_act<1>(z);
+        case SED_ACT_SILU: return sed_act<2>(z);
+        case SED_ACT_GELU: return sed_act<3>(z);
+    }
+    return z;
+}
+
+template <typename T> struct Quad { typedef T type __attribute__((ext_vector_type(4))); };
+
+// four consecutive columns of row m
+template <typename T> __device__ __forceinline__ void finish(const Epilogue& e, long m, int n, int N, floatx4 v, floatx4 bias) {
+    typedef typename Quad<T>::type T4;
+    typedef typename Kept<T>::type Z;
+    v += bias;
+    if (e.z) {
+        typename Quad<Z>::type k;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) k[r] = keep_z<T>(v[r], e.act);
+        *reinterpret_cast<typename Quad<Z>::type*>(reinterpret_cast<Z*>(e.z) + m * e.ldz + n) = k;      // ldz is a multiple of 8
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = act_of(v[r], e.act);
+    T* const y = reinterpret_cast<T*>(e.y) + m * N + n;
+    const T* const res = e.res ? reinterpret_cast<const T*>(e.res) + m * N + n : nullptr;
+    if (e.wide) {
+        if (res) {
+            const T4 q = *reinterpret_cast<const T4*>(res);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += (float)q[r];
+        }
+        T4 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
+        *reinterpret_cast<T4*>(y) = o;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < N) y[r] = (T)(v[r] + (res ? (float)res[r] : 0.f));
+    }
+}
+__device__ __forceinline__ floatx4 bias4(const Epilogue& e, int n, int N) {
+    floatx4 b = {0.f, 0.f, 0.f, 0.f};
+    if (e.bias)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < N) b[r] = load_typed(e.bias, e.btype, n + r);
+    return b;
+}
+
+// ---- 16 bytes of k of 16 rows: one instruction in 16 bits, four in 32 (they take the k of a lane in any order, as long as P and Q agree)
+template <typename T> struct Frag;
+template <> struct Frag<_Float16> { typedef half8 type; };
+template <> struct Frag<__bf16> { typedef bf8 type; };
+template <> struct Frag<float> { typedef floatx4 type; };
+__device__ __forceinline__ floatx4 mma(half8 p, half8 q, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, c, 0, 0, 0); }
+__device__ __forceinline__ floatx4 mma(bf8 p, bf8 q, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, q, c, 0, 0, 0); }
+__device__ __forceinline__ floatx4 mma(floatx4 p, floatx4 q, floatx4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[j], q[j], c, 0, 0, 0);
+    return c;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- tiles
+// A step takes 128 bytes of k: 64 elements in 16 bits, 32 in 32.  One operand's tile of R rows is R * 128 bytes.
+//   k contiguous: [R][128 bytes]; 16-byte piece c of row r lies at place c ^ (r & 7).
+//   rows contiguous: [steps of k][R elements]; piece c of line k lies at place c ^ swizzle(k), so that the lines of one transposing read
+//   lie in different banks.
+struct Operand {
+    const void* base;
+    long ld;                                       // elements from one line to the next
+    int rows;                                      // rows (m or n)
+};
+struct GemmP {
+    Operand p, q;
+    int M, N;
+    long K;
+    long kslice;                                   // k of one slice, a multiple of the step
+    int tm, tn;                                    // tiles
+    float* part;                                   // [slices][M][ldp] where the product is cut along k
+    long ldp;
+    Epilogue e;
+};
+
+template <typename T, int R, bool ROWS, int THREADS> struct Stage {
+    static constexpr int E = 16 / sizeof(T), STEP = 128 / sizeof(T), PIECES = R * 8, PER = PIECES / THREADS;
+    static constexpr int LINE = ROWS ? R / E : 8;            // pieces in a line
+    __device__ __forceinline__ static int swizzle(int line) {
+        if (!ROWS) return line & 7;
+        return sizeof(T) == 2 ? 2 * ((line & 3) + 4 * ((line >> 3) & 1)) : 4 * ((line >> 2) & 3);
+    }
+    // byte offset of this lane's i-th piece from the tile's first element, OUTSIDE where its row does not exist
+    __device__ __forceinline__ static void offsets(const Operand& o, int row0, unsigned (&off)[PER]) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int slot = i * THREADS + threadIdx.x, line = slot / LINE, c = (slot % LINE) ^ swizzle(line);
+            const bool ok = ROWS ? row0 + c * E < o.rows : row0 + line < o.rows;
+            off[i] = ok ? (unsigned)(line * o.ld * (long)sizeof(T)) + c * 16 : OUTSIDE;
+        }
+    }
+    __device__ __forceinline__ static void load(const Operand& o, int row0, long k0, long K, const unsigned (&off)[PER], unsigned char* lds) {
+        const T* const at = reinterpret_cast<const T*>(o.base) + (ROWS ? k0 * o.ld + row0 : row0 * o.ld + k0);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(at), 0, 0x7fffffff, 0x00020000);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const bool whole = k0 + STEP <= K;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            unsigned v = off[i];
+            if (!whole) {
+                const int slot = i * THREADS + threadIdx.x, line = slot / LINE, c = (slot % LINE) ^ swizzle(line);
+                if (k0 + (ROWS ? line : c * E) >= K) v = OUTSIDE;
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (i * THREADS + wave * 64) * 16), 16, (int)v, 0, 0, 0);
+        }
+    }
+    // 16 rows from `row` on, the kk-th half of the step's k
+    __device__ __forceinline__ static typename Frag<T>::type frag(const unsigned char* lds, int row, int kk) {
+        typedef typename Frag<T>::type Fr;
+        const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+        if constexpr (!ROWS) {
+            const int r = row + l;
+            return *reinterpret_cast<const Fr*>(lds + r * 128 + (((kk * 4 + g) ^ swizzle(r)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            const int k = kk * 32 + 8 * g + (l >> 2), c = row + (l & 3) * 4;
+            const unsigned char* const at = lds + k * (R * 2) + (((c >> 3) ^ swizzle(k)) << 4) + (c & 7) * 2;
+            typedef __attribute__((address_space(3))) short4t* L;
+            const short4t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L)(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L)(at + 4 * (R * 2)));
+            return __builtin_bit_cast(Fr, short8t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+        } else {
+            Fr f;
+            const int c = row + l;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = kk * 16 + 4 * g + j;
+                f[j] = *reinterpret_cast<const float*>(lds + k * (R * 4) + (((c >> 2) ^ swizzle(k)) << 4) + (c & 3) * 4);
+            }
+            return f;
+        }
+    }
+};
+
+__device__ __forceinline__ int xcd_spread(int bid, int nblk) {       // neighbours in the result are on one XCD and share its L2
+    const int q = nblk >> 3, r = nblk & 7, xcd = bid & 7;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+}
+
+template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmP a) {
+    constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
+    typedef Stage<T, BN, PROWS, THREADS> SP;
+    typedef Stage<T, BM, QROWS, THREADS> SQ;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2][(BM + BN) * 128];
+    const int tiles = a.tm * a.tn, id = xcd_spread(blockIdx.x, gridDim.x);
+    const int slice = id / tiles, tile = id % tiles;
+    const int m0 = (tile % a.tm) * BM, n0 = (tile / a.tm) * BN;
+    const long k0 = slice * a.kslice, k1 = CUT ? min(a.K, k0 + a.kslice) : a.K;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    unsigned poff[SP::PER], qoff[SQ::PER];
+    SP::offsets(a.p, n0, poff);
+    SQ::offsets(a.q, m0, qoff);
+    floatx4 acc[MI][NI] = {};
+    SP::load(a.p, n0, k0, k1, poff, lds[0]);
+    SQ::load(a.q, m0, k0, k1, qoff, lds[0] + BN * 128);
+    __syncthreads();
+    int cur = 0;
+    for (long k = k0; k < k1; k += SP::STEP, cur ^= 1) {
+        if (k + SP::STEP < k1) {
+            SP::load(a.p, n0, k + SP::STEP, k1, poff, lds[cur ^ 1]);
+            SQ::load(a.q, m0, k + SP::STEP, k1, qoff, lds[cur ^ 1] + BN * 128);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            typename Frag<T>::type p[NI], q[MI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) p[i] = SP::frag(lds[cur], wn + 16 * i, kk);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) q[i] = SQ::frag(lds[cur] + BN * 128, wm + 16 * i, kk);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = mma(p[j], q[i], acc[i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
+        if (n >= a.N) continue;
+        const floatx4 b = CUT ? floatx4{0.f, 0.f, 0.f, 0.f} : bias4(a.e, n, a.N);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m0 + wm + 16 * i + (lane & 15);
+            if (m >= a.M) continue;
+            if (CUT) *reinterpret_cast<floatx4*>(a.part + ((long)slice * a.M + m) * a.ldp + n) = acc[i][j];      // ldp is a multiple of 4
+            else finish<T>(a.e, m, n, a.N, acc[i][j], b);
+        }
+    }
+}
+
+// the slices of a cut product, added in order, and the epilogue
+template <typename T> __global__ __launch_bounds__(256) void join_kernel(const float* part, int slices, int M, int N, long ldp, Epilogue e) {
+    const long quads = ldp / 4, total = quads * M;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long m = i / quads;
+        const int n = (int)(i % quads) * 4;
+        floatx4 v = *reinterpret_cast<const floatx4*>(part + m * ldp + n);
+        for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const floatx4*>(part + ((long)s * M + m) * ldp + n);
+        finish<T>(e, m, n, N, v, bias4(e, n, N));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few rows
+// Up to 16 * MT rows of x: the product is a pass over W.  A workgroup owns 16 rows of W, its waves split k, 64 bytes a row and
+// instruction; the waves' sums are added through LDS.  No alignment is asked of x and W.
+template <typename T> __device__ __forceinline__ typename Frag<T>::type piece(const T* row, long k, long K, bool ok) {
+    constexpr int E = 16 / sizeof(T);
+    typename Frag<T>::type f;
+    if (ok && k + E <= K) {
+        __builtin_memcpy(&f, row + k, 16);
+        return f;
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = ok && k + j < K ? row[k + j] : (T)0.f;
+    return f;
+}
+template <typename T, int MT> __global__ __launch_bounds__(512) void rows_kernel(const T* x, const T* w, int M, int N, long K, Epilogue e) {
+    constexpr int E = 16 / sizeof(T), U = 2;
+    __shared__ __attribute__((aligned(16))) floatx4 sums[8][MT][64];
+    const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const bool pn = n0 + l < N;
+    const T* const wr = w + (long)(pn ? n0 + l : 0) * K;
+    const T* xr[MT];
+    bool pm[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        pm[i] = i * 16 + l < M;
+        xr[i] = x + (long)(pm[i] ? i * 16 + l : 0) * K;
+    }
+    floatx4 acc[MT] = {};
+    for (long k = (long)wave * 4 * E * U; k < K; k += (long)waves * 4 * E * U) {
+        typename Frag<T>::type p[U], q[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            p[u] = piece<T>(wr, k + (u * 4 + g) * E, K, pn);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) q[u][i] = piece<T>(xr[i], k + (u * 4 + g) * E, K, pm[i]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mma(p[u], q[u][i], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < MT; i += waves) {
+        floatx4 v = sums[0][i][lane];
+        for (int s = 1; s < waves; ++s) v += sums[s][i][lane];
+        const int m = i * 16 + l, n = n0 + 4 * g;
+        if (m < M && n < N) finish<T>(e, m, n, N, v, bias4(e, n, N));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- passes around them
+// copy of [R][C] with lines of ld elements, zeros behind the C-th: operands whose lines do not begin at multiples of 16 bytes
+template <typename T> __global__ __launch_bounds__(256) void pad_kernel(const T* src, long R, int C, int ld, T* dst) {
+    constexpr int E = 16 / sizeof(T);
+    const int per = ld / E;
+    const long total = R * per;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long r = i / per;
+        const int c = (int)(i % per) * E;
+        T v[E];
+        if (c + E <= C) __builtin_memcpy(v, src + r * C + c, 16);
+        else
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = c + j < C ? src[r * C + c + j] : (T)0.f;
+        __builtin_memcpy(dst + r * ld + c, v, 16);
+    }
+}
+
+// gz [M][ld] = gy act'(z) (null: only the sums) and per chunk of rows the column sums of gz in 32 bits, before it is rounded.
+// A thread owns E columns (16 bytes) of every RT-th row of a chunk.
+struct GradP {
+    const void* gy;
+    const void* z;                                 // null: no activation
+    void* gz;
+    float* sums;                                   // nullable, [chunks][ld]
+    long M, rows;
+    int N, ld, CT, RT, tiles, act;
+};
+template <typename T> __device__ __forceinline__ float act_grad_of(float z, int act) {
+    switch (act) {
+        case SED_ACT_RELU: return z;               // kept as 0 or 1
+        case SED_ACT_SILU: return sed_act_grad<2>(z);
+        case SED_ACT_GELU: return sed_act_grad<3>(z);
+    }
+    return 1.f;
+}
+template <typename T> __global__ __launch_bounds__(256) void act_grad_kernel(GradP p) {
+    constexpr int E = 16 / sizeof(T);
+    typedef typename Kept<T>::type Z;
+    __shared__ float red[256 * E];
+    const int tile = (int)(blockIdx.x % p.tiles), t = threadIdx.x, col = tile * p.CT + t % p.CT, r = t / p.CT, c = col * E;
+    const long chunk = blockIdx.x / p.tiles, s0 = chunk * p.rows, s1 = min(p.M, s0 + p.rows);
+    float sum[E] = {};
+    if (r < p.RT && c < p.ld)
+        for (long s = s0 + r; s < s1; s += p.RT) {
+            T g[E];
+            if (c + E <= p.N) __builtin_memcpy(g, reinterpret_cast<const T*>(p.gy) + s * p.N + c, 16);
+            else
+#pragma unroll
+                for (int j = 0; j < E; ++j) g[j] = c + j < p.N ? reinterpret_cast<const T*>(p.gy)[s * p.N + c + j] : (T)0.f;
+            float f[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) f[j] = (float)g[j];
+            if (p.z) {
+                Z z[E];
+                __builtin_memcpy(z, reinterpret_cast<const Z*>(p.z) + s * p.ld + c, sizeof(z));
+#pragma unroll
+                for (int j = 0; j < E; ++j) f[j] = c + j < p.N ? f[j] * act_grad_of<T>((float)z[j], p.act) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                sum[j] += f[j];
+                g[j] = (T)f[j];
+            }
+            if (p.gz) __builtin_memcpy(reinterpret_cast<T*>(p.gz) + s * p.ld + c, g, 16);
+        }
+    if (!p.sums) return;
+#pragma unroll
+    for (int j = 0; j < E; ++j) red[t * E + j] = sum[j];
+    __syncthreads();
+    for (int k = t; k < p.CT * E; k += 256) {
+        float v = 0.f;
+        for (int i = 0; i < p.RT; ++i) v += red[i * p.CT * E + k];
+        const int n = tile * p.CT * E + k;
+        if (n < p.ld) p.sums[chunk * p.ld + n] = v;
+    }
+}
+// gb [N] of `type` = the column sums of sums [chunks][ld]: 16 columns x 16 lanes
+__global__ __launch_bounds__(256) void column_sums_kernel(const float* sums, long chunks, int ld, int N, void* gb, int type) {
+    __shared__ float red[16][17];
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
+    float v = 0.f;
+    if (c < N)
+        for (long i = row; i < chunks; i += 16) v += sums[i * ld + c];
+    red[row][lane] = v;
+    __syncthreads();
+    if (row == 0 && c < N) {
+        for (int k = 1; k < 16; ++k) v += red[k][lane];
+        store_typed(gb, type, c, v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
+long padded(long n, int esize) { return (n + 16 / esize - 1) / (16 / esize) * (16 / esize); }
+long up256(long bytes) { return (bytes + 255) / 256 * 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool needs_pad(const void* p, long ld, int esize) { return !aligned16(p) || ld % (16 / esize); }
+
+constexpr int BM = 128, BN = 128;
+// how often the product is cut along k: into as many slices as leave every CU two workgroups, of at least eight steps each
+struct Plan {
+    int tm, tn, slices;
+    long kslice, part_bytes, ldp;
+};
+Plan plan_of(long M, long N, long K, int esize) {
+    Plan q;
+    q.tm = sed_cdiv(M, BM);
+    q.tn = sed_cdiv(N, BN);
+    const long step = 128 / esize, steps = (K + step - 1) / step, tiles = (long)q.tm * q.tn;
+    long s = 512 / tiles;
+    if (s > steps / 8) s = steps / 8;
+    if (s < 1) s = 1;
+    const long per = (steps + s - 1) / s;
+    q.slices = (int)((steps + per - 1) / per);
+    q.kslice = per * step;
+    q.ldp = (N + 3) / 4 * 4;
+    q.part_bytes = q.slices > 1 ? up256(q.slices * M * q.ldp * 4) : 0;
+    return q;
+}
+bool few_rows(long M) { return M <= 64; }
+
+template <typename T, bool PROWS, bool QROWS> int launch_gemm(GemmP a, const Plan& q, float* part, hipStream_t stream) {
+    a.tm = q.tm; a.tn = q.tn; a.kslice = q.kslice; a.part = part; a.ldp = q.ldp;
+    const dim3 grid((unsigned)((long)q.tm * q.tn * q.slices));
+    if (q.slices > 1) {
+        hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, BM, BN, 2, 2, true>), grid, dim3(256), 0, stream, a);
+        const long quads = q.ldp / 4 * a.M, nb = (quads + 255) / 256;
+        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(nb > 8192 ? 8192 : nb)), dim3(256), 0, stream, part, q.slices, a.M, a.N, q.ldp, a.e);
+    } else {
+        hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, BM, BN, 2, 2, false>), grid, dim3(256), 0, stream, a);
+    }
+    SED_LAUNCH_CHECK();
+    return 0;
+}
+template <typename T> const T* pad(const void* src, long R, long C, char*& ws, hipStream_t stream) {
+    const int ld = (int)padded(C, sizeof(T));
+    T* const dst = reinterpret_cast<T*>(ws);
+    ws += up256(R * ld * (long)sizeof(T));
+    const long total = R * (ld * (long)sizeof(T) / 16), nb = (total + 255) / 256;
+    hipLaunchKernelGGL((pad_kernel<T>), dim3((unsigned)(nb > 16384 ? 16384 : nb)), dim3(256), 0, stream, reinterpret_cast<const T*>(src), R, (int)C, ld, dst);
+    return dst;
+}
+
+// rows and columns that 32-bit tile counts and 32-bit offsets inside a tile can hold
+bool bad_shape(int dtype, long M, long N, long K, int act) {
+    return dtype < 0 || dtype > 2 || M < 1 || N < 1 || K < 1 || M > 0x7fffffffL - 256 || N > 1L << 21 || K > 1L << 21 || act < 0 || act > 3 ||
+           (M + 127) / 128 * ((N + 127) / 128) > 1L << 30 || (M + 127) / 128 * ((K + 127) / 128) > 1L << 30;
+}
+
+struct GradCut {
+    int CT, RT, tiles;
+    long rows, chunks;
+};
+GradCut grad_cut(long M, long ld, int esize) {
+    GradCut c;
+    const long cols = ld * esize / 16;
+    c.CT = (int)(cols < 256 ? cols : 256);
+    c.RT = 256 / c.CT;
+    c.tiles = (int)((cols + c.CT - 1) / c.CT);
+    const long want = (2048 + c.tiles - 1) / c.tiles;
+    long rows = (M + want - 1) / want;
+    const long lo = (long)c.RT * 4, hi = (long)c.RT * 64;
+    rows = rows < lo ? lo : (rows > hi ? hi : rows);
+    c.rows = rows;
+    c.chunks = (M + rows - 1) / rows;
+    return c;
+}
+
+template <typename T>
+int linear_fwd(const void* x, const void* w, const void* bias, const void* res, int btype, long M, long N, long K, int act, void* y, void* z,
+               char* ws, hipStream_t stream) {
+    Epilogue e{bias, res, y, z, padded(N, sizeof(T)), btype, act, 0};
+    e.wide = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(res)) % (4 * sizeof(T)) == 0;
+    if (few_rows(M)) {
+        const long steps = (K + 128 / (long)sizeof(T) - 1) / (128 / (long)sizeof(T));
+        const dim3 grid((unsigned)sed_cdiv(N, 16)), block((unsigned)(64 * (steps < 8 ? steps : 8)));
+        const T *xt = reinterpret_cast<const T*>(x), *wt = reinterpret_cast<const T*>(w);
+        if (M <= 16) hipLaunchKernelGGL((rows_kernel<T, 1>), grid, block, 0, stream, xt, wt, (int)M, (int)N, K, e);
+        else if (M <= 32) hipLaunchKernelGGL((rows_kernel<T, 2>), grid, block, 0, stream, xt, wt, (int)M, (int)N, K, e);
+        else hipLaunchKernelGGL((rows_kernel<T, 4>), grid, block, 0, stream, xt, wt, (int)M, (int)N, K, e);
+        SED_LAUNCH_CHECK();
+        return 0;
+    }
+    const long ld = padded(K, sizeof(T));
+    const bool px = needs_pad(x, K, sizeof(T)), pw = needs_pad(w, K, sizeof(T));
+    GemmP a{};
+    a.M = (int)M; a.N = (int)N; a.K = ld; a.e = e;
+    a.q = {px ? pad<T>(x, M, K, ws, stream) : x, ld, (int)M};
+    a.p = {pw ? pad<T>(w, N, K, ws, stream) : w, ld, (int)N};
+    return launch_gemm<T, false, false>(a, plan_of(M, N, ld, sizeof(T)), reinterpret_cast<float*>(ws), stream);
+}
+
+long fwd_ws(const void* x, const void* w, int esize, long M, long N, long K) {
+    if (few_rows(M)) return 0;
+    const long ld = padded(K, esize);
+    return (needs_pad(x, K, esize) ? up256(M * ld * esize) : 0) + (needs_pad(w, K, esize) ? up256(N * ld * esize) : 0) + plan_of(M, N, ld, esize).part_bytes;
+}
+
+struct BwdNeeds {
+    bool gz, px, pw;
+};
+BwdNeeds bwd_needs(const void* x, const void* w, const void* gy, int esize, long N, long K, int act, bool gx, bool gw) {
+    return {(gx || gw) && (act != SED_ACT_NONE || needs_pad(gy, N, esize)), gw && needs_pad(x, K, esize), gx && needs_pad(w, K, esize)};
+}
+long bwd_ws(const void* x, const void* w, const void* gy, int esize, long M, long N, long K, int act, bool gx, bool gw, bool gb) {
+    const BwdNeeds d = bwd_needs(x, w, gy, esize, N, K, act, gx, gw);
+    const long ldn = padded(N, esize), ldk = padded(K, esize);
+    long b = (d.gz ? up256(M * ldn * esize) : 0) + (d.px ? up256(M * ldk * esize) : 0) + (d.pw ? up256(N * ldk * esize) : 0);
+    if (gb) b += up256(grad_cut(M, ldn, esize).chunks * ldn * 4);
+    const long px = gx ? plan_of(M, K, ldn, esize).part_bytes : 0, pw = gw ? plan_of(N, K, M, esize).part_bytes : 0;
+    return b + (px > pw ? px : pw);
+}
+
+template <typename T>
+int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int btype, long M, long N, long K, int act, void* gx, void* gw, void* gb,
+               char* ws, hipStream_t stream) {
+    const int es = sizeof(T);
+    const BwdNeeds d = bwd_needs(x, w, gy, es, N, K, act, gx != nullptr, gw != nullptr);
+    const long ldn = padded(N, es), ldk = padded(K, es);
+    const GradCut c = grad_cut(M, ldn, es);
+    T* gz = nullptr;
+    if (d.gz) {
+        gz = reinterpret_cast<T*>(ws);
+        ws += up256(M * ldn * es);
+    }
+    float* sums = nullptr;
+    if (gb) {
+        sums = reinterpret_cast<float*>(ws);
+        ws += up256(c.chunks * ldn * 4);
+    }
+    if (gz || gb) {
+        GradP p{gy, act == SED_ACT_NONE ? nullptr : z, gz, sums, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act};
+        hipLaunchKernelGGL((act_grad_kernel<T>), dim3((unsigned)(c.chunks * c.tiles)), dim3(256), 0, stream, p);
+    }
+    if (gb) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(256), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
+    const void* const dz = gz ? gz : gy;
+    const void* const xp = d.px ? pad<T>(x, M, K, ws, stream) : x;
+    const void* const wp = d.pw ? pad<T>(w, N, K, ws, stream) : w;
+    SED_LAUNCH_CHECK();
+    const bool wide = K % 4 == 0;
+    if (gx) {
+        GemmP a{};
+        a.M = (int)M; a.N = (int)K; a.K = ldn;
+        a.e.y = gx; a.e.wide = wide && reinterpret_cast<uintptr_t>(gx) % (4 * es) == 0;
+        a.q = {dz, ldn, (int)M};
+        a.p = {wp, ldk, (int)ldk};
+        // gz has zeros behind its N-th column, W has no line there: k ends at N for W's lines and at ldn for gz's pieces
+        a.K = N;
+        const int rc = launch_gemm<T, true, false>(a, plan_of(M, K, ldn, es), reinterpret_cast<float*>(ws), stream);
+        if (rc) return rc;
+    }
+    if (gw) {
+        GemmP a{};
+        a.M = (int)N; a.N = (int)K; a.K = M;
+        a.e.y = gw; a.e.wide = wide && reinterpret_cast<uintptr_t>(gw) % (4 * es) == 0;
+        a.q = {dz, ldn, (int)ldn};
+        a.p = {xp, ldk, (int)ldk};
+        return launch_gemm<T, true, true>(a, plan_of(N, K, M, es), reinterpret_cast<float*>(ws), stream);
+    }
+    return 0;
+}
+
+}  // namespace
+
+SED_API long sed_linear_kept_elements(long M, long N) { return M < 1 || N < 1 ? 0 : M * padded(N, 2); }
+
+SED_API long sed_linear_fwd_ws_bytes(const void* x, const void* w, int dtype, long M, long N, long K) {
+    return bad_shape(dtype, M, N, K, 0) ? 0 : fwd_ws(x, w, esize_of(dtype), M, N, K);
+}
+
+SED_API int sed_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int dtype, int bdtype, long M, long N,
+                           long K, int act, void* y, void* z, void* ws, long ws_bytes, sed_stream_t stream) {
+    if (!x || !w || !y || bdtype < 0 || bdtype > 2 || bad_shape(dtype, M, N, K, act)) return SED_EINVAL;
+    const long need = fwd_ws(x, w, esize_of(dtype), M, N, K);
+    if (need && (!ws || ws_bytes < need || !aligned16(ws))) return SED_EINVAL;
+    char* const s = reinterpret_cast<char*>(ws);
+    if (dtype == SED_F32) return linear_fwd<float>(x, w, bias, residual, bdtype, M, N, K, act, y, z, s, stream);
+    if (dtype == SED_F16) return linear_fwd<_Float16>(x, w, bias, residual, bdtype, M, N, K, act, y, z, s, stream);
+    return linear_fwd<__bf16>(x, w, bias, residual, bdtype, M, N, K, act, y, z, s, stream);
+}
+
+SED_API long sed_linear_bwd_ws_bytes(const void* x, const void* w, const void* gy, int dtype, long M, long N, long K, int act, int gx,
+                                     int gw, int gb) {
+    return bad_shape(dtype, M, N, K, act) ? 0 : bwd_ws(x, w, gy, esize_of(dtype), M, N, K, act, gx, gw, gb);
+}
+
+SED_API int sed_linear_bwd(const void* x, const void* w, const void* gy, const void* z, int dtype, int bdtype, long M, long N, long K,
+                           int act, void* gx, void* gw, void* gb, void* ws, long ws_bytes, sed_stream_t stream) {
+    if (!gy || (gw && !x) || (gx && !w) || (act != SED_ACT_NONE && !z) || bdtype < 0 || bdtype > 2 || bad_shape(dtype, M, N, K, act)) return SED_EINVAL;
+    const long need = bwd_ws(x, w, gy, esize_of(dtype), M, N, K, act, gx, gw, gb);
+    if (need && (!ws || ws_bytes < need || !aligned16(ws))) return SED_EINVAL;
+    char* const s = reinterpret_cast<char*>(ws);
+    if (dtype == SED_F32) return linear_bwd<float>(x, w, gy, z, bdtype, M, N, K, act, gx, gw, gb, s, stream);
+    if (dtype == SED_F16) return linear_bwd<_Float16>(x, w, gy, z, bdtype, M, N, K, act, gx, gw, gb, s, stream);
+    return linear_bwd<__bf16>(x, w, gy, z, bdtype, M, N, K, act, gx, gw, gb, s, stream);
+}

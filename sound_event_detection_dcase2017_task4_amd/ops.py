@@ -2059,6 +2059,88 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         return _group_norm_fwd(x, weight, bias, groups, float(eps), act)[0]
 
 
+def _linear_fwd(x, weight, bias, residual, act, keep):
+    """x (M, K), all contiguous -> y (M, N) and, with keep, what the backward pass needs of z (None without an activation)."""
+    (M, K), N, dt = x.shape, weight.shape[0], DTYPE_CODES[x.dtype]
+    h = _lib.lib()
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    z = None
+    if keep and act:
+        z = torch.empty((int(h.sed_linear_kept_elements(M, N)),), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device)
+    need = int(h.sed_linear_fwd_ws_bytes(_ptr(x), _ptr(weight), dt, M, N, K))
+    ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+    _call("sed_linear_fwd", _ptr(x), _ptr(weight), _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt,
+          M, N, K, act, _ptr(y), _ptr(z), _ptr(ws), need, _stream())
+    return y, z
+
+
+class LinearActFn(torch.autograd.Function):
+    """Parameter gradients go to autograd, not into a gradient sink: a layer may be applied several times in one pass."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        with _on_device(x):
+            y, z = _linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, z)
+        ctx.act, ctx.btype = act, bias.dtype if bias is not None else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, z = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        gx = gw = gb = None
+        if any(want[:3]):
+            g = gy.contiguous()
+            (M, K), N, dt = x.shape, weight.shape[0], DTYPE_CODES[x.dtype]
+            h = _lib.lib()
+            with _on_device(x):
+                gx = torch.empty_like(x) if want[0] else None
+                gw = torch.empty_like(weight) if want[1] else None
+                gb = torch.empty((N,), dtype=ctx.btype, device=x.device) if want[2] else None
+                need = int(h.sed_linear_bwd_ws_bytes(_ptr(x), _ptr(weight), _ptr(g), dt, M, N, K, ctx.act, want[0], want[1], want[2]))
+                ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+                _call("sed_linear_bwd", _ptr(x), _ptr(weight), _ptr(g), _ptr(z), dt, DTYPE_CODES[ctx.btype] if want[2] else dt, M, N, K,
+                      ctx.act, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), need, _stream())
+        return gx, gw, gb, gy if want[3] else None, None
+
+
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """y = act(x W^T + b) + residual in one product: x (..., K), weight (N, K), bias (N,), residual and y (..., N).
+
+    x, weight and residual: float32, float16 or bfloat16, all of one type (any strides; non-contiguous ones are copied); bias: that
+    type or float32.  activation: 'none', 'relu', 'silu', 'gelu' (z Phi(z)).  Sums are held in 32 bits and y is rounded once; the
+    backward pass rounds gz = gy act'(z) to x's type for its two products.  Up to 64 rows the product is one pass over W (single
+    frames of a stream); an x without rows gives a y without rows."""
+    act = _act_code(activation)
+    if x.dtype not in DTYPE_CODES:
+        raise ValueError("x must be float32, float16 or bfloat16, got %s" % x.dtype)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError("x (..., K) and weight (N, K) do not fit: %s and %s" % (tuple(x.shape), tuple(weight.shape)))
+    N, K = weight.shape
+    shape = tuple(x.shape[:-1]) + (N,)
+    _chk_operand("weight", weight, (N, K), (x.dtype,), x.device)
+    if bias is not None:
+        _chk_operand("bias", bias, (N,), (x.dtype, torch.float32), x.device)
+    if residual is not None:
+        _chk_operand("residual", residual, shape, (x.dtype,), x.device)
+    _chk_dev(x)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    if x.numel() == 0:
+        y = torch.zeros(shape, dtype=x.dtype, device=x.device)
+        for t in (x, weight, bias, residual):             # stays part of the graph, with gradients of zero
+            y = y + t.sum().to(x.dtype) * 0 if grad and t is not None and t.requires_grad else y
+        return y
+    x2, weight = x.contiguous().view(-1, K), weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    r2 = residual if residual is None else residual.contiguous().view(-1, N)
+    if grad:
+        return LinearActFn.apply(x2, weight, bias, r2, act).view(shape)
+    with _on_device(x):
+        return _linear_fwd(x2, weight, bias, r2, act, False)[0].view(shape)
+
+
 def adamw_(rows, chunks, nchunks, m, v, m_scale, v_scale, master, state_bits, hyper, step, grad_scale=1.0, guard=None, skipped=None):
     """One AdamW step over the tensors of `rows` (device int64 (tensors, 6)) in one launch: see include/sed_hip.h, sed_adamw.
     hyper: host float64 array (groups, 5).  guard (default: on while the split-f16 kernels are in use): the step is refused when a
