@@ -10,6 +10,7 @@
 // Products of 32-bit tensors run on the fp32 matrix instructions; sums are held in 32 bits for all types.
 #include "common.h"
 #include "sed_hip.h"
+#include <stdlib.h>
 
 SED_OBJECT_FLAGS(linear)
 
@@ -20,6 +21,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short short4t __attribute__((__vector_size__(4 * sizeof(short))));
 typedef short short8t __attribute__((ext_vector_type(8)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 
 constexpr unsigned OUTSIDE = 0x80000000u;          // a byte offset behind every descriptor: such a lane receives zeros
 
@@ -29,7 +31,7 @@ struct Epilogue {
     void* y;                                       // [M][N]
     void* z;                                       // nullable: what the backward pass needs of z, [M][ldz]
     long ldz;
-    int btype, act, wide;                          // wide: y and res can be accessed four elements at a time
+    int btype, act, wide, bwide;                   // wide: y and res can be accessed 16 bytes at a time; bwide: the bias too
 };
 
 __device__ __forceinline__ float load_typed(const void* p, int type, long i) {
@@ -62,53 +64,71 @@ __device__ __forceinline__ float act_of(float z, int act) {
     return z;
 }
 
-template <typename T> struct Quad { typedef T type __attribute__((ext_vector_type(4))); };
+template <typename T> struct Type { static constexpr int code = SED_F32; };
+template <> struct Type<_Float16> { static constexpr int code = SED_F16; };
+template <> struct Type<__bf16> { static constexpr int code = SED_BF16; };
+template <typename T, int V> struct Wide { typedef T type __attribute__((ext_vector_type(V))); };
+constexpr int RUNTIME = -1;                        // an activation that is not known to the compiler
 
-// four consecutive columns of row m
-template <typename T> __device__ __forceinline__ void finish(const Epilogue& e, long m, int n, int N, floatx4 v, floatx4 bias) {
-    typedef typename Quad<T>::type T4;
-    typedef typename Kept<T>::type Z;
-    v += bias;
-    if (e.z) {
-        typename Quad<Z>::type k;
+// V consecutive columns of row m, n a multiple of V: the residual, and everything behind it (v = z - bias)
+template <typename T, int V> __device__ __forceinline__ void load_residual(const Epilogue& e, long m, int n, int N, float (&r)[V]) {
+    const T* const at = reinterpret_cast<const T*>(e.res) + m * N + n;
+    if (!e.res) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) k[r] = keep_z<T>(v[r], e.act);
-        *reinterpret_cast<typename Quad<Z>::type*>(reinterpret_cast<Z*>(e.z) + m * e.ldz + n) = k;      // ldz is a multiple of 8
-    }
+        for (int j = 0; j < V; ++j) r[j] = 0.f;
+    } else if (e.wide) {
+        const auto q = *reinterpret_cast<const typename Wide<T, V>::type*>(at);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = act_of(v[r], e.act);
-    T* const y = reinterpret_cast<T*>(e.y) + m * N + n;
-    const T* const res = e.res ? reinterpret_cast<const T*>(e.res) + m * N + n : nullptr;
-    if (e.wide) {
-        if (res) {
-            const T4 q = *reinterpret_cast<const T4*>(res);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += (float)q[r];
-        }
-        T4 o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
-        *reinterpret_cast<T4*>(y) = o;
+        for (int j = 0; j < V; ++j) r[j] = (float)q[j];
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < N) y[r] = (T)(v[r] + (res ? (float)res[r] : 0.f));
+        for (int j = 0; j < V; ++j) r[j] = n + j < N ? (float)at[j] : 0.f;
     }
 }
-__device__ __forceinline__ floatx4 bias4(const Epilogue& e, int n, int N) {
-    floatx4 b = {0.f, 0.f, 0.f, 0.f};
-    if (e.bias)
+template <typename T, int V> __device__ __forceinline__ void load_bias(const Epilogue& e, int n, int N, float (&b)[V]) {
+    if (!e.bias) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < N) b[r] = load_typed(e.bias, e.btype, n + r);
-    return b;
+        for (int r = 0; r < V; ++r) b[r] = 0.f;
+    } else if (e.bwide) {                          // of type T
+        const auto q = *reinterpret_cast<const typename Wide<T, V>::type*>(reinterpret_cast<const T*>(e.bias) + n);
+#pragma unroll
+        for (int r = 0; r < V; ++r) b[r] = (float)q[r];
+    } else {
+#pragma unroll
+        for (int r = 0; r < V; ++r) b[r] = n + r < N ? load_typed(e.bias, e.btype, n + r) : 0.f;
+    }
+}
+template <typename T, int V, int ACT> __device__ __forceinline__ void finish(const Epilogue& e, long m, int n, int N, float (&v)[V], const float (&bias)[V], const float (&res)[V]) {
+    typedef typename Kept<T>::type Z;
+#pragma unroll
+    for (int r = 0; r < V; ++r) v[r] += bias[r];
+    if (e.z) {
+        typename Wide<Z, V>::type k;
+#pragma unroll
+        for (int r = 0; r < V; ++r) k[r] = keep_z<T>(v[r], ACT == RUNTIME ? e.act : ACT);
+        *reinterpret_cast<typename Wide<Z, V>::type*>(reinterpret_cast<Z*>(e.z) + m * e.ldz + n) = k;      // ldz is a multiple of V
+    }
+#pragma unroll
+    for (int r = 0; r < V; ++r) v[r] = (ACT == RUNTIME ? act_of(v[r], e.act) : sed_act<ACT>(v[r])) + res[r];
+    T* const y = reinterpret_cast<T*>(e.y) + m * N + n;
+    if (e.wide) {
+        typename Wide<T, V>::type o;
+#pragma unroll
+        for (int r = 0; r < V; ++r) o[r] = (T)v[r];
+        *reinterpret_cast<typename Wide<T, V>::type*>(y) = o;
+    } else {
+#pragma unroll
+        for (int r = 0; r < V; ++r)
+            if (n + r < N) y[r] = (T)v[r];
+    }
 }
 
-// ---- 16 bytes of k of 16 rows: one instruction in 16 bits, four in 32 (they take the k of a lane in any order, as long as P and Q agree)
+// ---- 16 bytes of k of every row: one instruction in 16 bits, four in 32 (they take the k of a lane in any order, as long as P and Q agree)
 template <typename T> struct Frag;
 template <> struct Frag<_Float16> { typedef half8 type; };
 template <> struct Frag<__bf16> { typedef bf8 type; };
 template <> struct Frag<float> { typedef floatx4 type; };
+// 16 rows, 64 bytes of k
 __device__ __forceinline__ floatx4 mma(half8 p, half8 q, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, c, 0, 0, 0); }
 __device__ __forceinline__ floatx4 mma(bf8 p, bf8 q, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, q, c, 0, 0, 0); }
 __device__ __forceinline__ floatx4 mma(floatx4 p, floatx4 q, floatx4 c) {
@@ -116,12 +136,19 @@ __device__ __forceinline__ floatx4 mma(floatx4 p, floatx4 q, floatx4 c) {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p[j], q[j], c, 0, 0, 0);
     return c;
 }
+// 32 rows, 32 bytes of k
+__device__ __forceinline__ floatx16 mma(half8 p, half8 q, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(p, q, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mma(bf8 p, bf8 q, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(p, q, c, 0, 0, 0); }
+__device__ __forceinline__ floatx16 mma(floatx4 p, floatx4 q, floatx16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(p[j], q[j], c, 0, 0, 0);
+    return c;
+}
 
 // ---------------------------------------------------------------------------------------------------------------- tiles
 // A step takes 128 bytes of k: 64 elements in 16 bits, 32 in 32.  One operand's tile of R rows is R * 128 bytes.
-//   k contiguous: [R][128 bytes]; 16-byte piece c of row r lies at place c ^ (r & 7).
-//   rows contiguous: [steps of k][R elements]; piece c of line k lies at place c ^ swizzle(k), so that the lines of one transposing read
-//   lie in different banks.
+//   k contiguous: [R][128 bytes];  rows contiguous: [k][R elements];  16-byte piece c of a line lies at place c ^ swizzle(line), so that
+//   the lanes that are served together lie in different banks.
 struct Operand {
     const void* base;
     long ld;                                       // elements from one line to the next
@@ -138,56 +165,63 @@ struct GemmP {
     Epilogue e;
 };
 
-template <typename T, int R, bool ROWS, int THREADS> struct Stage {
+// Row i = 8a + 4h + b of a fragment of 32 rows comes out in register 4a + b of the lanes of half h.  In 16 bits the rows of P are taken in
+// the order 16 (a / 2) + 8h + 4 (a % 2) + b, so that a lane's results are runs of eight consecutive n: 16 bytes to store.
+template <typename T, int R, bool ROWS, int THREADS, bool RUNS> struct Stage {
     static constexpr int E = 16 / sizeof(T), STEP = 128 / sizeof(T), PIECES = R * 8, PER = PIECES / THREADS;
     static constexpr int LINE = ROWS ? R / E : 8;            // pieces in a line
+    static_assert(PIECES % THREADS == 0 && THREADS % LINE == 0 && (ROWS || THREADS / LINE % 16 == 0), "a lane's pieces repeat the swizzle");
     __device__ __forceinline__ static int swizzle(int line) {
-        if (!ROWS) return line & 7;
-        return sizeof(T) == 2 ? 2 * ((line & 3) + 4 * ((line >> 3) & 1)) : 4 * ((line >> 2) & 3);
+        if (!ROWS) return RUNS ? (line & 3) | (line >> 1 & 4) : line & 7;
+        return (sizeof(T) == 2 ? 4 * (line & 3) : 8 * (line >> 2 & 1)) & (LINE - 1);
     }
+    __device__ __forceinline__ static int line_of(int i) { return i * (THREADS / LINE) + threadIdx.x / LINE; }
+    __device__ __forceinline__ static int piece_of(int i) { return (threadIdx.x % LINE) ^ swizzle(line_of(i)); }
     // byte offset of this lane's i-th piece from the tile's first element, OUTSIDE where its row does not exist
     __device__ __forceinline__ static void offsets(const Operand& o, int row0, unsigned (&off)[PER]) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int slot = i * THREADS + threadIdx.x, line = slot / LINE, c = (slot % LINE) ^ swizzle(line);
-            const bool ok = ROWS ? row0 + c * E < o.rows : row0 + line < o.rows;
-            off[i] = ok ? (unsigned)(line * o.ld * (long)sizeof(T)) + c * 16 : OUTSIDE;
+            const bool ok = row0 + (ROWS ? piece_of(i) * E : line_of(i)) < o.rows;
+            off[i] = ok ? (unsigned)(line_of(i) * o.ld * (long)sizeof(T)) + piece_of(i) * 16 : OUTSIDE;
         }
     }
-    __device__ __forceinline__ static void load(const Operand& o, int row0, long k0, long K, const unsigned (&off)[PER], unsigned char* lds) {
-        const T* const at = reinterpret_cast<const T*>(o.base) + (ROWS ? k0 * o.ld + row0 : row0 * o.ld + k0);
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(at), 0, 0x7fffffff, 0x00020000);
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const bool whole = k0 + STEP <= K;
+    // where the step that begins at k lies, and how much of it: what is behind K lies outside and comes as zeros -- all of a step
+    // behind the end, the lines behind K, or, where the last step ends inside the lines, the pieces that are taken out of `off` for good
+    __device__ __forceinline__ static uint4v descriptor(const Operand& o, int row0, long k, long K, unsigned (&off)[PER]) {
+        const unsigned long at = reinterpret_cast<unsigned long>(reinterpret_cast<const T*>(o.base) + (ROWS ? k * o.ld + row0 : row0 * o.ld + k));
+        const int left = (int)max(0l, min(K - k, (long)STEP));
+        if (!ROWS && left > 0 && left < STEP)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            unsigned v = off[i];
-            if (!whole) {
-                const int slot = i * THREADS + threadIdx.x, line = slot / LINE, c = (slot % LINE) ^ swizzle(line);
-                if (k0 + (ROWS ? line : c * E) >= K) v = OUTSIDE;
-            }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (i * THREADS + wave * 64) * 16), 16, (int)v, 0, 0, 0);
-        }
+            for (int i = 0; i < PER; ++i) off[i] = piece_of(0) * E < left ? off[i] : OUTSIDE;
+        const unsigned size = ROWS ? (unsigned)(left * o.ld * (long)sizeof(T)) : (left > 0 ? 0x7fffffffu : 0u);
+        return {(unsigned)at, (unsigned)(at >> 32) & 0xffffu, size, 0x00020000u};
     }
-    // 16 rows from `row` on, the kk-th half of the step's k
+    // The i-th request of a step into the slot of LDS at `lds`.  Written as assembly: it has no register to write, and the compiler, which
+    // cannot tell the slots apart, would wait for it at the next transposing read.  The kernel waits in arrived().  (M0 is the
+    // compiler's, but for nothing that this file uses.)
+    __device__ __forceinline__ static void request(uint4v descriptor, unsigned off, unsigned lds, int i) {
+        asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(descriptor), "s"(lds), "n"(i * THREADS * 16) : "memory", "scc");
+    }
+    // 32 rows from `row` on, the kk-th quarter of the step's k
     __device__ __forceinline__ static typename Frag<T>::type frag(const unsigned char* lds, int row, int kk) {
         typedef typename Frag<T>::type Fr;
-        const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+        const int lane = threadIdx.x & 63, i = lane & 31, half = lane >> 5;
         if constexpr (!ROWS) {
-            const int r = row + l;
-            return *reinterpret_cast<const Fr*>(lds + r * 128 + (((kk * 4 + g) ^ swizzle(r)) << 4));
+            const int r = row + (RUNS ? (i & 16) | (i & 4) << 1 | (i & 8) >> 1 | (i & 3) : i);
+            return *reinterpret_cast<const Fr*>(lds + r * 128 + (((kk * 2 + half) ^ swizzle(r)) << 4));
         } else if constexpr (sizeof(T) == 2) {
-            const int k = kk * 32 + 8 * g + (l >> 2), c = row + (l & 3) * 4;
+            // a transposing read takes 8-byte pieces of four lines from 16 lanes and gives each lane one column of them
+            const int k = kk * 16 + 8 * half + (i >> 2 & 3), j = i & 3, c = row + (i & 16) + (RUNS ? 8 * (j & 1) + 4 * (j >> 1) : 4 * j);
             const unsigned char* const at = lds + k * (R * 2) + (((c >> 3) ^ swizzle(k)) << 4) + (c & 7) * 2;
             typedef __attribute__((address_space(3))) short4t* L;
             const short4t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L)(at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L)(at + 4 * (R * 2)));
             return __builtin_bit_cast(Fr, short8t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
         } else {
             Fr f;
-            const int c = row + l;
+            const int c = row + i;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int k = kk * 16 + 4 * g + j;
+                const int k = kk * 8 + 4 * half + j;
                 f[j] = *reinterpret_cast<const float*>(lds + k * (R * 4) + (((c >> 2) ^ swizzle(k)) << 4) + (c & 3) * 4);
             }
             return f;
@@ -200,56 +234,122 @@ __device__ __forceinline__ int xcd_spread(int bid, int nblk) {       // neighbou
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
 }
 
-template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmP a) {
-    constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 16, NI = BN / WN / 16;
-    typedef Stage<T, BN, PROWS, THREADS> SP;
-    typedef Stage<T, BM, QROWS, THREADS> SQ;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2][(BM + BN) * 128];
+// all but the last LATER requests of every wave have been served, and its LDS reads are done
+template <int LATER> __device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
+    __syncthreads();
+}
+
+// A step is taken in four quarters with two sets of fragments: while the instructions of one quarter run, the next quarter's fragments
+// are read.  In the last quarter every wave holds the rest of the step in registers.
+// LDS is a ring of five slots of one operand's step each: P(t), Q(t), P(t+1), Q(t+1) and the one that P(t+2) goes to during the first
+// three quarters of step t; Q(t+2) goes to P(t)'s slot in the last one, behind a barrier.  The requests of a step are so spread over
+// all of it (a wave that issues sixteen at once waits for the address unit: 57 % of the matrix rate against 80 %), and have at least
+// three quarters to arrive.  Steps behind the end are requested and read like any other, as zeros: the loop has no other branch.
+template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT, int ACT>
+__global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gemm_kernel(GemmP a) {
+    constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, V = 16 / sizeof(T);
+    typedef Stage<T, BN, PROWS, THREADS, V == 8> SP;
+    typedef Stage<T, BM, QROWS, THREADS, false> SQ;
+    typedef typename Frag<T>::type Fr;
+    static_assert(BM == BN, "one size of slot");
+    constexpr int SLOT = BM * 128, FRAGS = NI + MI, MFMAS = MI * NI;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[5 * SLOT];
     const int tiles = a.tm * a.tn, id = xcd_spread(blockIdx.x, gridDim.x);
     const int slice = id / tiles, tile = id % tiles;
-    const int m0 = (tile % a.tm) * BM, n0 = (tile / a.tm) * BN;
-    const long k0 = slice * a.kslice, k1 = CUT ? min(a.K, k0 + a.kslice) : a.K;
+    // tiles in groups of eight rows of tiles: the 32 that an XCD works on share 8 + 4 operand tiles, not 32 + 1
+    const int group = tile / (8 * a.tn), gm = min(8, a.tm - 8 * group), in = tile - group * 8 * a.tn;
+    const int m0 = (8 * group + in % gm) * BM, n0 = in / gm * BN;
+    const long k0 = CUT ? slice * a.kslice : 0, k1 = CUT ? min(a.K, k0 + a.kslice) : a.K;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
     unsigned poff[SP::PER], qoff[SQ::PER];
     SP::offsets(a.p, n0, poff);
     SQ::offsets(a.q, m0, qoff);
-    floatx4 acc[MI][NI] = {};
-    SP::load(a.p, n0, k0, k1, poff, lds[0]);
-    SQ::load(a.q, m0, k0, k1, qoff, lds[0] + BN * 128);
-    __syncthreads();
-    int cur = 0;
-    for (long k = k0; k < k1; k += SP::STEP, cur ^= 1) {
-        if (k + SP::STEP < k1) {
-            SP::load(a.p, n0, k + SP::STEP, k1, poff, lds[cur ^ 1]);
-            SQ::load(a.q, m0, k + SP::STEP, k1, qoff, lds[cur ^ 1] + BN * 128);
+    floatx16 acc[MI][NI] = {};
+    Fr p[2][NI], q[2][MI];
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)lds + wave * 1024;
+    auto ask_p = [&](uint4v d, int slot, int o) { SP::request(d, poff[o], lds0 + slot * SLOT, o); };
+    auto ask_q = [&](uint4v d, int slot, int o) { SQ::request(d, qoff[o], lds0 + slot * SLOT, o); };
+    auto read = [&](int ps, int qs, int kk, int set, int o) {         // one of the fragments of a quarter
+        if (o < NI) p[set][o] = SP::frag(lds + ps * SLOT, wn + 32 * o, kk);
+        else q[set][o - NI] = SQ::frag(lds + qs * SLOT, wm + 32 * (o - NI), kk);
+    };
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const uint4v dp = SP::descriptor(a.p, n0, k0 + t * SP::STEP, k1, poff), dq = SQ::descriptor(a.q, m0, k0 + t * SP::STEP, k1, qoff);
+#pragma unroll
+        for (int o = 0; o < SP::PER; ++o) ask_p(dp, 2 * t, o);
+#pragma unroll
+        for (int o = 0; o < SQ::PER; ++o) ask_q(dq, 2 * t + 1, o);
+    }
+    arrived<SP::PER + SQ::PER>();
+#pragma unroll
+    for (int o = 0; o < FRAGS; ++o) read(0, 1, 0, 0, o);
+    int ps = 0;                                    // P(t)'s slot; the next ones follow around the ring
+    auto ring = [&](int i) { return ps + i < 5 ? ps + i : ps + i - 5; };
+    for (long k = k0; k < k1; k += SP::STEP) {
+        const uint4v dp = SP::descriptor(a.p, n0, k + 2 * SP::STEP, k1, poff), dq = SQ::descriptor(a.q, m0, k + 2 * SP::STEP, k1, qoff);
+        const int qs = ring(1), pn = ring(2), qn = ring(3), spare = ring(4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            if (kk == 3) arrived<SP::PER>();       // the step's fragments are in registers everywhere, the next step is in LDS
+            const int first = SP::PER * kk / 3, asked = kk == 3 ? SQ::PER : SP::PER * (kk + 1) / 3 - first, others = FRAGS + asked;
+            int o = 0;
+#pragma unroll
+            for (int f = 0; f < MFMAS; ++f) {
+                acc[f / NI][f % NI] = mma(p[kk & 1][f % NI], q[kk & 1][f / NI], acc[f / NI][f % NI]);
+#pragma unroll
+                for (; o < others * (f + 1) / MFMAS; ++o) {
+                    if (o < FRAGS) read(kk == 3 ? pn : ps, kk == 3 ? qn : qs, (kk + 1) & 3, (kk + 1) & 1, o);
+                    else if (kk == 3) ask_q(dq, ps, o - FRAGS);
+                    else ask_p(dp, spare, first + o - FRAGS);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        ps = pn;
+    }
+    arrived<0>();                                  // no request is in flight when the workgroup ends
+    constexpr int RUNS = 16 / V, COLS = NI * RUNS;  // a lane has COLS runs of V consecutive n, in MI rows each
+    auto column = [&](int c) { return n0 + wn + 32 * (c / RUNS) + 2 * V * (c % RUNS) + V * (lane >> 5); };
+    auto row = [&](int i) { return m0 + wm + 32 * i + (lane & 31); };
+    if (CUT) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            typename Frag<T>::type p[NI], q[MI];
-#pragma unroll
-            for (int i = 0; i < NI; ++i) p[i] = SP::frag(lds[cur], wn + 16 * i, kk);
-#pragma unroll
-            for (int i = 0; i < MI; ++i) q[i] = SQ::frag(lds[cur] + BN * 128, wm + 16 * i, kk);
+        for (int c = 0; c < COLS; ++c)
 #pragma unroll
             for (int i = 0; i < MI; ++i)
+                if (column(c) < a.N && row(i) < a.M) {
+                    float* const to = a.part + ((long)slice * a.M + row(i)) * a.ldp + column(c);              // ldp is a multiple of 8
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mma(p[j], q[i], acc[i][j]);
-        }
-        __syncthreads();
+                    for (int r = 0; r < V; r += 4) {
+                        const int at = V * (c % RUNS) + r;
+                        *reinterpret_cast<floatx4*>(to + r) = floatx4{acc[i][c / RUNS][at], acc[i][c / RUNS][at + 1], acc[i][c / RUNS][at + 2], acc[i][c / RUNS][at + 3]};
+                    }
+                }
+        return;
     }
+    // bias and residual of the next run of columns are on their way while one run is finished
+    float bias[2][V], res[2][MI][V];
+    auto fetch = [&](int c) {
+        if (column(c) >= a.N) return;
+        load_bias<T, V>(a.e, column(c), a.N, bias[c & 1]);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-        const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
-        if (n >= a.N) continue;
-        const floatx4 b = CUT ? floatx4{0.f, 0.f, 0.f, 0.f} : bias4(a.e, n, a.N);
+        for (int i = 0; i < MI; ++i)
+            if (row(i) < a.M) load_residual<T, V>(a.e, row(i), column(c), a.N, res[c & 1][i]);
+    };
+    fetch(0);
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+        if (c + 1 < COLS) fetch(c + 1);
+        if (column(c) >= a.N) continue;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            const int m = m0 + wm + 16 * i + (lane & 15);
-            if (m >= a.M) continue;
-            if (CUT) *reinterpret_cast<floatx4*>(a.part + ((long)slice * a.M + m) * a.ldp + n) = acc[i][j];      // ldp is a multiple of 4
-            else finish<T>(a.e, m, n, a.N, acc[i][j], b);
+            if (row(i) >= a.M) continue;
+            float v[V];
+#pragma unroll
+            for (int r = 0; r < V; ++r) v[r] = acc[i][c / RUNS][V * (c % RUNS) + r];
+            finish<T, V, ACT>(a.e, row(i), column(c), a.N, v, bias[c & 1], res[c & 1][i]);
         }
     }
 }
@@ -260,9 +360,13 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const f
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long m = i / quads;
         const int n = (int)(i % quads) * 4;
-        floatx4 v = *reinterpret_cast<const floatx4*>(part + m * ldp + n);
-        for (int s = 1; s < slices; ++s) v += *reinterpret_cast<const floatx4*>(part + ((long)s * M + m) * ldp + n);
-        finish<T>(e, m, n, N, v, bias4(e, n, N));
+        if (n >= N) continue;
+        floatx4 s = *reinterpret_cast<const floatx4*>(part + m * ldp + n);
+        for (int k = 1; k < slices; ++k) s += *reinterpret_cast<const floatx4*>(part + ((long)k * M + m) * ldp + n);
+        float v[4] = {s[0], s[1], s[2], s[3]}, b[4], r[4];
+        load_bias<T, 4>(e, n, N, b);
+        load_residual<T, 4>(e, m, n, N, r);
+        finish<T, 4, RUNTIME>(e, m, n, N, v, b, r);
     }
 }
 
@@ -315,7 +419,12 @@ template <typename T, int MT> __global__ __launch_bounds__(512) void rows_kernel
         floatx4 v = sums[0][i][lane];
         for (int s = 1; s < waves; ++s) v += sums[s][i][lane];
         const int m = i * 16 + l, n = n0 + 4 * g;
-        if (m < M && n < N) finish<T>(e, m, n, N, v, bias4(e, n, N));
+        if (m < M && n < N) {
+            float f[4] = {v[0], v[1], v[2], v[3]}, b[4], r[4];
+            load_bias<T, 4>(e, n, N, b);
+            load_residual<T, 4>(e, m, n, N, r);
+            finish<T, 4, RUNTIME>(e, m, n, N, f, b, r);
+        }
     }
 }
 
@@ -418,38 +527,52 @@ long up256(long bytes) { return (bytes + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool needs_pad(const void* p, long ld, int esize) { return !aligned16(p) || ld % (16 / esize); }
 
-constexpr int BM = 128, BN = 128;
-// how often the product is cut along k: into as many slices as leave every CU two workgroups, of at least eight steps each
+// how the product is cut: tile edge, and slices along k
 struct Plan {
-    int tm, tn, slices;
+    int edge, tm, tn, slices;
     long kslice, part_bytes, ldp;
 };
 Plan plan_of(long M, long N, long K, int esize) {
     Plan q;
-    q.tm = sed_cdiv(M, BM);
-    q.tn = sed_cdiv(N, BN);
-    const long step = 128 / esize, steps = (K + step - 1) / step, tiles = (long)q.tm * q.tn;
-    long s = 512 / tiles;
+    const char* env = getenv("SED_EDGE");
+    const long step = 128 / esize, steps = (K + step - 1) / step;
+    q.edge = env ? atoi(env) : 128;
+    if (esize == 4 && q.edge > 128) q.edge = 128;
+    q.tm = sed_cdiv(M, q.edge);
+    q.tn = sed_cdiv(N, q.edge);
+    const long tiles = (long)q.tm * q.tn;
+    long s = (q.edge == 256 ? 256 : q.edge == 128 ? 512 : 1024) / tiles;
     if (s > steps / 8) s = steps / 8;
     if (s < 1) s = 1;
     const long per = (steps + s - 1) / s;
     q.slices = (int)((steps + per - 1) / per);
     q.kslice = per * step;
-    q.ldp = (N + 3) / 4 * 4;
+    q.ldp = (N + 7) / 8 * 8;
     q.part_bytes = q.slices > 1 ? up256(q.slices * M * q.ldp * 4) : 0;
     return q;
 }
 bool few_rows(long M) { return M <= 64; }
 
+template <typename T, bool PROWS, bool QROWS, int EDGE> void launch_edge(const GemmP& a, const Plan& q, hipStream_t stream) {
+    const dim3 grid((unsigned)((long)q.tm * q.tn * q.slices));
+    if (q.slices > 1) { hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, true, 0>), grid, dim3(256), 0, stream, a); return; }
+    if constexpr (!PROWS) {                        // only the forward product has an epilogue
+        switch (a.e.act) {
+            case SED_ACT_RELU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 1>), grid, dim3(256), 0, stream, a); return;
+            case SED_ACT_SILU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 2>), grid, dim3(256), 0, stream, a); return;
+            case SED_ACT_GELU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 3>), grid, dim3(256), 0, stream, a); return;
+        }
+    }
+    hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 0>), grid, dim3(256), 0, stream, a);
+}
 template <typename T, bool PROWS, bool QROWS> int launch_gemm(GemmP a, const Plan& q, float* part, hipStream_t stream) {
     a.tm = q.tm; a.tn = q.tn; a.kslice = q.kslice; a.part = part; a.ldp = q.ldp;
-    const dim3 grid((unsigned)((long)q.tm * q.tn * q.slices));
+    if (q.edge == 64) launch_edge<T, PROWS, QROWS, 64>(a, q, stream);
+    else if (q.edge == 128 || sizeof(T) == 4) launch_edge<T, PROWS, QROWS, 128>(a, q, stream);
+    else if constexpr (sizeof(T) == 2) launch_edge<T, PROWS, QROWS, 256>(a, q, stream);
     if (q.slices > 1) {
-        hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, BM, BN, 2, 2, true>), grid, dim3(256), 0, stream, a);
         const long quads = q.ldp / 4 * a.M, nb = (quads + 255) / 256;
         hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(nb > 8192 ? 8192 : nb)), dim3(256), 0, stream, part, q.slices, a.M, a.N, q.ldp, a.e);
-    } else {
-        hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, BM, BN, 2, 2, false>), grid, dim3(256), 0, stream, a);
     }
     SED_LAUNCH_CHECK();
     return 0;
@@ -491,8 +614,9 @@ GradCut grad_cut(long M, long ld, int esize) {
 template <typename T>
 int linear_fwd(const void* x, const void* w, const void* bias, const void* res, int btype, long M, long N, long K, int act, void* y, void* z,
                char* ws, hipStream_t stream) {
-    Epilogue e{bias, res, y, z, padded(N, sizeof(T)), btype, act, 0};
-    e.wide = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(res)) % (4 * sizeof(T)) == 0;
+    Epilogue e{bias, res, y, z, padded(N, sizeof(T)), btype, act, 0, 0};
+    e.wide = N % (16 / sizeof(T)) == 0 && aligned16(y) && aligned16(res);
+    e.bwide = N % (16 / sizeof(T)) == 0 && aligned16(bias) && btype == Type<T>::code;
     if (few_rows(M)) {
         const long steps = (K + 128 / (long)sizeof(T) - 1) / (128 / (long)sizeof(T));
         const dim3 grid((unsigned)sed_cdiv(N, 16)), block((unsigned)(64 * (steps < 8 ? steps : 8)));
@@ -559,11 +683,11 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
     const void* const xp = d.px ? pad<T>(x, M, K, ws, stream) : x;
     const void* const wp = d.pw ? pad<T>(w, N, K, ws, stream) : w;
     SED_LAUNCH_CHECK();
-    const bool wide = K % 4 == 0;
+    const bool wide = K % (16 / es) == 0;
     if (gx) {
         GemmP a{};
         a.M = (int)M; a.N = (int)K; a.K = ldn;
-        a.e.y = gx; a.e.wide = wide && reinterpret_cast<uintptr_t>(gx) % (4 * es) == 0;
+        a.e.y = gx; a.e.wide = wide && aligned16(gx);
         a.q = {dz, ldn, (int)M};
         a.p = {wp, ldk, (int)ldk};
         // gz has zeros behind its N-th column, W has no line there: k ends at N for W's lines and at ldn for gz's pieces
@@ -574,7 +698,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
     if (gw) {
         GemmP a{};
         a.M = (int)N; a.N = (int)K; a.K = M;
-        a.e.y = gw; a.e.wide = wide && reinterpret_cast<uintptr_t>(gw) % (4 * es) == 0;
+        a.e.y = gw; a.e.wide = wide && aligned16(gw);
         a.q = {dz, ldn, (int)ldn};
         a.p = {xp, ldk, (int)ldk};
         return launch_gemm<T, true, true>(a, plan_of(N, K, M, es), reinterpret_cast<float*>(ws), stream);
