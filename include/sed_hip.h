@@ -507,7 +507,7 @@ int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const 
  * before that.
  * ws: 16-byte aligned scratch of sed_linear_*_ws_bytes bytes (0: none).  M, N, K >= 1; N, K <= 2^21.  The tensors need no more than
  * their element's alignment; lines of a multiple of 16 bytes at 16-byte addresses are read in place, others are copied into ws first
- * (not where M <= 64 in the forward product). */
+ * (not in the forward product of up to 64 rows and lines of up to 16 KB). */
 long sed_linear_kept_elements(long M, long N);
 long sed_linear_fwd_ws_bytes(const void* x, const void* weight, int dtype, long M, long N, long K);
 int sed_linear_fwd(const void* x, const void* weight, const void* bias, const void* residual, int dtype, int bdtype, long M, long N,

@@ -10,7 +10,6 @@
 // Products of 32-bit tensors run on the fp32 matrix instructions; sums are held in 32 bits for all types.
 #include "common.h"
 #include "sed_hip.h"
-#include <stdlib.h>
 
 SED_OBJECT_FLAGS(linear)
 
@@ -266,6 +265,27 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gem
     unsigned poff[SP::PER], qoff[SQ::PER];
     SP::offsets(a.p, n0, poff);
     SQ::offsets(a.q, m0, qoff);
+    // For the epilogue a wave passes 32 rows of its results at a time through LDS: a lane then has V consecutive n of row 32 i + PASS it + lane
+    // / LINE, and its neighbours have the rest of the line.  (Stored from where the instructions leave them, 32 bytes a line, a
+    // bf16 product of 32000 x 2048 x 2048 with silu, residual and kept z took 402 us, now 330.)
+    constexpr int W = BN / WN, LINE = W / V, PASS = 64 / LINE, PASSES = 32 / PASS, PITCH = 4 * W + 16;
+    static_assert(4 * 32 * PITCH <= 5 * SLOT, "the waves' rows fit the ring");
+    const int n = n0 + wn + lane % LINE * V;
+    auto row = [&](int i, int it) { return m0 + wm + 32 * i + PASS * it + lane / LINE; };
+    // All of a lane's residual is requested at once, and from the first where registers are left for it (edges 64 and 128): read run by run
+    // at the end, its latency was a third of the time of a product with K = 512.
+    typedef typename Wide<T, V>::type Run;
+    constexpr bool FORWARD = !PROWS && !CUT, EARLY = BM <= 128;          // only the forward product has an epilogue
+    Run res[FORWARD ? MI : 1][FORWARD ? PASSES : 1];
+    auto fetch = [&]() {
+        if (FORWARD && a.e.res && a.e.wide && n < a.N)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int it = 0; it < PASSES; ++it)
+                    if (row(i, it) < a.M) res[i][it] = *reinterpret_cast<const Run*>(reinterpret_cast<const T*>(a.e.res) + (long)row(i, it) * a.N + n);
+    };
+    if (EARLY) fetch();
     floatx16 acc[MI][NI] = {};
     Fr p[2][NI], q[2][MI];
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)lds + wave * 1024;
@@ -300,7 +320,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gem
             for (int f = 0; f < MFMAS; ++f) {
                 acc[f / NI][f % NI] = mma(p[kk & 1][f % NI], q[kk & 1][f / NI], acc[f / NI][f % NI]);
 #pragma unroll
-                for (; o < others * (f + 1) / MFMAS; ++o) {
+                for (; o < (f < MFMAS / 2 ? FRAGS * 2 * (f + 1) / MFMAS : FRAGS + (others - FRAGS) * (f + 1 - MFMAS / 2) / (MFMAS - MFMAS / 2)); ++o) {
                     if (o < FRAGS) read(kk == 3 ? pn : ps, kk == 3 ? qn : qs, (kk + 1) & 3, (kk + 1) & 1, o);
                     else if (kk == 3) ask_q(dq, ps, o - FRAGS);
                     else ask_p(dp, spare, first + o - FRAGS);
@@ -311,45 +331,47 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gem
         ps = pn;
     }
     arrived<0>();                                  // no request is in flight when the workgroup ends
-    constexpr int RUNS = 16 / V, COLS = NI * RUNS;  // a lane has COLS runs of V consecutive n, in MI rows each
-    auto column = [&](int c) { return n0 + wn + 32 * (c / RUNS) + 2 * V * (c % RUNS) + V * (lane >> 5); };
-    auto row = [&](int i) { return m0 + wm + 32 * i + (lane & 31); };
-    if (CUT) {
+    if (!EARLY) fetch();
+    float bias[V] = {};
+    if (FORWARD && n < a.N) load_bias<T, V>(a.e, n, a.N, bias);
+    // 16-byte piece c of a line lies at place c ^ (c / 8 % 2): two neighbours' pieces, as a lane reads them in 16 bits, lie in other banks
+    unsigned char* const mine = lds + wave * 32 * PITCH;
+    auto place = [](int c) { return (c ^ (c >> 3 & 1)) * 16; };
 #pragma unroll
-        for (int c = 0; c < COLS; ++c)
+    for (int i = 0; i < MI; ++i) {
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
-                if (column(c) < a.N && row(i) < a.M) {
-                    float* const to = a.part + ((long)slice * a.M + row(i)) * a.ldp + column(c);              // ldp is a multiple of 8
+        for (int j = 0; j < NI; ++j)
 #pragma unroll
-                    for (int r = 0; r < V; r += 4) {
-                        const int at = V * (c % RUNS) + r;
-                        *reinterpret_cast<floatx4*>(to + r) = floatx4{acc[i][c / RUNS][at], acc[i][c / RUNS][at + 1], acc[i][c / RUNS][at + 2], acc[i][c / RUNS][at + 3]};
-                    }
-                }
-        return;
-    }
-    // bias and residual of the next run of columns are on their way while one run is finished
-    float bias[2][V], res[2][MI][V];
-    auto fetch = [&](int c) {
-        if (column(c) >= a.N) return;
-        load_bias<T, V>(a.e, column(c), a.N, bias[c & 1]);
+            for (int r = 0; r < 4; ++r) {          // four registers are four consecutive n
+                const int half = lane >> 5, c = 8 * j + (V == 8 ? 4 * (r >> 1) + 2 * half + (r & 1) : 2 * r + half);
+                *reinterpret_cast<floatx4*>(mine + (lane & 31) * PITCH + place(c)) =
+                    floatx4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+            }
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-            if (row(i) < a.M) load_residual<T, V>(a.e, row(i), column(c), a.N, res[c & 1][i]);
-    };
-    fetch(0);
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        if (c + 1 < COLS) fetch(c + 1);
-        if (column(c) >= a.N) continue;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            if (row(i) >= a.M) continue;
+        for (int it = 0; it < PASSES; ++it) {
             float v[V];
 #pragma unroll
-            for (int r = 0; r < V; ++r) v[r] = acc[i][c / RUNS][V * (c % RUNS) + r];
-            finish<T, V, ACT>(a.e, row(i), column(c), a.N, v, bias[c & 1], res[c & 1][i]);
+            for (int h = 0; h < V / 4; ++h) {
+                const floatx4 q = *reinterpret_cast<const floatx4*>(mine + (PASS * it + lane / LINE) * PITCH + place(lane % LINE * (V / 4) + h));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * h + j] = q[j];
+            }
+            const int m = row(i, it);
+            if (m >= a.M || n >= a.N) continue;
+            if (CUT) {
+                float* const to = a.part + ((long)slice * a.M + m) * a.ldp + n;              // ldp is a multiple of 8
+#pragma unroll
+                for (int h = 0; h < V; h += 4) *reinterpret_cast<floatx4*>(to + h) = floatx4{v[h], v[h + 1], v[h + 2], v[h + 3]};
+            } else {
+                float r[V] = {};
+                if (FORWARD && a.e.res) {
+                    if (!a.e.wide) load_residual<T, V>(a.e, m, n, a.N, r);
+                    else
+#pragma unroll
+                        for (int j = 0; j < V; ++j) r[j] = (float)res[FORWARD ? i : 0][FORWARD ? it : 0][j];
+                }
+                finish<T, V, ACT>(a.e, m, n, a.N, v, bias, r);
+            }
         }
     }
 }
@@ -371,41 +393,42 @@ template <typename T> __global__ __launch_bounds__(256) void join_kernel(const f
 }
 
 // ---------------------------------------------------------------------------------------------------------------- few rows
-// Up to 16 * MT rows of x: the product is a pass over W.  A workgroup owns 16 rows of W, its waves split k, 64 bytes a row and
-// instruction; the waves' sums are added through LDS.  No alignment is asked of x and W.
-template <typename T> __device__ __forceinline__ typename Frag<T>::type piece(const T* row, long k, long K, bool ok) {
+// Up to 16 * MT rows of x: the product is a pass over W.  A workgroup owns 16 rows of W, its waves split k in runs of U times 64 bytes, all of
+// them requested at once; the waves' sums are added through LDS.  No alignment is asked of x and W.  Rows that do not exist are
+// read as the first one: they only reach results that are not stored.
+template <typename T> __device__ __forceinline__ typename Frag<T>::type piece(const T* row, long k, long K) {
     constexpr int E = 16 / sizeof(T);
     typename Frag<T>::type f;
-    if (ok && k + E <= K) {
-        __builtin_memcpy(&f, row + k, 16);
-        return f;
-    }
 #pragma unroll
-    for (int j = 0; j < E; ++j) f[j] = ok && k + j < K ? row[k + j] : (T)0.f;
+    for (int j = 0; j < E; ++j) f[j] = k + j < K ? row[k + j] : (T)0.f;
     return f;
 }
-template <typename T, int MT> __global__ __launch_bounds__(512) void rows_kernel(const T* x, const T* w, int M, int N, long K, Epilogue e) {
-    constexpr int E = 16 / sizeof(T), U = 2;
-    __shared__ __attribute__((aligned(16))) floatx4 sums[8][MT][64];
+template <typename T, int MT, int U> __global__ __launch_bounds__(1024) void rows_kernel(const T* x, const T* w, int M, int N, long K, Epilogue e) {
+    constexpr int E = 16 / sizeof(T), RUN = 4 * E * U;
+    __shared__ __attribute__((aligned(16))) floatx4 sums[16][MT][64];
     const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16;
-    const bool pn = n0 + l < N;
-    const T* const wr = w + (long)(pn ? n0 + l : 0) * K;
+    const T* const wr = w + (long)(n0 + l < N ? n0 + l : 0) * K;
     const T* xr[MT];
-    bool pm[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        pm[i] = i * 16 + l < M;
-        xr[i] = x + (long)(pm[i] ? i * 16 + l : 0) * K;
-    }
+    for (int i = 0; i < MT; ++i) xr[i] = x + (long)(i * 16 + l < M ? i * 16 + l : 0) * K;
     floatx4 acc[MT] = {};
-    for (long k = (long)wave * 4 * E * U; k < K; k += (long)waves * 4 * E * U) {
-        typename Frag<T>::type p[U], q[U][MT];
+    typename Frag<T>::type p[U], q[U][MT];
+    for (long k = (long)wave * RUN; k < K; k += (long)waves * RUN) {
+        if (k + RUN <= K) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            p[u] = piece<T>(wr, k + (u * 4 + g) * E, K, pn);
+            for (int u = 0; u < U; ++u) {
+                __builtin_memcpy(&p[u], wr + k + (u * 4 + g) * E, 16);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) q[u][i] = piece<T>(xr[i], k + (u * 4 + g) * E, K, pm[i]);
+                for (int i = 0; i < MT; ++i) __builtin_memcpy(&q[u][i], xr[i] + k + (u * 4 + g) * E, 16);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                p[u] = piece<T>(wr, k + (u * 4 + g) * E, K);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) q[u][i] = piece<T>(xr[i], k + (u * 4 + g) * E, K);
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -426,6 +449,13 @@ template <typename T, int MT> __global__ __launch_bounds__(512) void rows_kernel
             finish<T, 4, RUNTIME>(e, m, n, N, f, b, r);
         }
     }
+}
+template <typename T, int U> void launch_rows(const T* x, const T* w, int M, int N, long K, const Epilogue& e, hipStream_t stream) {
+    const long runs = (K * (long)sizeof(T) + 64 * U - 1) / (64 * U);
+    const dim3 grid((unsigned)sed_cdiv(N, 16)), block((unsigned)(64 * (runs < 16 ? runs : 16)));
+    if (M <= 16) hipLaunchKernelGGL((rows_kernel<T, 1, U>), grid, block, 0, stream, x, w, M, N, K, e);
+    else if (M <= 32) hipLaunchKernelGGL((rows_kernel<T, 2, U>), grid, block, 0, stream, x, w, M, N, K, e);
+    else hipLaunchKernelGGL((rows_kernel<T, 4, 2>), grid, block, 0, stream, x, w, M, N, K, e);          // few_rows(): lines of up to 1 KB, U = 2
 }
 
 // ---------------------------------------------------------------------------------------------------------------- passes around them
@@ -450,49 +480,50 @@ template <typename T> __global__ __launch_bounds__(256) void pad_kernel(const T*
 // A thread owns E columns (16 bytes) of every RT-th row of a chunk.
 struct GradP {
     const void* gy;
-    const void* z;                                 // null: no activation
+    const void* z;
     void* gz;
     float* sums;                                   // nullable, [chunks][ld]
     long M, rows;
     int N, ld, CT, RT, tiles, act;
 };
-template <typename T> __device__ __forceinline__ float act_grad_of(float z, int act) {
-    switch (act) {
-        case SED_ACT_RELU: return z;               // kept as 0 or 1
-        case SED_ACT_SILU: return sed_act_grad<2>(z);
-        case SED_ACT_GELU: return sed_act_grad<3>(z);
-    }
-    return 1.f;
-}
-template <typename T> __global__ __launch_bounds__(256) void act_grad_kernel(GradP p) {
-    constexpr int E = 16 / sizeof(T);
+template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) void act_grad_kernel(GradP p) {       // WHOLE: N is a multiple of E
+    constexpr int E = 16 / sizeof(T), U = 4;
     typedef typename Kept<T>::type Z;
     __shared__ float red[256 * E];
     const int tile = (int)(blockIdx.x % p.tiles), t = threadIdx.x, col = tile * p.CT + t % p.CT, r = t / p.CT, c = col * E;
     const long chunk = blockIdx.x / p.tiles, s0 = chunk * p.rows, s1 = min(p.M, s0 + p.rows);
+    const T* const gy = reinterpret_cast<const T*>(p.gy) + c;
+    const Z* const kept = reinterpret_cast<const Z*>(p.z) + c;
     float sum[E] = {};
     if (r < p.RT && c < p.ld)
-        for (long s = s0 + r; s < s1; s += p.RT) {
-            T g[E];
-            if (c + E <= p.N) __builtin_memcpy(g, reinterpret_cast<const T*>(p.gy) + s * p.N + c, 16);
-            else
+        for (long s = s0 + r; s < s1; s += U * p.RT) {
+            T g[U][E];
+            Z z[U][E];
+            // rows behind the chunk are read as its last one and left out of the sums
 #pragma unroll
-                for (int j = 0; j < E; ++j) g[j] = c + j < p.N ? reinterpret_cast<const T*>(p.gy)[s * p.N + c + j] : (T)0.f;
-            float f[E];
+            for (int u = 0; u < U; ++u) {
+                const long at = min(s + u * p.RT, s1 - 1);
+                if (WHOLE) __builtin_memcpy(g[u], gy + at * p.N, 16);
+                else
 #pragma unroll
-            for (int j = 0; j < E; ++j) f[j] = (float)g[j];
-            if (p.z) {
-                Z z[E];
-                __builtin_memcpy(z, reinterpret_cast<const Z*>(p.z) + s * p.ld + c, sizeof(z));
-#pragma unroll
-                for (int j = 0; j < E; ++j) f[j] = c + j < p.N ? f[j] * act_grad_of<T>((float)z[j], p.act) : 0.f;
+                    for (int j = 0; j < E; ++j) g[u][j] = c + j < p.N ? gy[at * p.N + j] : (T)0.f;
+                if (ACT) __builtin_memcpy(z[u], kept + at * p.ld, sizeof(z[u]));
             }
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                sum[j] += f[j];
-                g[j] = (T)f[j];
+            for (int u = 0; u < U; ++u) {
+                const long at = s + u * p.RT;
+                if (at >= s1) continue;
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    float f = (float)g[u][j];
+                    if (ACT == SED_ACT_RELU) f = (float)z[u][j] != 0.f ? f : 0.f;             // kept as 1 or 0
+                    else if (ACT) f *= sed_act_grad<ACT>((float)z[u][j]);
+                    if (!WHOLE && c + j >= p.N) f = 0.f;   // z is not written there
+                    sum[j] += f;
+                    g[u][j] = (T)f;
+                }
+                if (p.gz) __builtin_memcpy(reinterpret_cast<T*>(p.gz) + at * p.ld + c, g[u], 16);
             }
-            if (p.gz) __builtin_memcpy(reinterpret_cast<T*>(p.gz) + s * p.ld + c, g, 16);
         }
     if (!p.sums) return;
 #pragma unroll
@@ -505,19 +536,30 @@ template <typename T> __global__ __launch_bounds__(256) void act_grad_kernel(Gra
         if (n < p.ld) p.sums[chunk * p.ld + n] = v;
     }
 }
-// gb [N] of `type` = the column sums of sums [chunks][ld]: 16 columns x 16 lanes
-__global__ __launch_bounds__(256) void column_sums_kernel(const float* sums, long chunks, int ld, int N, void* gb, int type) {
-    __shared__ float red[16][17];
+template <typename T, bool WHOLE> void launch_act_grad(const GradP& p, unsigned blocks, hipStream_t stream) {
+    switch (p.act) {
+        case SED_ACT_NONE: hipLaunchKernelGGL((act_grad_kernel<T, 0, WHOLE>), dim3(blocks), dim3(256), 0, stream, p); break;
+        case SED_ACT_RELU: hipLaunchKernelGGL((act_grad_kernel<T, 1, WHOLE>), dim3(blocks), dim3(256), 0, stream, p); break;
+        case SED_ACT_SILU: hipLaunchKernelGGL((act_grad_kernel<T, 2, WHOLE>), dim3(blocks), dim3(256), 0, stream, p); break;
+        default: hipLaunchKernelGGL((act_grad_kernel<T, 3, WHOLE>), dim3(blocks), dim3(256), 0, stream, p);
+    }
+}
+// gb [N] of `type` = the column sums of sums [chunks][ld]: 16 columns x 64 lanes
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* sums, long chunks, int ld, int N, void* gb, int type) {
+    __shared__ float red[64][17];
     const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
     float v = 0.f;
-    if (c < N)
-        for (long i = row; i < chunks; i += 16) v += sums[i * ld + c];
+    if (c < N) {
+#pragma unroll 4
+        for (long i = row; i < chunks; i += 64) v += sums[i * ld + c];
+    }
     red[row][lane] = v;
     __syncthreads();
-    if (row == 0 && c < N) {
-        for (int k = 1; k < 16; ++k) v += red[k][lane];
-        store_typed(gb, type, c, v);
+    for (int s = 32; s > 0; s >>= 1) {
+        if (row < s) red[row][lane] += red[row + s][lane];
+        __syncthreads();
     }
+    if (row == 0 && c < N) store_typed(gb, type, c, red[0][lane]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -527,31 +569,42 @@ long up256(long bytes) { return (bytes + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool needs_pad(const void* p, long ld, int esize) { return !aligned16(p) || ld % (16 / esize); }
 
-// how the product is cut: tile edge, and slices along k
+// How a product is cut: tile edge, and slices along k that a second pass adds.  The cut with the least time by what was measured on an
+// MI355X: a step of 128 bytes of k takes a tile of 64, 128 or 256 the microseconds below when 1, 2, .. of them share a CU (LDS holds 4, 2
+// or 1), a tile costs as much again at its ends, and a cut one passes its 32-bit sums through memory.  It picks the fastest of all
+// cuts, or one within 8 %, at (rows, N, K) from (100, 512, 512) to (32000, 2048, 2048); e.g. bf16 (4000, 512, 512) 7.6 us with edge 64 and
+// 9.4 with 128, (4000, 2048, 512) 15.0 with 128, 18.9 with 64, 25.2 with 256, (4096, 4096, 4096) 117 with 256 and 133 with 128.
 struct Plan {
     int edge, tm, tn, slices;
     long kslice, part_bytes, ldp;
 };
 Plan plan_of(long M, long N, long K, int esize) {
-    Plan q;
-    const char* env = getenv("SED_EDGE");
+    static const int edges[3] = {64, 128, 256}, room[3] = {4, 2, 1};
+    static const float ends[3] = {4.f, 6.f, 16.f};
+    static const float step16[3][4] = {{.30f, .45f, .65f, .80f}, {.60f, .95f}, {1.65f}}, step32[2][4] = {{.65f, 1.23f, 1.7f, 2.1f}, {2.0f, 3.9f}};
     const long step = 128 / esize, steps = (K + step - 1) / step;
-    q.edge = env ? atoi(env) : 128;
-    if (esize == 4 && q.edge > 128) q.edge = 128;
-    q.tm = sed_cdiv(M, q.edge);
-    q.tn = sed_cdiv(N, q.edge);
-    const long tiles = (long)q.tm * q.tn;
-    long s = (q.edge == 256 ? 256 : q.edge == 128 ? 512 : 1024) / tiles;
-    if (s > steps / 8) s = steps / 8;
-    if (s < 1) s = 1;
-    const long per = (steps + s - 1) / s;
-    q.slices = (int)((steps + per - 1) / per);
-    q.kslice = per * step;
-    q.ldp = (N + 7) / 8 * 8;
-    q.part_bytes = q.slices > 1 ? up256(q.slices * M * q.ldp * 4) : 0;
-    return q;
+    Plan best{};
+    float least = 0.f;
+    for (int e = 0; e < (esize == 2 ? 3 : 2); ++e) {
+        const float* const us = esize == 2 ? step16[e] : step32[e];
+        const long tm = (M + edges[e] - 1) / edges[e], tn = (N + edges[e] - 1) / edges[e];
+        for (long s = 1; s <= 64 && (s == 1 || (steps / s >= 4 && tm * tn * s <= 2048)); s *= 2) {
+            const long per = (steps + s - 1) / s, slices = (steps + per - 1) / per, on = (tm * tn * slices + 255) / 256;
+            float t = (float)(on / room[e]) * (per * us[room[e] - 1] + ends[e]);
+            if (on % room[e]) t += per * us[on % room[e] - 1] + ends[e];
+            if (slices > 1) t += 4.f + (float)slices * M * N * 8.f / 5e6f;
+            if (best.edge && t >= least) continue;
+            least = t;
+            best.edge = edges[e]; best.tm = (int)tm; best.tn = (int)tn; best.slices = (int)slices; best.kslice = per * step;
+        }
+    }
+    best.ldp = (N + 7) / 8 * 8;
+    best.part_bytes = best.slices > 1 ? up256(best.slices * M * best.ldp * 4) : 0;
+    return best;
 }
-bool few_rows(long M) { return M <= 64; }
+// A few rows are a pass over W with 16 of its rows per workgroup, which reads all of x: one row of bf16 (1, 4096, 4096) takes 7.4 us, 16
+// rows 10.1, 64 rows 24.7 against 15.2 in tiles; (64, 2048, 512) 5.1 against 5.5, (64, 512, 2048) 13.4 against 8.1.
+bool few_rows(long M, long K, int esize) { return M <= 64 && K * esize <= (M <= 16 ? 16384 : M <= 32 ? 4096 : 1024); }
 
 template <typename T, bool PROWS, bool QROWS, int EDGE> void launch_edge(const GemmP& a, const Plan& q, hipStream_t stream) {
     const dim3 grid((unsigned)((long)q.tm * q.tn * q.slices));
@@ -616,14 +669,12 @@ int linear_fwd(const void* x, const void* w, const void* bias, const void* res, 
                char* ws, hipStream_t stream) {
     Epilogue e{bias, res, y, z, padded(N, sizeof(T)), btype, act, 0, 0};
     e.wide = N % (16 / sizeof(T)) == 0 && aligned16(y) && aligned16(res);
-    e.bwide = N % (16 / sizeof(T)) == 0 && aligned16(bias) && btype == Type<T>::code;
-    if (few_rows(M)) {
-        const long steps = (K + 128 / (long)sizeof(T) - 1) / (128 / (long)sizeof(T));
-        const dim3 grid((unsigned)sed_cdiv(N, 16)), block((unsigned)(64 * (steps < 8 ? steps : 8)));
+    e.bwide = bias && N % (16 / sizeof(T)) == 0 && aligned16(bias) && btype == Type<T>::code;
+    if (few_rows(M, K, sizeof(T))) {
         const T *xt = reinterpret_cast<const T*>(x), *wt = reinterpret_cast<const T*>(w);
-        if (M <= 16) hipLaunchKernelGGL((rows_kernel<T, 1>), grid, block, 0, stream, xt, wt, (int)M, (int)N, K, e);
-        else if (M <= 32) hipLaunchKernelGGL((rows_kernel<T, 2>), grid, block, 0, stream, xt, wt, (int)M, (int)N, K, e);
-        else hipLaunchKernelGGL((rows_kernel<T, 4>), grid, block, 0, stream, xt, wt, (int)M, (int)N, K, e);
+        // as many waves as there are runs, and longer runs once there are more than sixteen
+        if (K * (long)sizeof(T) > 16 * 128) launch_rows<T, 4>(xt, wt, (int)M, (int)N, K, e, stream);
+        else launch_rows<T, 2>(xt, wt, (int)M, (int)N, K, e, stream);
         SED_LAUNCH_CHECK();
         return 0;
     }
@@ -637,7 +688,7 @@ int linear_fwd(const void* x, const void* w, const void* bias, const void* res, 
 }
 
 long fwd_ws(const void* x, const void* w, int esize, long M, long N, long K) {
-    if (few_rows(M)) return 0;
+    if (few_rows(M, K, esize)) return 0;
     const long ld = padded(K, esize);
     return (needs_pad(x, K, esize) ? up256(M * ld * esize) : 0) + (needs_pad(w, K, esize) ? up256(N * ld * esize) : 0) + plan_of(M, N, ld, esize).part_bytes;
 }
@@ -675,10 +726,11 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         ws += up256(c.chunks * ldn * 4);
     }
     if (gz || gb) {
-        GradP p{gy, act == SED_ACT_NONE ? nullptr : z, gz, sums, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act};
-        hipLaunchKernelGGL((act_grad_kernel<T>), dim3((unsigned)(c.chunks * c.tiles)), dim3(256), 0, stream, p);
+        GradP p{gy, z, gz, sums, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act};
+        if (N % (16 / es) == 0) launch_act_grad<T, true>(p, (unsigned)(c.chunks * c.tiles), stream);
+        else launch_act_grad<T, false>(p, (unsigned)(c.chunks * c.tiles), stream);
     }
-    if (gb) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(256), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
+    if (gb) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(1024), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
     const void* const dz = gz ? gz : gy;
     const void* const xp = d.px ? pad<T>(x, M, K, ws, stream) : x;
     const void* const wp = d.pw ? pad<T>(w, N, K, ws, stream) : w;
