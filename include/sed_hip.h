@@ -487,15 +487,15 @@ int sed_guard_publish(const int* err_dev, float* flag_out, sed_stream_t stream);
  * x, y, gy, gx [N][S][C] of `dtype` (SED_F32 / SED_F16 / SED_BF16); group g = channels [g C/G, (g+1) C/G).
  *   mean, rstd [N][G] (float): over the S rows and C/G channels of a group, rstd = 1 / sqrt(variance + eps), variance / count
  *   z = (x - mean) rstd weight + bias;  y = act(z);  weight, bias [C] of wdtype, nullable (1 and 0)
- *   gz = gy act'(z);  gweight = sum gz xhat;  gbias = sum gz  (float [C], nullable)
+ *   gz = gy act'(z);  gweight = sum gz xhat;  gbias = sum gz  ([C] of wdtype, nullable)
  *   gx = rstd (gz weight - mean_g(gz weight) - xhat mean_g(gz weight xhat))  (nullable)
- * ws: sed_group_norm_ws_floats(N, S, C, G, backward) floats of scratch.  No pointer needs more than its element's alignment.
+ * ws: sed_group_norm_ws_floats(..) floats of scratch (0: null will do).  No pointer needs more than its element's alignment.
  * N, S, C >= 1, C % G == 0. */
-long sed_group_norm_ws_floats(long N, long S, int C, int G, int backward);
+long sed_group_norm_ws_floats(int dtype, long N, long S, int C, int G, int backward);
 int sed_group_norm_fwd(const void* x, const void* weight, const void* bias, int dtype, int wdtype, long N, long S, int C, int G,
                        float eps, int act, void* y, float* mean, float* rstd, float* ws, sed_stream_t stream);
 int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const void* bias, int dtype, int wdtype, long N, long S,
-                       int C, int G, int act, const float* mean, const float* rstd, void* gx, float* gweight, float* gbias, float* ws,
+                       int C, int G, int act, const float* mean, const float* rstd, void* gx, void* gweight, void* gbias, float* ws,
                        sed_stream_t stream);
 
 /* ---- matrix product with bias, activation and residual in its epilogue -----------------------------------------------

@@ -3,7 +3,9 @@
 //   mean, rstd over the S rows and the C/G channels of a group;  xhat = (x - mean) rstd;  z = xhat w + b;  y = act(z)
 //   gz = gy act'(z);  gw = sum gz xhat;  gb = sum gz;  h = gz w;  gx = rstd (h - mean_g(h) - xhat mean_g(h xhat))
 //
-// Bound by HBM.  The statistics of a group need every row of a sample before any element of it can be written.
+// Bound by HBM.  The statistics of a group need every row of a sample before any element of it can be written.  Where the rows of some
+// groups fit the registers of a workgroup they are read once (the one-pass kernels); beyond that a first pass leaves sums per chunk
+// of rows and channel, a small kernel adds them up, and a second pass reads the rows again.
 //
 // A thread owns V channels (16 bytes) of every RT-th row of a chunk of rows, whatever the group width: sums are held per channel and
 // folded to groups afterwards.  A row that is not a multiple of V channels ends in a vector that overlaps its neighbour (the twice
@@ -68,6 +70,12 @@ __device__ __forceinline__ float load_param(const void* p, int type, int c, floa
     if (type == SED_F32) return reinterpret_cast<const float*>(p)[c];
     if (type == SED_F16) return (float)reinterpret_cast<const _Float16*>(p)[c];
     return (float)reinterpret_cast<const __bf16*>(p)[c];
+}
+
+__device__ __forceinline__ void store_param(void* p, int type, int c, float v) {
+    if (type == SED_F32) reinterpret_cast<float*>(p)[c] = v;
+    else if (type == SED_F16) reinterpret_cast<_Float16*>(p)[c] = (_Float16)v;
+    else reinterpret_cast<__bf16*>(p)[c] = (__bf16)v;
 }
 
 // where this thread works: sample, chunk, first channel, row lane
@@ -263,60 +271,79 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
     });
 }
 
-// one workgroup per (sample, group): the chunks' sums per channel, chan [N][2][C], and the group's two means, coef [N][G][2]
-__global__ __launch_bounds__(128) void norm_bwd_fold_kernel(const float* parts, long S, long chunks, int C, int G, const void* w, int wdtype, float* chan, float* coef) {
-    __shared__ float red[2][2];
-    const long n = blockIdx.x / G;
-    const int g = (int)(blockIdx.x % G), cg = C / G;
-    const float* const base = parts + n * chunks * 2 * C + g * cg;
-    float ga = 0.f, gb = 0.f;
-    for (int k = threadIdx.x; k < cg; k += 128) {
+// per (sample, bundle of `per` groups): the chunks' sums per channel, chan [N][2][C], and the groups' two means, coef [N][G][2].  A channel's
+// chunks are shared out to as many threads as there are for it.
+__global__ __launch_bounds__(256) void norm_bwd_fold_kernel(const float* parts, long S, long chunks, int C, int G, int per, const void* w, int wdtype, float* chan, float* coef) {
+    __shared__ float red[2][256];
+    const int bundles = (G + per - 1) / per, cg = C / G;
+    const long n = blockIdx.x / bundles;
+    const int g0 = (int)(blockIdx.x % bundles) * per, c0 = g0 * cg, c1 = min(G, g0 + per) * cg, t = threadIdx.x;
+    const float* const base = parts + n * chunks * 2 * C;
+    const int lanes = min(256, c1 - c0), share = 256 / lanes, lane = t % lanes, first = t / lanes;
+    for (int c = c0; c < c1; c += lanes) {         // more than 256 channels only where per is 1
         float a = 0.f, b = 0.f;
-        for (long i = 0; i < chunks; ++i) {
-            a += base[i * 2 * C + k];
-            b += base[i * 2 * C + C + k];
+        const int k = c + lane;
+        if (first < share && k < c1)
+#pragma unroll 4
+            for (long i = first; i < chunks; i += share) {
+                a += base[i * 2 * C + k];
+                b += base[i * 2 * C + C + k];
+            }
+        __syncthreads();
+        red[0][t] = a;
+        red[1][t] = b;
+        __syncthreads();
+        if (t < lanes && k < c1) {
+            for (int i = 1; i < share; ++i) {
+                a += red[0][i * lanes + t];
+                b += red[1][i * lanes + t];
+            }
+            chan[n * 2 * C + k] = a;
+            chan[n * 2 * C + C + k] = b;
         }
-        const int c = g * cg + k;
-        chan[n * 2 * C + c] = a;
-        chan[n * 2 * C + C + c] = b;
-        const float wc = load_param(w, wdtype, c, 1.f);
-        ga = fmaf(wc, a, ga);
-        gb = fmaf(wc, b, gb);
     }
-    ga = wave_sum(ga);
-    gb = wave_sum(gb);
-    if ((threadIdx.x & 63) == 0) {
-        red[0][threadIdx.x >> 6] = ga;
-        red[1][threadIdx.x >> 6] = gb;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const float scale = 1.f / ((float)S * (float)cg);
-        coef[blockIdx.x * 2l] = (red[0][0] + red[0][1]) * scale;
-        coef[blockIdx.x * 2l + 1] = (red[1][0] + red[1][1]) * scale;
+    __syncthreads();                               // the workgroup's own stores to chan are read back below
+    for (int g = g0 + (t >> 6); g < min(G, g0 + per); g += 4) {
+        float a = 0.f, b = 0.f;
+        for (int k = t & 63; k < cg; k += 64) {
+            const int c = g * cg + k;
+            const float wc = load_param(w, wdtype, c, 1.f);
+            a = fmaf(wc, chan[n * 2 * C + c], a);
+            b = fmaf(wc, chan[n * 2 * C + C + c], b);
+        }
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if ((t & 63) == 0) {
+            const float scale = 1.f / ((float)S * (float)cg);
+            coef[(n * G + g) * 2] = a * scale;
+            coef[(n * G + g) * 2 + 1] = b * scale;
+        }
     }
 }
 
-// gbias, gweight [C]: the sums of chan [N][2][C] over the samples; 16 channels x 16 sample lanes per workgroup
-__global__ __launch_bounds__(256) void norm_bwd_params_kernel(const float* chan, long N, int C, float* gw, float* gb) {
-    __shared__ float red[2][16][17];
+// gbias, gweight [C] of wdtype: the sums of chan [N][2][C] over the samples; 16 channels x 64 sample lanes per workgroup
+__global__ __launch_bounds__(1024) void norm_bwd_params_kernel(const float* chan, long N, int C, void* gw, void* gb, int wdtype) {
+    __shared__ float red[2][64][17];
     const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
     float a = 0.f, b = 0.f;
     if (c < C)
-        for (long n = row; n < N; n += 16) {
+        for (long n = row; n < N; n += 64) {
             a += chan[n * 2 * C + c];
             b += chan[n * 2 * C + C + c];
         }
     red[0][row][lane] = a;
     red[1][row][lane] = b;
     __syncthreads();
-    if (row == 0 && c < C) {
-        for (int k = 1; k < 16; ++k) {
-            a += red[0][k][lane];
-            b += red[1][k][lane];
+    for (int s = 32; s > 0; s >>= 1) {
+        if (row < s) {
+            red[0][row][lane] += red[0][row + s][lane];
+            red[1][row][lane] += red[1][row + s][lane];
         }
-        if (gb) gb[c] = a;
-        if (gw) gw[c] = b;
+        __syncthreads();
+    }
+    if (row == 0 && c < C) {
+        if (gb) store_param(gb, wdtype, c, red[0][0][lane]);
+        if (gw) store_param(gw, wdtype, c, red[1][0][lane]);
     }
 }
 
@@ -362,10 +389,236 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
     }
 }
 
+// ---- one pass: the rows of a bundle of whole groups stay in the registers of one workgroup, up to 128 KB (forward) or 2 x 64 KB
+// (backward), and are read once.  The statistics are then the plain two-step ones: mean, then squared deviations from it.
+struct OneP {
+    const void* x;
+    const void* gy;
+    const void* w;
+    const void* b;
+    void* y;                             // y, or gx (nullable)
+    float* mean;
+    float* rstd;
+    float* chan;                         // backward: [N][2][C], sum gz and sum gz xhat
+    long S;
+    int C, G, per, bundles, wdtype;      // per: groups in a bundle
+    float eps;
+};
+constexpr int MAX_BUNDLE = 1024;         // channels of a bundle
+constexpr int ONE_THREADS = 512, ONE_FWD = 16, ONE_BWD = 8;        // threads, and 16-byte vectors of x that one of them holds
+
+// Sums of a[V], b[V] over the row lanes of each of the bundle's channels, left in out[2][channels] (LDS).  scratch: 2 * blockDim * V floats.
+template <int V> __device__ __forceinline__ void channel_sums(int CT, int RT, int K, int width, const float (&a)[V], const float (&b)[V], float* scratch, float* out) {
+    const int t = threadIdx.x, T = blockDim.x, NC = CT * V;
+    float* const ra = scratch;
+    float* const rb = scratch + T * V;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        ra[t * V + j] = a[j];
+        rb[t * V + j] = b[j];
+    }
+    __syncthreads();
+    // NC columns of RT numbers: share = how many threads add up one column, in two steps
+    const int share = max(1, min(T / NC, 16)), lane = t / NC, k0 = t % NC;
+    if (share > 1) {
+        float sa = 0.f, sb = 0.f;
+        if (lane < share)
+            for (int r = lane; r < RT; r += share) {
+                sa += ra[r * NC + k0];
+                sb += rb[r * NC + k0];
+            }
+        __syncthreads();
+        if (lane < share) {
+            ra[lane * NC + k0] = sa;
+            rb[lane * NC + k0] = sb;
+        }
+        __syncthreads();
+    }
+    const int rows = share > 1 ? share : RT;
+    for (int k = t; k < NC; k += T) {
+        float sa = 0.f, sb = 0.f;
+        for (int r = 0; r < rows; ++r) {
+            sa += ra[r * NC + k];
+            sb += rb[r * NC + k];
+        }
+        const int own = k / V * V, c = min(own, width - V) + k % V;
+        if (k / V < K && c >= own) {
+            out[c] = sa;
+            out[MAX_BUNDLE + c] = sb;
+        }
+    }
+    __syncthreads();
+}
+// sums over a group's channels of two LDS arrays, times f(channel); result to every thread through LDS, per group of the bundle
+template <typename F> __device__ __forceinline__ void group_sums(const float* chan, int groups, int cg, F f, float* out) {
+    const int t = threadIdx.x, waves = (blockDim.x + 63) >> 6;
+    for (int g = t >> 6; g < groups; g += waves) {
+        float a = 0.f, b = 0.f;
+        for (int k = t & 63; k < cg; k += 64) {
+            const float w = f(g * cg + k);
+            a = fmaf(w, chan[g * cg + k], a);
+            b = fmaf(w, chan[MAX_BUNDLE + g * cg + k], b);
+        }
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if ((t & 63) == 0) {
+            out[2 * g] = a;
+            out[2 * g + 1] = b;
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS) void norm_one_kernel(OneP p) {
+    extern __shared__ float scratch[];             // 2 * blockDim * V floats
+    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE];
+    const long n = blockIdx.x / p.bundles;
+    const int g0 = (int)(blockIdx.x % p.bundles) * p.per, groups = min(p.per, p.G - g0), cg = p.C / p.G, width = groups * cg;
+    const int K = (width + V - 1) / V, RT = blockDim.x / K, t = threadIdx.x, col = t % K, r0 = t / K;
+    const bool on = r0 < RT;
+    const int own = col * V, c0 = min(own, width - V);
+    const long at = n * p.S * p.C + g0 * cg + c0;
+    const T* const x = reinterpret_cast<const T*>(p.x) + at;
+    Vec<T, V> v[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (on && r0 + u * RT < p.S) v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
+    const float scale = 1.f / ((float)p.S * (float)cg);
+    float s1[V] = {}, s2[V] = {}, m[V], r[V];
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (on && r0 + u * RT < p.S)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s1[j] += (float)v[u].v[j];
+    channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
+    group_sums(chan, groups, cg, [](int) { return 1.f; }, grp);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        m[j] = grp[2 * ((c0 + j) / cg)] * scale;
+        s1[j] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (on && r0 + u * RT < p.S)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = (float)v[u].v[j] - m[j];
+                s1[j] = fmaf(d, d, s1[j]);
+            }
+    __syncthreads();                               // every thread has its mean
+    if (t < groups) p.mean[n * p.G + g0 + t] = grp[2 * t] * scale;
+    __syncthreads();
+    channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
+    group_sums(chan, groups, cg, [](int) { return 1.f; }, grp);
+    if (t < groups) p.rstd[n * p.G + g0 + t] = 1.f / sqrtf(grp[2 * t] * scale + p.eps);
+    if (!on) return;
+    float b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        r[j] = 1.f / sqrtf(grp[2 * ((c0 + j) / cg)] * scale + p.eps) * load_param(p.w, p.wdtype, g0 * cg + c0 + j, 1.f);
+        b[j] = load_param(p.b, p.wdtype, g0 * cg + c0 + j, 0.f);
+    }
+    T* const y = reinterpret_cast<T*>(p.y) + at;
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (r0 + u * RT < p.S) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u].v[j] = (T)sed_act<ACT>(fmaf((float)v[u].v[j] - m[j], r[j], b[j]));
+            store_vec<T, V>(y + (long)(r0 + u * RT) * p.C, v[u]);
+        }
+}
+
+template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS) void norm_one_bwd_kernel(OneP p) {
+    extern __shared__ float scratch[];
+    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE];
+    const long n = blockIdx.x / p.bundles;
+    const int g0 = (int)(blockIdx.x % p.bundles) * p.per, groups = min(p.per, p.G - g0), cg = p.C / p.G, width = groups * cg;
+    const int K = (width + V - 1) / V, RT = blockDim.x / K, t = threadIdx.x, col = t % K, r0 = t / K;
+    const bool on = r0 < RT;
+    const int own = col * V, c0 = min(own, width - V);
+    const long at = n * p.S * p.C + g0 * cg + c0;
+    const T* const x = reinterpret_cast<const T*>(p.x) + at;
+    const T* const gy = reinterpret_cast<const T*>(p.gy) + at;
+    Vec<T, V> v[R], g[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (on && r0 + u * RT < p.S) {
+            v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
+            g[u] = load_vec<T, V>(gy + (long)(r0 + u * RT) * p.C);
+        }
+    float s1[V] = {}, s2[V] = {}, m[V], r[V], w[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = g0 * cg + c0 + j;
+        const long ng = n * p.G + c / cg;
+        m[j] = p.mean[ng];
+        r[j] = p.rstd[ng];
+        w[j] = load_param(p.w, p.wdtype, c, 1.f);
+        b[j] = load_param(p.b, p.wdtype, c, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (on && r0 + u * RT < p.S)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = ((float)v[u].v[j] - m[j]) * r[j];
+                const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
+                s1[j] += gz;
+                s2[j] = fmaf(gz, xh, s2[j]);
+            }
+    channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
+    for (int k = t; k < width; k += blockDim.x) {
+        p.chan[n * 2 * p.C + g0 * cg + k] = chan[k];
+        p.chan[n * 2 * p.C + p.C + g0 * cg + k] = chan[MAX_BUNDLE + k];
+    }
+    if (!p.y) return;
+    group_sums(chan, groups, cg, [&](int k) { return load_param(p.w, p.wdtype, g0 * cg + k, 1.f); }, grp);
+    if (!on) return;
+    const float scale = 1.f / ((float)p.S * (float)cg);
+    T* const gx = reinterpret_cast<T*>(p.y) + at;
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (r0 + u * RT < p.S) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int gr = (c0 + j) / cg;
+                const float xh = ((float)v[u].v[j] - m[j]) * r[j];
+                const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
+                v[u].v[j] = (T)(r[j] * (fmaf(gz, w[j], -grp[2 * gr] * scale) - xh * (grp[2 * gr + 1] * scale)));
+            }
+            store_vec<T, V>(gx + (long)(r0 + u * RT) * p.C, v[u]);
+        }
+}
+
 int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
 bool bad_shape(int dtype, int wdtype, long N, long S, int C, int G, int act) {
     return dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2 || N < 1 || S < 1 || C < 1 || G < 1 || C % G || act < 0 || act > 3 ||
            N * G > 0x7fffffffL || cut_of(N, S, C, esize_of(dtype)).blocks > 0x7fffffffL;
+}
+// How the one-pass kernels cut: bundles of whole groups with at least 128 bytes of a row (or all of it), a workgroup of so many threads
+// that each holds up to R vectors.  threads = 0: the rows do not fit, or a row has fewer channels than a vector.
+struct One {
+    int per, bundles, threads, R;
+};
+One one_of(long N, long S, int C, int G, int esize, int most) {
+    One o{};
+    const int V = 16 / esize, cg = C / G;
+    o.per = (128 / esize + cg - 1) / cg;
+    if (o.per > G) o.per = G;
+    // the last bundle has what is left: it must hold a vector too, else it joins its neighbours
+    while (o.per < G && (G % o.per ? G % o.per : o.per) * cg < V) ++o.per;
+    const long width = (long)o.per * cg;
+    o.bundles = (G + o.per - 1) / o.per;
+    const long K = (width + V - 1) / V;
+    if (C < V || width > MAX_BUNDLE || K > 256 || S > (long)ONE_THREADS * most || N * o.bundles > 0x7fffffffL) return o;
+    const long want = K * ((S + 3) / 4);           // four vectors a thread, as far as the threads go
+    o.threads = (int)(want < 64 ? 64 : want > ONE_THREADS ? ONE_THREADS : (want + 63) / 64 * 64);
+    if (o.threads < K) o.threads = (int)((K + 63) / 64 * 64);
+    const long each = (S + o.threads / K - 1) / (o.threads / K);
+    if (each > most) o.threads = 0;
+    else o.R = each <= 4 ? 4 : most;
+    return o;
 }
 NormP params_of(const Cut& c, const void* x, const void* w, const void* b, int wdtype, long S, int C, int G, float* ws) {
     NormP p{};
@@ -392,20 +645,43 @@ NormP params_of(const Cut& c, const void* x, const void* w, const void* b, int w
         else if (dtype == SED_F16) { WHAT(__VA_ARGS__, _Float16, 8) }                            \
         else { WHAT(__VA_ARGS__, __bf16, 8) }                                                    \
     }
+#define ONE_ACT(KERNEL, MOST, T, V)                                                                                                          \
+    switch (act) {                                                                                                                           \
+        case SED_ACT_NONE: ONE_R(KERNEL, MOST, T, V, 0) break;                                                                               \
+        case SED_ACT_RELU: ONE_R(KERNEL, MOST, T, V, 1) break;                                                                               \
+        case SED_ACT_SILU: ONE_R(KERNEL, MOST, T, V, 2) break;                                                                               \
+        default: ONE_R(KERNEL, MOST, T, V, 3)                                                                                                \
+    }
+#define ONE_R(KERNEL, MOST, T, V, ACT)                                                                                                       \
+    if (one.R == 4) hipLaunchKernelGGL((KERNEL<T, V, ACT, 4>), grid, dim3(one.threads), 2 * one.threads * V * 4, stream, p);                 \
+    else hipLaunchKernelGGL((KERNEL<T, V, ACT, MOST>), grid, dim3(one.threads), 2 * one.threads * V * 4, stream, p);
+#define ONE_TYPE(KERNEL, MOST)                                        \
+    if (dtype == SED_F32) { ONE_ACT(KERNEL, MOST, float, 4) }         \
+    else if (dtype == SED_F16) { ONE_ACT(KERNEL, MOST, _Float16, 8) } \
+    else { ONE_ACT(KERNEL, MOST, __bf16, 8) }
 #define NORM_PLAIN(KERNEL, T, V) hipLaunchKernelGGL((KERNEL<T, V>), grid, dim3(THREADS), 0, stream, p);
 
 }  // namespace
 
-SED_API long sed_group_norm_ws_floats(long N, long S, int C, int G, int backward) {
-    if (bad_shape(SED_F32, SED_F32, N, S, C, G, 0) || bad_shape(SED_F16, SED_F32, N, S, C, G, 0)) return 0;
-    const long a = cut_of(N, S, C, 4).chunks, b = cut_of(N, S, C, 2).chunks;
-    const long parts = N * (a > b ? a : b) * 2 * C;
+SED_API long sed_group_norm_ws_floats(int dtype, long N, long S, int C, int G, int backward) {
+    if (bad_shape(dtype, SED_F32, N, S, C, G, 0)) return 0;
+    if (one_of(N, S, C, G, esize_of(dtype), backward ? ONE_BWD : ONE_FWD).threads) return backward ? N * 2 * C : 0;
+    const long parts = N * cut_of(N, S, C, esize_of(dtype)).chunks * 2 * C;
     return backward ? parts + N * 2 * C + N * 2 * G : parts;
 }
 
 SED_API int sed_group_norm_fwd(const void* x, const void* weight, const void* bias, int dtype, int wdtype, long N, long S, int C, int G,
                                float eps, int act, void* y, float* mean, float* rstd, float* ws, sed_stream_t stream) {
-    if (!x || !y || !mean || !rstd || !ws || !(eps >= 0.f) || bad_shape(dtype, wdtype, N, S, C, G, act)) return SED_EINVAL;
+    if (!x || !y || !mean || !rstd || !(eps >= 0.f) || bad_shape(dtype, wdtype, N, S, C, G, act)) return SED_EINVAL;
+    const One one = one_of(N, S, C, G, esize_of(dtype), ONE_FWD);
+    if (!one.threads && !ws) return SED_EINVAL;
+    if (one.threads) {
+        const dim3 grid((unsigned)(N * one.bundles));
+        OneP p{x, nullptr, weight, bias, y, mean, rstd, nullptr, S, C, G, one.per, one.bundles, wdtype, eps};
+        ONE_TYPE(norm_one_kernel, ONE_FWD)
+        SED_LAUNCH_CHECK();
+        return 0;
+    }
     const Cut c = cut_of(N, S, C, esize_of(dtype));
     const dim3 grid((unsigned)c.blocks);
     NormP p = params_of(c, x, weight, bias, wdtype, S, C, G, ws);
@@ -418,9 +694,19 @@ SED_API int sed_group_norm_fwd(const void* x, const void* weight, const void* bi
 }
 
 SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const void* bias, int dtype, int wdtype, long N, long S,
-                               int C, int G, int act, const float* mean, const float* rstd, void* gx, float* gweight, float* gbias,
+                               int C, int G, int act, const float* mean, const float* rstd, void* gx, void* gweight, void* gbias,
                                float* ws, sed_stream_t stream) {
     if (!x || !gy || !mean || !rstd || !ws || bad_shape(dtype, wdtype, N, S, C, G, act)) return SED_EINVAL;
+    const One one = one_of(N, S, C, G, esize_of(dtype), ONE_BWD);
+    if (one.threads) {
+        const dim3 grid((unsigned)(N * one.bundles));
+        OneP p{x, gy, weight, bias, gx, const_cast<float*>(mean), const_cast<float*>(rstd), ws, S, C, G, one.per, one.bundles, wdtype, 0.f};
+        ONE_TYPE(norm_one_bwd_kernel, ONE_BWD)
+        if (gweight || gbias)
+            hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, ws, N, C, gweight, gbias, wdtype);
+        SED_LAUNCH_CHECK();
+        return 0;
+    }
     const Cut c = cut_of(N, S, C, esize_of(dtype));
     const dim3 grid((unsigned)c.blocks);
     NormP p = params_of(c, x, weight, bias, wdtype, S, C, G, ws);
@@ -428,9 +714,11 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
     float* const coef = chan + N * 2 * C;
     p.gy = gy; p.y = gx; p.mean = mean; p.rstd = rstd; p.coef = coef;
     NORM_TYPE(NORM_ACT, norm_bwd_sums_kernel)
-    hipLaunchKernelGGL(norm_bwd_fold_kernel, dim3((unsigned)(N * G)), dim3(128), 0, stream, ws, S, c.chunks, C, G, weight, wdtype, chan, coef);
+    const int cg = C / G, per = cg >= 64 ? 1 : 64 / cg < G ? 64 / cg : G;
+    hipLaunchKernelGGL(norm_bwd_fold_kernel, dim3((unsigned)(N * ((G + per - 1) / per))), dim3(256), 0, stream, ws, S, c.chunks, C, G, per, weight, wdtype,
+                       chan, coef);
     if (gweight || gbias)
-        hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(256), 0, stream, chan, N, C, gweight, gbias);
+        hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, chan, N, C, gweight, gbias, wdtype);
     if (gx) { NORM_TYPE(NORM_ACT, norm_bwd_apply_kernel) }
     SED_LAUNCH_CHECK();
     return 0;

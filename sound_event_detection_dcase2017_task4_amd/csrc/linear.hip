@@ -459,20 +459,28 @@ template <typename T, int U> void launch_rows(const T* x, const T* w, int M, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------- passes around them
-// copy of [R][C] with lines of ld elements, zeros behind the C-th: operands whose lines do not begin at multiples of 16 bytes
-template <typename T> __global__ __launch_bounds__(256) void pad_kernel(const T* src, long R, int C, int ld, T* dst) {
+// copies of up to two [R][C] with lines of ld elements, zeros behind the C-th: operands whose lines do not begin at multiples of 16 bytes
+struct PadP {
+    const void* src[2];
+    void* dst[2];
+    long R[2];
+    int C, ld;
+};
+template <typename T> __global__ __launch_bounds__(256) void pad_kernel(PadP p) {
     constexpr int E = 16 / sizeof(T);
-    const int per = ld / E;
-    const long total = R * per;
+    const int per = p.ld / E;
+    const long first = p.R[0] * per, total = first + p.R[1] * per;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long r = i / per;
+        const int which = i >= first;
+        const long r = (i - which * first) / per;
         const int c = (int)(i % per) * E;
+        const T* const src = reinterpret_cast<const T*>(p.src[which]) + r * p.C + c;
         T v[E];
-        if (c + E <= C) __builtin_memcpy(v, src + r * C + c, 16);
+        if (c + E <= p.C) __builtin_memcpy(v, src, 16);
         else
 #pragma unroll
-            for (int j = 0; j < E; ++j) v[j] = c + j < C ? src[r * C + c + j] : (T)0.f;
-        __builtin_memcpy(dst + r * ld + c, v, 16);
+            for (int j = 0; j < E; ++j) v[j] = c + j < p.C ? src[j] : (T)0.f;
+        __builtin_memcpy(reinterpret_cast<T*>(p.dst[which]) + r * p.ld + c, v, 16);
     }
 }
 
@@ -592,7 +600,7 @@ Plan plan_of(long M, long N, long K, int esize) {
             const long per = (steps + s - 1) / s, slices = (steps + per - 1) / per, on = (tm * tn * slices + 255) / 256;
             float t = (float)(on / room[e]) * (per * us[room[e] - 1] + ends[e]);
             if (on % room[e]) t += per * us[on % room[e] - 1] + ends[e];
-            if (slices > 1) t += 4.f + (float)slices * M * N * 8.f / 5e6f;
+            if (slices > 1) t += 6.f + (float)slices * M * N * 8.f / 5e6f;
             if (best.edge && t >= least) continue;
             least = t;
             best.edge = edges[e]; best.tm = (int)tm; best.tn = (int)tn; best.slices = (int)slices; best.kslice = per * step;
@@ -630,13 +638,21 @@ template <typename T, bool PROWS, bool QROWS> int launch_gemm(GemmP a, const Pla
     SED_LAUNCH_CHECK();
     return 0;
 }
-template <typename T> const T* pad(const void* src, long R, long C, char*& ws, hipStream_t stream) {
-    const int ld = (int)padded(C, sizeof(T));
-    T* const dst = reinterpret_cast<T*>(ws);
-    ws += up256(R * ld * (long)sizeof(T));
-    const long total = R * (ld * (long)sizeof(T) / 16), nb = (total + 255) / 256;
-    hipLaunchKernelGGL((pad_kernel<T>), dim3((unsigned)(nb > 16384 ? 16384 : nb)), dim3(256), 0, stream, reinterpret_cast<const T*>(src), R, (int)C, ld, dst);
-    return dst;
+// x [M][C] and w [N][C] with lines of a multiple of 16 bytes, those of them that need it, in one launch
+template <typename T> void pad(const void*& x, long M, bool px, const void*& w, long N, bool pw, long C, char*& ws, hipStream_t stream) {
+    if (!px && !pw) return;
+    PadP p{};
+    p.C = (int)C; p.ld = (int)padded(C, sizeof(T));
+    auto take = [&](int i, const void*& src, long R) {
+        p.src[i] = src; p.R[i] = R; p.dst[i] = ws;
+        src = ws;
+        ws += up256(R * p.ld * (long)sizeof(T));
+    };
+    int used = 0;
+    if (px) take(used++, x, M);
+    if (pw) take(used++, w, N);
+    const long nb = ((p.R[0] + p.R[1]) * (p.ld * (long)sizeof(T) / 16) + 255) / 256;
+    hipLaunchKernelGGL((pad_kernel<T>), dim3((unsigned)(nb > 16384 ? 16384 : nb)), dim3(256), 0, stream, p);
 }
 
 // rows and columns that 32-bit tile counts and 32-bit offsets inside a tile can hold
@@ -679,11 +695,11 @@ int linear_fwd(const void* x, const void* w, const void* bias, const void* res, 
         return 0;
     }
     const long ld = padded(K, sizeof(T));
-    const bool px = needs_pad(x, K, sizeof(T)), pw = needs_pad(w, K, sizeof(T));
+    pad<T>(x, M, needs_pad(x, K, sizeof(T)), w, N, needs_pad(w, K, sizeof(T)), K, ws, stream);
     GemmP a{};
     a.M = (int)M; a.N = (int)N; a.K = ld; a.e = e;
-    a.q = {px ? pad<T>(x, M, K, ws, stream) : x, ld, (int)M};
-    a.p = {pw ? pad<T>(w, N, K, ws, stream) : w, ld, (int)N};
+    a.q = {x, ld, (int)M};
+    a.p = {w, ld, (int)N};
     return launch_gemm<T, false, false>(a, plan_of(M, N, ld, sizeof(T)), reinterpret_cast<float*>(ws), stream);
 }
 
@@ -732,8 +748,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
     }
     if (gb) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(1024), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
     const void* const dz = gz ? gz : gy;
-    const void* const xp = d.px ? pad<T>(x, M, K, ws, stream) : x;
-    const void* const wp = d.pw ? pad<T>(w, N, K, ws, stream) : w;
+    pad<T>(x, M, d.px, w, N, d.pw, K, ws, stream);
     SED_LAUNCH_CHECK();
     const bool wide = K % (16 / es) == 0;
     if (gx) {
@@ -741,7 +756,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         a.M = (int)M; a.N = (int)K; a.K = ldn;
         a.e.y = gx; a.e.wide = wide && aligned16(gx);
         a.q = {dz, ldn, (int)M};
-        a.p = {wp, ldk, (int)ldk};
+        a.p = {w, ldk, (int)ldk};
         // gz has zeros behind its N-th column, W has no line there: k ends at N for W's lines and at ldn for gz's pieces
         a.K = N;
         const int rc = launch_gemm<T, true, false>(a, plan_of(M, K, ldn, es), reinterpret_cast<float*>(ws), stream);
@@ -752,7 +767,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         a.M = (int)N; a.N = (int)K; a.K = M;
         a.e.y = gw; a.e.wide = wide && aligned16(gw);
         a.q = {dz, ldn, (int)ldn};
-        a.p = {xp, ldk, (int)ldk};
+        a.p = {x, ldk, (int)ldk};
         return launch_gemm<T, true, true>(a, plan_of(N, K, M, es), reinterpret_cast<float*>(ws), stream);
     }
     return 0;

@@ -1967,26 +1967,57 @@ def _act_code(activation):
     return ACTIVATIONS[activation]
 
 
-def _chk_operand(name, t, shape, dtypes, device):
-    """A further operand of an operator whose first one fixes device and sizes."""
-    if tuple(t.shape) != tuple(shape):
+def _chk_operand(name, t, shape, dtype, other, device):
+    """A further operand of an operator whose first one fixes device and sizes; `other`: a second type it may have."""
+    if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if t.dtype not in dtypes:
-        raise ValueError("%s must be %s, got %s" % (name, " or ".join(str(d) for d in dtypes), t.dtype))
+    if t.dtype is not dtype and t.dtype is not other:
+        raise ValueError("%s must be %s, got %s" % (name, dtype if other is dtype else "%s or %s" % (dtype, other), t.dtype))
     if t.device != device:
         raise ValueError("%s is on %s, the input on %s" % (name, t.device, device))
 
 
+def _bytes(n, device):
+    return torch.empty((n,), dtype=torch.uint8, device=device) if n else None
+
+
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _group_norm_fwd(x, weight, bias, groups, eps, act):
     C = x.shape[-1]
-    N, S = x.shape[0], x.numel() // (x.shape[0] * C)
+    N = x.shape[0]
+    S = x.numel() // (N * C)
+    h = _lib.lib()
     y = torch.empty_like(x)
-    stats = torch.empty((2, N, groups), dtype=torch.float32, device=x.device)
-    ws = torch.empty((int(_lib.lib().sed_group_norm_ws_floats(N, S, C, groups, 0)),), dtype=torch.float32, device=x.device)
-    _call("sed_group_norm_fwd", _ptr(x), _ptr(weight), _ptr(bias), DTYPE_CODES[x.dtype],
-          DTYPE_CODES[weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32], N, S, C, groups, eps,
-          act, _ptr(y), stats.data_ptr(), stats.data_ptr() + 4 * N * groups, _ptr(ws), _stream())
+    stats = torch.empty((2 * N * groups,), dtype=torch.float32, device=x.device)           # mean, 1 / sigma
+    at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
+    ws = _bytes(4 * int(h.sed_group_norm_ws_floats(dt, N, S, C, groups, 0)), x.device)
+    par = weight if weight is not None else bias
+    _call("sed_group_norm_fwd", x.data_ptr(), _ptr(weight), _ptr(bias), dt, DTYPE_CODES[par.dtype] if par is not None else 0,
+          N, S, C, groups, eps, act, y.data_ptr(), at, at + 4 * N * groups, _ptr(ws), _stream())
     return y, stats
+
+
+def _group_norm_bwd(ctx, gy):
+    x, weight, bias, stats = ctx.saved_tensors
+    gy = _contiguous(gy)
+    C, G, N = x.shape[-1], ctx.groups, x.shape[0]
+    S = x.numel() // (N * C)
+    par = weight if weight is not None else bias
+    want = ctx.needs_input_grad
+    h = _lib.lib()
+    with _on_device(x):
+        gx = torch.empty_like(x) if want[0] else None
+        gw = torch.empty_like(weight) if want[1] else None
+        gb = torch.empty_like(bias) if want[2] else None
+        at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
+        ws = _bytes(4 * int(h.sed_group_norm_ws_floats(dt, N, S, C, G, 1)), x.device)
+        _call("sed_group_norm_bwd", x.data_ptr(), gy.data_ptr(), _ptr(weight), _ptr(bias), dt,
+              DTYPE_CODES[par.dtype] if par is not None else 0, N, S, C, G, ctx.act, at, at + 4 * N * G, _ptr(gx), _ptr(gw), _ptr(gb),
+              _ptr(ws), _stream())
+    return gx, gw, gb, None, None, None
 
 
 class GroupNormActFn(torch.autograd.Function):
@@ -1995,31 +2026,18 @@ class GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
         with _on_device(x):
-            y, stats = _group_norm_fwd(x, weight, bias, groups, eps, act)
-        ctx.save_for_backward(x, weight, bias, stats)
+            x = _contiguous(x)
+            y, stats = _group_norm_fwd(x, _contiguous(weight), _contiguous(bias), groups, eps, act)
+        ctx.save_for_backward(x, _contiguous(weight), _contiguous(bias), stats)
         ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, weight, bias, stats = ctx.saved_tensors
-        gy = gy.contiguous()
-        C, G = x.shape[-1], ctx.groups
-        N, S = x.shape[0], x.numel() // (x.shape[0] * C)
-        par = weight if weight is not None else bias
-        want = ctx.needs_input_grad
-        with _on_device(x):
-            gx = torch.empty_like(x) if want[0] else None
-            gp = torch.empty((2, C), dtype=torch.float32, device=x.device) if want[1] or want[2] else None
-            ws = torch.empty((int(_lib.lib().sed_group_norm_ws_floats(N, S, C, G, 1)),), dtype=torch.float32, device=x.device)
-            _call("sed_group_norm_bwd", _ptr(x), _ptr(gy), _ptr(weight), _ptr(bias), DTYPE_CODES[x.dtype],
-                  DTYPE_CODES[par.dtype if par is not None else torch.float32], N, S, C, G, ctx.act, stats.data_ptr(),
-                  stats.data_ptr() + 4 * N * G, _ptr(gx), gp[0].data_ptr() if want[1] else None, gp[1].data_ptr() if want[2] else None,
-                  _ptr(ws), _stream())
-            gw = gp[0].to(weight.dtype) if want[1] else None
-            gb = gp[1].to(bias.dtype) if want[2] else None
-        return gx, gw, gb, None, None, None
+        return _once_group_norm_bwd(ctx, gy) if torch.is_grad_enabled() else _group_norm_bwd(ctx, gy)
+
+
+_once_group_norm_bwd = torch.autograd.function.once_differentiable(_group_norm_bwd)
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
@@ -2039,39 +2057,61 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         raise ValueError("groups must divide the channels: %d channels, %d groups" % (C, groups))
     if not eps >= 0.0:
         raise ValueError("eps must not be negative, got %r" % (eps,))
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _chk_operand(name, t, (C,), (torch.float32, x.dtype), x.device)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one type, got %s and %s" % (weight.dtype, bias.dtype))
+    if weight is not None:
+        _chk_operand("weight", weight, (C,), torch.float32, x.dtype, x.device)
+    if bias is not None:
+        _chk_operand("bias", bias, (C,), torch.float32, x.dtype, x.device)
+        if weight is not None and bias.dtype != weight.dtype:
+            raise ValueError("weight and bias must have one type, got %s and %s" % (weight.dtype, bias.dtype))
     _chk_dev(x)
+    grad = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
     if x.numel() == 0:
         y = torch.zeros_like(x)
         for t in (x, weight, bias):                       # stays part of the graph, with gradients of zero
-            y = y if t is None or not (torch.is_grad_enabled() and t.requires_grad) else y + t.sum().to(x.dtype) * 0
+            y = y + t.sum().to(x.dtype) * 0 if grad and t is not None and t.requires_grad else y
         return y
-    weight = weight if weight is None else weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
-    x = x.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if grad:
         return GroupNormActFn.apply(x, weight, bias, groups, float(eps), act)
     with _on_device(x):
-        return _group_norm_fwd(x, weight, bias, groups, float(eps), act)[0]
+        return _group_norm_fwd(_contiguous(x), _contiguous(weight), _contiguous(bias), groups, float(eps), act)[0]
 
 
 def _linear_fwd(x, weight, bias, residual, act, keep):
-    """x (M, K), all contiguous -> y (M, N) and, with keep, what the backward pass needs of z (None without an activation)."""
-    (M, K), N, dt = x.shape, weight.shape[0], DTYPE_CODES[x.dtype]
+    """x (..., K), all contiguous -> y (..., N) and, with keep, what the backward pass needs of z (None without an activation)."""
+    N, K = weight.shape
+    M, dt = x.numel() // K, DTYPE_CODES[x.dtype]
     h = _lib.lib()
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
     z = None
     if keep and act:
-        z = torch.empty((int(h.sed_linear_kept_elements(M, N)),), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device)
-    need = int(h.sed_linear_fwd_ws_bytes(_ptr(x), _ptr(weight), dt, M, N, K))
-    ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
-    _call("sed_linear_fwd", _ptr(x), _ptr(weight), _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt,
-          M, N, K, act, _ptr(y), _ptr(z), _ptr(ws), need, _stream())
+        z = torch.empty((int(h.sed_linear_kept_elements(M, N)),), dtype=torch.float16 if dt else torch.float32, device=x.device)
+    px, pw = x.data_ptr(), weight.data_ptr()
+    need = int(h.sed_linear_fwd_ws_bytes(px, pw, dt, M, N, K))
+    ws = _bytes(need, x.device)
+    _call("sed_linear_fwd", px, pw, _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt, M, N, K, act,
+          y.data_ptr(), _ptr(z), _ptr(ws), need, _stream())
     return y, z
+
+
+def _linear_bwd(ctx, gy):
+    want = ctx.needs_input_grad
+    if not (want[0] or want[1] or want[2]):
+        return None, None, None, gy, None
+    x, weight, z = ctx.saved_tensors
+    g = _contiguous(gy)
+    N, K = weight.shape
+    M, dt = x.numel() // K, DTYPE_CODES[x.dtype]
+    h = _lib.lib()
+    with _on_device(x):
+        gx = torch.empty_like(x) if want[0] else None
+        gw = torch.empty_like(weight) if want[1] else None
+        gb = torch.empty((N,), dtype=ctx.btype, device=x.device) if want[2] else None
+        px, pw, pg = x.data_ptr(), weight.data_ptr(), g.data_ptr()
+        need = int(h.sed_linear_bwd_ws_bytes(px, pw, pg, dt, M, N, K, ctx.act, want[0], want[1], want[2]))
+        ws = _bytes(need, x.device)
+        _call("sed_linear_bwd", px, pw, pg, _ptr(z), dt, DTYPE_CODES[ctx.btype] if want[2] else dt, M, N, K, ctx.act, _ptr(gx), _ptr(gw),
+              _ptr(gb), _ptr(ws), need, _stream())
+    return gx, gw, gb, gy if want[3] else None, None
 
 
 class LinearActFn(torch.autograd.Function):
@@ -2079,31 +2119,20 @@ class LinearActFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
+        want = ctx.needs_input_grad
         with _on_device(x):
-            y, z = _linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+            x, weight = _contiguous(x), _contiguous(weight)
+            y, z = _linear_fwd(x, weight, _contiguous(bias), _contiguous(residual), act, want[0] or want[1] or want[2])
         ctx.save_for_backward(x, weight, z)
         ctx.act, ctx.btype = act, bias.dtype if bias is not None else None
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, weight, z = ctx.saved_tensors
-        want = ctx.needs_input_grad
-        gx = gw = gb = None
-        if any(want[:3]):
-            g = gy.contiguous()
-            (M, K), N, dt = x.shape, weight.shape[0], DTYPE_CODES[x.dtype]
-            h = _lib.lib()
-            with _on_device(x):
-                gx = torch.empty_like(x) if want[0] else None
-                gw = torch.empty_like(weight) if want[1] else None
-                gb = torch.empty((N,), dtype=ctx.btype, device=x.device) if want[2] else None
-                need = int(h.sed_linear_bwd_ws_bytes(_ptr(x), _ptr(weight), _ptr(g), dt, M, N, K, ctx.act, want[0], want[1], want[2]))
-                ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
-                _call("sed_linear_bwd", _ptr(x), _ptr(weight), _ptr(g), _ptr(z), dt, DTYPE_CODES[ctx.btype] if want[2] else dt, M, N, K,
-                      ctx.act, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), need, _stream())
-        return gx, gw, gb, gy if want[3] else None, None
+        return _once_linear_bwd(ctx, gy) if torch.is_grad_enabled() else _linear_bwd(ctx, gy)
+
+
+_once_linear_bwd = torch.autograd.function.once_differentiable(_linear_bwd)
 
 
 def linear_act(x, weight, bias=None, activation="none", residual=None):
@@ -2111,34 +2140,32 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
 
     x, weight and residual: float32, float16 or bfloat16, all of one type (any strides; non-contiguous ones are copied); bias: that
     type or float32.  activation: 'none', 'relu', 'silu', 'gelu' (z Phi(z)).  Sums are held in 32 bits and y is rounded once; the
-    backward pass rounds gz = gy act'(z) to x's type for its two products.  Up to 64 rows the product is one pass over W (single
-    frames of a stream); an x without rows gives a y without rows."""
+    backward pass rounds gz = gy act'(z) to x's type for its two products.  A few rows are one pass over W (single frames of a
+    stream); an x without rows gives a y without rows."""
     act = _act_code(activation)
-    if x.dtype not in DTYPE_CODES:
-        raise ValueError("x must be float32, float16 or bfloat16, got %s" % x.dtype)
+    dtype, device = x.dtype, x.device
+    if dtype not in DTYPE_CODES:
+        raise ValueError("x must be float32, float16 or bfloat16, got %s" % dtype)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError("x (..., K) and weight (N, K) do not fit: %s and %s" % (tuple(x.shape), tuple(weight.shape)))
-    N, K = weight.shape
-    shape = tuple(x.shape[:-1]) + (N,)
-    _chk_operand("weight", weight, (N, K), (x.dtype,), x.device)
+    N = weight.shape[0]
+    _chk_operand("weight", weight, weight.shape, dtype, dtype, device)
     if bias is not None:
-        _chk_operand("bias", bias, (N,), (x.dtype, torch.float32), x.device)
+        _chk_operand("bias", bias, (N,), dtype, torch.float32, device)
     if residual is not None:
-        _chk_operand("residual", residual, shape, (x.dtype,), x.device)
+        _chk_operand("residual", residual, x.shape[:-1] + (N,), dtype, dtype, device)
     _chk_dev(x)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                        or (residual is not None and residual.requires_grad))
     if x.numel() == 0:
-        y = torch.zeros(shape, dtype=x.dtype, device=x.device)
+        y = torch.zeros(x.shape[:-1] + (N,), dtype=dtype, device=device)
         for t in (x, weight, bias, residual):             # stays part of the graph, with gradients of zero
-            y = y + t.sum().to(x.dtype) * 0 if grad and t is not None and t.requires_grad else y
+            y = y + t.sum().to(dtype) * 0 if grad and t is not None and t.requires_grad else y
         return y
-    x2, weight = x.contiguous().view(-1, K), weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
-    r2 = residual if residual is None else residual.contiguous().view(-1, N)
     if grad:
-        return LinearActFn.apply(x2, weight, bias, r2, act).view(shape)
+        return LinearActFn.apply(x, weight, bias, residual, act)
     with _on_device(x):
-        return _linear_fwd(x2, weight, bias, r2, act, False)[0].view(shape)
+        return _linear_fwd(_contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), act, False)[0]
 
 
 def adamw_(rows, chunks, nchunks, m, v, m_scale, v_scale, master, state_bits, hyper, step, grad_scale=1.0, guard=None, skipped=None):

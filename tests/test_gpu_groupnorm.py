@@ -268,8 +268,10 @@ def test_c_entries_refuse_bad_arguments():
     def bwd(**kw):
         a = dict(ok, **kw)
         return h.sed_group_norm_bwd(a["x"], a["y"], a["w"], a["b"], a["t"], a["wt"], a["N"], a["S"], a["C"], a["G"], a["act"], a["m"], a["r"], None, None, None, a["ws"], None)
-    for bad in ({"x": None}, {"y": None}, {"m": None}, {"r": None}, {"ws": None}, {"t": 3}, {"t": -1}, {"wt": 3}, {"N": 0}, {"S": 0}, {"C": 0}, {"G": 3},
+    for bad in ({"x": None}, {"y": None}, {"m": None}, {"r": None}, {"t": 3}, {"t": -1}, {"wt": 3}, {"N": 0}, {"S": 0}, {"C": 0}, {"G": 3},
                 {"G": 0}, {"act": 4}, {"act": -1}, {"N": 1 << 40}):
         assert fwd(**bad) == -22 and bwd(**bad) == -22, bad
     assert fwd(eps=-1.0) == -22 and fwd(eps=float("nan")) == -22
-    assert h.sed_group_norm_ws_floats(2, 3, 8, 3, 0) == 0 and h.sed_group_norm_ws_floats(2, 3, 8, 2, 1) > 0
+    assert fwd(S=1 << 20, ws=None) == -22
+    assert h.sed_group_norm_ws_floats(0, 2, 3, 8, 3, 0) == 0 and h.sed_group_norm_ws_floats(0, 2, 3, 8, 2, 1) > 0
+    assert h.sed_group_norm_ws_floats(0, 2, 1 << 20, 8, 2, 0) > 0
