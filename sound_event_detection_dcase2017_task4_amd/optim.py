@@ -407,7 +407,7 @@ class FusedAdamW(object):
         self._rows[:, 2], self._rows[:, 3] = self.offsets, self._copy_at
         self._rows[:, 4] = [p.numel() for p in self.params]
         self._rows[:, 5] = [k | ops.DTYPE_CODES[p.dtype] << 32 for k, p in zip(group, self.params)]
-        self._sent = self._dev_rows = self._sent_on = None
+        self._sent = self._dev_rows = None
         per = int(ops._lib.lib().sed_adamw_chunk())
         count = -(-self._rows[:, 4] // per)
         first = np.repeat(np.cumsum(count) - count, count)
@@ -460,28 +460,25 @@ class FusedAdamW(object):
     def _table(self):
         """Device table of this step's tensors; the gradients it points to are returned with it and stay alive until the launch."""
         grads = [p.grad for p in self.params]
-        if not all(g is None or g.is_contiguous() for g in grads):
+        if not all([g is None or g.is_contiguous() for g in grads]):
             grads = [g if g is None else g.contiguous() for g in grads]
+        at = [p.data_ptr() for p in self.params], [p.numel() for p in self.params], [0 if g is None else g.data_ptr() for g in grads], ops._stream()
+        if at == self._sent:                       # every address and size as in the table that the kernel read last, on the same stream
+            return grads
         rows = self._rows
-        where = [p.data_ptr() for p in self.params]
-        if where != self._sent_params():
+        if self._sent is None or at[:2] != self._sent[:2]:
             self._check_params()
-            if [p.numel() for p in self.params] != rows[:, 4].tolist() or [ops.DTYPE_CODES[p.dtype] for p in self.params] != (rows[:, 5] >> 32).tolist():
+            if at[1] != rows[:, 4].tolist() or [ops.DTYPE_CODES[p.dtype] for p in self.params] != (rows[:, 5] >> 32).tolist():
                 raise ValueError("FusedAdamW: a parameter changed its size or type since the optimiser was made")
-            rows[:, 0] = where
-        rows[:, 1] = [0 if g is None else g.data_ptr() for g in grads]
         for p, g in zip(self.params, grads):
-            if g is not None and (g.dtype != p.dtype or g.device != p.device or g.layout != torch.strided):
-                raise ValueError("FusedAdamW: a gradient of type %s on %s for a parameter of type %s on %s" % (g.dtype, g.device, p.dtype, p.device))
-        stream = ops._stream()
-        if self._sent is None or self._sent_on != stream or not np.array_equal(self._sent, rows):
-            # uploaded on the stream that reads it, into new memory: a step still in flight keeps the table it was given
-            self._dev_rows = ops.upload_small(rows, self.device, torch.int64)
-            self._sent, self._sent_on = rows.copy(), stream
+            if g is not None and (g.dtype != p.dtype or g.device != p.device or g.numel() != p.numel()):
+                raise ValueError("FusedAdamW: a gradient %s of type %s on %s for a parameter %s of type %s on %s"
+                                 % (tuple(g.shape), g.dtype, g.device, tuple(p.shape), p.dtype, p.device))
+        rows[:, 0], rows[:, 1] = at[0], at[2]
+        # uploaded on the stream that reads it, into new memory: a step still in flight keeps the table it was given
+        self._dev_rows = ops.upload_small(rows, self.device, torch.int64)
+        self._sent = at
         return grads
-
-    def _sent_params(self):
-        return None if self._sent is None else self._sent[:, 0].tolist()
 
     @torch.no_grad()
     def step(self, grad_scale=1.0):

@@ -297,7 +297,7 @@ def test_more_than_two_to_the_31_elements():
     p.grad[5] = 1.0
     opt = optim.FusedAdamW([p], lr=0.5, weight_decay=0.0, state_bits=8)
     opt.step()
-    assert torch.equal(p.detach()[-300:], torch.full((300,), -0.5, dtype=torch.float16, device="cuda")) and float(p[5]) == -0.5
+    assert torch.equal(p.detach()[-300:], torch.full((300,), -0.5, dtype=torch.float16, device="cuda")) and float(p.detach()[5]) == -0.5
     assert not p.detach()[6:100000].any() and not p.detach()[-100000:-300].any()
     assert int((opt.exp_avg[:n] != 0).sum()) == 301
 
@@ -316,10 +316,14 @@ def test_refusals_on_the_gpu():
         optim.FusedAdamW(flat.params)
     opt = optim.FusedAdamW([p])
     p.grad = torch.ones_like(p)
-    p.data = torch.ones(5, 6, device="cuda")
-    with pytest.raises(ValueError):
-        opt.step()
-    assert opt.step_count == 0
+    opt.step()
+    for smaller in (torch.ones(5, 6, device="cuda"), p.data[:2]):      # the second one at the same address
+        p.data = smaller
+        p.grad = None
+        p.grad = torch.ones_like(p)
+        with pytest.raises(ValueError):
+            opt.step()
+    assert opt.step_count == 1
 
 
 def test_refusals_on_the_cpu():
