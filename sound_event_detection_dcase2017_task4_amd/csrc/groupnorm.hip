@@ -18,7 +18,9 @@ SED_OBJECT_FLAGS(groupnorm)
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int UNROLL = 4;
+// rows that a thread has in flight: the backward passes read two tensors, and are slower with more registers a thread (65 M bf16 elements,
+// sums and gx: 63 and 73 us with two rows, 79 and 97 with four, 74 and 73 with one)
+constexpr int UNROLL = 4, BWD_UNROLL = 2;
 
 // How a launch cuts the tensor: CT column vectors (of K a row) x RT row lanes per workgroup, `tiles` column tiles, chunks of rows.
 struct Cut {
@@ -244,16 +246,16 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
             w[j] = load_param(p.w, p.wdtype, c, 1.f);
             b[j] = load_param(p.b, p.wdtype, c, 0.f);
         }
-        for (long s = q.s0 + q.r; s < q.s1; s += (long)p.RT * UNROLL) {
-            Vec<T, V> v[UNROLL], g[UNROLL];
+        for (long s = q.s0 + q.r; s < q.s1; s += (long)p.RT * BWD_UNROLL) {
+            Vec<T, V> v[BWD_UNROLL], g[BWD_UNROLL];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
+            for (int u = 0; u < BWD_UNROLL; ++u)
                 if (s + (long)u * p.RT < q.s1) {
                     v[u] = load_vec<T, V>(x + (s + (long)u * p.RT) * p.C);
                     g[u] = load_vec<T, V>(gy + (s + (long)u * p.RT) * p.C);
                 }
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
+            for (int u = 0; u < BWD_UNROLL; ++u)
                 if (s + (long)u * p.RT < q.s1)
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
@@ -367,16 +369,16 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
         c1[j] = p.coef[2 * ng];
         c2[j] = p.coef[2 * ng + 1];
     }
-    for (long s = q.s0 + q.r; s < q.s1; s += (long)p.RT * UNROLL) {
-        Vec<T, V> v[UNROLL], g[UNROLL];
+    for (long s = q.s0 + q.r; s < q.s1; s += (long)p.RT * BWD_UNROLL) {
+        Vec<T, V> v[BWD_UNROLL], g[BWD_UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < BWD_UNROLL; ++u)
             if (s + (long)u * p.RT < q.s1) {
                 v[u] = load_vec<T, V>(x + (s + (long)u * p.RT) * p.C);
                 g[u] = load_vec<T, V>(gy + (s + (long)u * p.RT) * p.C);
             }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < BWD_UNROLL; ++u)
             if (s + (long)u * p.RT < q.s1) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
