@@ -491,6 +491,8 @@ struct GradP {
     const void* z;
     void* gz;
     float* sums;                                   // nullable, [chunks][ld]
+    void* gb;                                      // where there is one chunk, its sums are the result, of btype
+    int btype;
     long M, rows;
     int N, ld, CT, RT, tiles, act;
 };
@@ -533,7 +535,7 @@ template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) voi
                 if (p.gz) __builtin_memcpy(reinterpret_cast<T*>(p.gz) + at * p.ld + c, g[u], 16);
             }
         }
-    if (!p.sums) return;
+    if (!p.sums && !p.gb) return;
 #pragma unroll
     for (int j = 0; j < E; ++j) red[t * E + j] = sum[j];
     __syncthreads();
@@ -541,7 +543,8 @@ template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) voi
         float v = 0.f;
         for (int i = 0; i < p.RT; ++i) v += red[i * p.CT * E + k];
         const int n = tile * p.CT * E + k;
-        if (n < p.ld) p.sums[chunk * p.ld + n] = v;
+        if (p.gb && n < p.N) store_typed(p.gb, p.btype, n, v);
+        else if (p.sums && n < p.ld) p.sums[chunk * p.ld + n] = v;
     }
 }
 template <typename T, bool WHOLE> void launch_act_grad(const GradP& p, unsigned blocks, hipStream_t stream) {
@@ -675,6 +678,7 @@ GradCut grad_cut(long M, long ld, int esize) {
     long rows = (M + want - 1) / want;
     const long lo = (long)c.RT * 4, hi = (long)c.RT * 64;
     rows = rows < lo ? lo : (rows > hi ? hi : rows);
+    if (M <= 4 * lo) rows = M;                              // a few rows in one chunk: a launch less
     c.rows = rows;
     c.chunks = (M + rows - 1) / rows;
     return c;
@@ -742,11 +746,12 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         ws += up256(c.chunks * ldn * 4);
     }
     if (gz || gb) {
-        GradP p{gy, z, gz, sums, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act};
+        const bool one = gb && c.chunks == 1;
+        GradP p{gy, z, gz, one ? nullptr : sums, one ? gb : nullptr, btype, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act};
         if (N % (16 / es) == 0) launch_act_grad<T, true>(p, (unsigned)(c.chunks * c.tiles), stream);
         else launch_act_grad<T, false>(p, (unsigned)(c.chunks * c.tiles), stream);
     }
-    if (gb) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(1024), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
+    if (gb && c.chunks > 1) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(1024), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
     const void* const dz = gz ? gz : gy;
     pad<T>(x, M, d.px, w, N, d.pw, K, ws, stream);
     SED_LAUNCH_CHECK();

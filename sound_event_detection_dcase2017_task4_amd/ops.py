@@ -1941,21 +1941,12 @@ def guard_publish(flag_out):
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}       # SED_F32, SED_F16, SED_BF16
 
 
-class _on_device(object):
-    """Makes the device of `t` the current one around a launch (its current stream is then the one that is used)."""
-
-    def __init__(self, t):
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-        return False
+def _there(t, f, *args):
+    """f(*args) with t's device as the current one: its current stream is then the one that is used."""
+    if t.device.index == torch._C._cuda_getDevice():
+        return f(*args)
+    with torch.cuda.device(t.device):
+        return f(*args)
 
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}                  # SED_ACT_*; gelu is z Phi(z)
@@ -1989,11 +1980,10 @@ def _group_norm_fwd(x, weight, bias, groups, eps, act):
     C = x.shape[-1]
     N = x.shape[0]
     S = x.numel() // (N * C)
-    h = _lib.lib()
     y = torch.empty_like(x)
     stats = torch.empty((2 * N * groups,), dtype=torch.float32, device=x.device)           # mean, 1 / sigma
     at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
-    ws = _bytes(4 * int(h.sed_group_norm_ws_floats(dt, N, S, C, groups, 0)), x.device)
+    ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, groups, 0), x.device)
     par = weight if weight is not None else bias
     _call("sed_group_norm_fwd", x.data_ptr(), _ptr(weight), _ptr(bias), dt, DTYPE_CODES[par.dtype] if par is not None else 0,
           N, S, C, groups, eps, act, y.data_ptr(), at, at + 4 * N * groups, _ptr(ws), _stream())
@@ -2007,16 +1997,14 @@ def _group_norm_bwd(ctx, gy):
     S = x.numel() // (N * C)
     par = weight if weight is not None else bias
     want = ctx.needs_input_grad
-    h = _lib.lib()
-    with _on_device(x):
-        gx = torch.empty_like(x) if want[0] else None
-        gw = torch.empty_like(weight) if want[1] else None
-        gb = torch.empty_like(bias) if want[2] else None
-        at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
-        ws = _bytes(4 * int(h.sed_group_norm_ws_floats(dt, N, S, C, G, 1)), x.device)
-        _call("sed_group_norm_bwd", x.data_ptr(), gy.data_ptr(), _ptr(weight), _ptr(bias), dt,
-              DTYPE_CODES[par.dtype] if par is not None else 0, N, S, C, G, ctx.act, at, at + 4 * N * G, _ptr(gx), _ptr(gw), _ptr(gb),
-              _ptr(ws), _stream())
+    gx = torch.empty_like(x) if want[0] else None
+    gw = torch.empty_like(weight) if want[1] else None
+    gb = torch.empty_like(bias) if want[2] else None
+    at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
+    ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, G, 1), x.device)
+    _call("sed_group_norm_bwd", x.data_ptr(), gy.data_ptr(), _ptr(weight), _ptr(bias), dt,
+          DTYPE_CODES[par.dtype] if par is not None else 0, N, S, C, G, ctx.act, at, at + 4 * N * G, _ptr(gx), _ptr(gw), _ptr(gb),
+          _ptr(ws), _stream())
     return gx, gw, gb, None, None, None
 
 
@@ -2025,16 +2013,15 @@ class GroupNormActFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        with _on_device(x):
-            x = _contiguous(x)
-            y, stats = _group_norm_fwd(x, _contiguous(weight), _contiguous(bias), groups, eps, act)
-        ctx.save_for_backward(x, _contiguous(weight), _contiguous(bias), stats)
+        x, weight, bias = _contiguous(x), _contiguous(weight), _contiguous(bias)
+        y, stats = _there(x, _group_norm_fwd, x, weight, bias, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        return _once_group_norm_bwd(ctx, gy) if torch.is_grad_enabled() else _group_norm_bwd(ctx, gy)
+        return _there(gy, _once_group_norm_bwd if torch.is_grad_enabled() else _group_norm_bwd, ctx, gy)
 
 
 _once_group_norm_bwd = torch.autograd.function.once_differentiable(_group_norm_bwd)
@@ -2072,8 +2059,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         return y
     if grad:
         return GroupNormActFn.apply(x, weight, bias, groups, float(eps), act)
-    with _on_device(x):
-        return _group_norm_fwd(_contiguous(x), _contiguous(weight), _contiguous(bias), groups, float(eps), act)[0]
+    return _there(x, _group_norm_fwd, _contiguous(x), _contiguous(weight), _contiguous(bias), groups, float(eps), act)[0]
 
 
 def _linear_fwd(x, weight, bias, residual, act, keep):
@@ -2084,9 +2070,9 @@ def _linear_fwd(x, weight, bias, residual, act, keep):
     y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
     z = None
     if keep and act:
-        z = torch.empty((int(h.sed_linear_kept_elements(M, N)),), dtype=torch.float16 if dt else torch.float32, device=x.device)
+        z = torch.empty((h.sed_linear_kept_elements(M, N),), dtype=torch.float16 if dt else torch.float32, device=x.device)
     px, pw = x.data_ptr(), weight.data_ptr()
-    need = int(h.sed_linear_fwd_ws_bytes(px, pw, dt, M, N, K))
+    need = h.sed_linear_fwd_ws_bytes(px, pw, dt, M, N, K)
     ws = _bytes(need, x.device)
     _call("sed_linear_fwd", px, pw, _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt, M, N, K, act,
           y.data_ptr(), _ptr(z), _ptr(ws), need, _stream())
@@ -2101,16 +2087,14 @@ def _linear_bwd(ctx, gy):
     g = _contiguous(gy)
     N, K = weight.shape
     M, dt = x.numel() // K, DTYPE_CODES[x.dtype]
-    h = _lib.lib()
-    with _on_device(x):
-        gx = torch.empty_like(x) if want[0] else None
-        gw = torch.empty_like(weight) if want[1] else None
-        gb = torch.empty((N,), dtype=ctx.btype, device=x.device) if want[2] else None
-        px, pw, pg = x.data_ptr(), weight.data_ptr(), g.data_ptr()
-        need = int(h.sed_linear_bwd_ws_bytes(px, pw, pg, dt, M, N, K, ctx.act, want[0], want[1], want[2]))
-        ws = _bytes(need, x.device)
-        _call("sed_linear_bwd", px, pw, pg, _ptr(z), dt, DTYPE_CODES[ctx.btype] if want[2] else dt, M, N, K, ctx.act, _ptr(gx), _ptr(gw),
-              _ptr(gb), _ptr(ws), need, _stream())
+    gx = torch.empty_like(x) if want[0] else None
+    gw = torch.empty_like(weight) if want[1] else None
+    gb = torch.empty((N,), dtype=ctx.btype, device=x.device) if want[2] else None
+    px, pw, pg = x.data_ptr(), weight.data_ptr(), g.data_ptr()
+    need = _lib.lib().sed_linear_bwd_ws_bytes(px, pw, pg, dt, M, N, K, ctx.act, want[0], want[1], want[2])
+    ws = _bytes(need, x.device)
+    _call("sed_linear_bwd", px, pw, pg, _ptr(z), dt, DTYPE_CODES[ctx.btype] if want[2] else dt, M, N, K, ctx.act, _ptr(gx), _ptr(gw),
+          _ptr(gb), _ptr(ws), need, _stream())
     return gx, gw, gb, gy if want[3] else None, None
 
 
@@ -2120,16 +2104,15 @@ class LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         want = ctx.needs_input_grad
-        with _on_device(x):
-            x, weight = _contiguous(x), _contiguous(weight)
-            y, z = _linear_fwd(x, weight, _contiguous(bias), _contiguous(residual), act, want[0] or want[1] or want[2])
+        x, weight = _contiguous(x), _contiguous(weight)
+        y, z = _there(x, _linear_fwd, x, weight, _contiguous(bias), _contiguous(residual), act, want[0] or want[1] or want[2])
         ctx.save_for_backward(x, weight, z)
         ctx.act, ctx.btype = act, bias.dtype if bias is not None else None
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        return _once_linear_bwd(ctx, gy) if torch.is_grad_enabled() else _linear_bwd(ctx, gy)
+        return _there(gy, _once_linear_bwd if torch.is_grad_enabled() else _linear_bwd, ctx, gy)
 
 
 _once_linear_bwd = torch.autograd.function.once_differentiable(_linear_bwd)
@@ -2164,8 +2147,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         return y
     if grad:
         return LinearActFn.apply(x, weight, bias, residual, act)
-    with _on_device(x):
-        return _linear_fwd(_contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), act, False)[0]
+    return _there(x, _linear_fwd, _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), act, False)[0]
 
 
 def adamw_(rows, chunks, nchunks, m, v, m_scale, v_scale, master, state_bits, hyper, step, grad_scale=1.0, guard=None, skipped=None):

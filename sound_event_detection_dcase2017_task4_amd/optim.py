@@ -486,25 +486,24 @@ class FusedAdamW(object):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW.step() cannot be captured into a graph (the step number is an argument of the launch): "
                                "capture forward and backward, and call step() behind the replay")
-        hyper = self._hyper()
-        with ops._on_device(self.exp_avg):
-            if self.master is not None:
-                self._refresh_copies()
-            grads = self._table()
-            self.step_count += 1
-            if len(self._chunks):
-                ops.adamw_(self._dev_rows, self._chunks, len(self._chunks), self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
-                           self.exp_avg_sq_scale, self.master, self.state_bits, hyper, self.step_count, float(grad_scale),
-                           skipped=self._skipped)
-        del grads
+        ops._there(self.exp_avg, self._update, self._hyper(), float(grad_scale))
         ops.check_device_errors()
+
+    def _update(self, hyper, grad_scale):
+        if self.master is not None:
+            self._refresh_copies()
+        grads = self._table()
+        self.step_count += 1
+        if len(self._chunks):
+            ops.adamw_(self._dev_rows, self._chunks, len(self._chunks), self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
+                       self.exp_avg_sq_scale, self.master, self.state_bits, hyper, self.step_count, grad_scale, skipped=self._skipped)
+        del grads
 
     def moments(self):
         """(exp_avg, exp_avg_sq) as flat float32 buffers: the state itself with 32 bits, the values that the codes stand for with 8."""
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
-        with ops._on_device(self.exp_avg):
-            return ops.adamw_moments(self.exp_avg, self.exp_avg_scale, self.exp_avg_sq, self.exp_avg_sq_scale)
+        return ops._there(self.exp_avg, ops.adamw_moments, self.exp_avg, self.exp_avg_scale, self.exp_avg_sq, self.exp_avg_sq_scale)
 
     _STATE = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")
 
