@@ -596,7 +596,7 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
 int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
 bool bad_shape(int dtype, int wdtype, long N, long S, int C, int G, int act) {
     return dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2 || N < 1 || S < 1 || C < 1 || G < 1 || C % G || act < 0 || act > 3 ||
-           N * G > 0x7fffffffL || cut_of(N, S, C, esize_of(dtype)).blocks > 0x7fffffffL;
+           N * G >= 1L << 25 || cut_of(N, S, C, esize_of(dtype)).blocks >= 1L << 24;         // a launch takes fewer than 2^32 threads
 }
 // How the one-pass kernels cut: bundles of whole groups with at least 128 bytes of a row (or all of it), a workgroup of so many threads
 // that each holds up to R vectors.  threads = 0: the rows do not fit, or a row has fewer channels than a vector.
@@ -613,7 +613,7 @@ One one_of(long N, long S, int C, int G, int esize, int most) {
     const long width = (long)o.per * cg;
     o.bundles = (G + o.per - 1) / o.per;
     const long K = (width + V - 1) / V;
-    if (C < V || width > MAX_BUNDLE || K > 256 || S > (long)ONE_THREADS * most || N * o.bundles > 0x7fffffffL) return o;
+    if (C < V || width > MAX_BUNDLE || K > 256 || S > (long)ONE_THREADS * most || N * o.bundles >= (1L << 32) / ONE_THREADS) return o;
     const long want = K * ((S + 3) / 4);           // four vectors a thread, as far as the threads go
     o.threads = (int)(want < 64 ? 64 : want > ONE_THREADS ? ONE_THREADS : (want + 63) / 64 * 64);
     if (o.threads < K) o.threads = (int)((K + 63) / 64 * 64);

@@ -243,7 +243,7 @@ template <int LATER> __device__ __forceinline__ void arrived() {
 // are read.  In the last quarter every wave holds the rest of the step in registers.
 // LDS is a ring of five slots of one operand's step each: P(t), Q(t), P(t+1), Q(t+1) and the one that P(t+2) goes to during the first
 // three quarters of step t; Q(t+2) goes to P(t)'s slot in the last one, behind a barrier.  The requests of a step are so spread over
-// all of it (a wave that issues sixteen at once waits for the address unit: 57 % of the matrix rate against 80 %), and have at least
+// all of it (a wave that issues sixteen at once waits for the address unit: 57 % of the matrix rate against 72 %), and have at least
 // three quarters to arrive.  Steps behind the end are requested and read like any other, as zeros: the loop has no other branch.
 template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT, int ACT>
 __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gemm_kernel(GemmP a) {
@@ -265,9 +265,9 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gem
     unsigned poff[SP::PER], qoff[SQ::PER];
     SP::offsets(a.p, n0, poff);
     SQ::offsets(a.q, m0, qoff);
-    // For the epilogue a wave passes 32 rows of its results at a time through LDS: a lane then has V consecutive n of row 32 i + PASS it + lane
-    // / LINE, and its neighbours have the rest of the line.  (Stored from where the instructions leave them, 32 bytes a line, a
-    // bf16 product of 32000 x 2048 x 2048 with silu, residual and kept z took 402 us, now 330.)
+    // For the epilogue a wave passes 32 rows of its results at a time through LDS: a lane then has V consecutive n of row
+    // 32 i + PASS it + lane / LINE, and its neighbours have the rest of the line.  (Stored from where the instructions leave them, 32 bytes
+    // a line, a bf16 product of 32000 x 2048 x 2048 with silu, residual and kept z took 402 us, now 330.)
     constexpr int W = BN / WN, LINE = W / V, PASS = 64 / LINE, PASSES = 32 / PASS, PITCH = 4 * W + 16;
     static_assert(4 * 32 * PITCH <= 5 * SLOT, "the waves' rows fit the ring");
     const int n = n0 + wn + lane % LINE * V;
@@ -582,9 +582,9 @@ bool needs_pad(const void* p, long ld, int esize) { return !aligned16(p) || ld %
 
 // How a product is cut: tile edge, and slices along k that a second pass adds.  The cut with the least time by what was measured on an
 // MI355X: a step of 128 bytes of k takes a tile of 64, 128 or 256 the microseconds below when 1, 2, .. of them share a CU (LDS holds 4, 2
-// or 1), a tile costs as much again at its ends, and a cut one passes its 32-bit sums through memory.  It picks the fastest of all
-// cuts, or one within 8 %, at (rows, N, K) from (100, 512, 512) to (32000, 2048, 2048); e.g. bf16 (4000, 512, 512) 7.6 us with edge 64 and
-// 9.4 with 128, (4000, 2048, 512) 15.0 with 128, 18.9 with 64, 25.2 with 256, (4096, 4096, 4096) 117 with 256 and 133 with 128.
+// or 1), a tile costs as much again at its ends, and a cut one passes its 32-bit sums through memory.  E.g. bf16
+// (rows, N, K) = (4000, 512, 512) takes 7.6 us with edge 64 and 9.4 with 128, (4000, 2048, 512) 15.0 with 128, 18.9 with 64, 25.2 with 256,
+// (4096, 4096, 4096) 117 with 256 and 133 with 128.
 struct Plan {
     int edge, tm, tn, slices;
     long kslice, part_bytes, ldp;
@@ -599,6 +599,7 @@ Plan plan_of(long M, long N, long K, int esize) {
     for (int e = 0; e < (esize == 2 ? 3 : 2); ++e) {
         const float* const us = esize == 2 ? step16[e] : step32[e];
         const long tm = (M + edges[e] - 1) / edges[e], tn = (N + edges[e] - 1) / edges[e];
+        if (tm * tn >= 1L << 24) continue;         // 2^32 threads are more than a launch takes; edge 128 fits every shape that is let in
         for (long s = 1; s <= 64 && (s == 1 || (steps / s >= 4 && tm * tn * s <= 2048)); s *= 2) {
             const long per = (steps + s - 1) / s, slices = (steps + per - 1) / per, on = (tm * tn * slices + 255) / 256;
             float t = (float)(on / room[e]) * (per * us[room[e] - 1] + ends[e]);
@@ -658,10 +659,11 @@ template <typename T> void pad(const void*& x, long M, bool px, const void*& w, 
     hipLaunchKernelGGL((pad_kernel<T>), dim3((unsigned)(nb > 16384 ? 16384 : nb)), dim3(256), 0, stream, p);
 }
 
-// rows and columns that 32-bit tile counts and 32-bit offsets inside a tile can hold
+// rows and columns that 32-bit offsets inside a tile and the tiles of one launch can hold: 2^38 elements of x, W or y at most
 bool bad_shape(int dtype, long M, long N, long K, int act) {
     return dtype < 0 || dtype > 2 || M < 1 || N < 1 || K < 1 || M > 0x7fffffffL - 256 || N > 1L << 21 || K > 1L << 21 || act < 0 || act > 3 ||
-           (M + 127) / 128 * ((N + 127) / 128) > 1L << 30 || (M + 127) / 128 * ((K + 127) / 128) > 1L << 30;
+           (M + 127) / 128 * ((N + 127) / 128) >= 1L << 24 || (M + 127) / 128 * ((K + 127) / 128) >= 1L << 24 ||
+           (N + 127) / 128 * ((K + 127) / 128) >= 1L << 24;
 }
 
 struct GradCut {
