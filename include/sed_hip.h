@@ -489,8 +489,8 @@ int sed_guard_publish(const int* err_dev, float* flag_out, sed_stream_t stream);
  *   z = (x - mean) rstd weight + bias;  y = act(z);  weight, bias [C] of wdtype, nullable (1 and 0)
  *   gz = gy act'(z);  gweight = sum gz xhat;  gbias = sum gz  ([C] of wdtype, nullable)
  *   gx = rstd (gz weight - mean_g(gz weight) - xhat mean_g(gz weight xhat))  (nullable)
- * ws: sed_group_norm_ws_floats(..) floats of scratch (0: null will do).  No pointer needs more than its element's alignment.
- * N, S, C >= 1, C % G == 0. */
+ * ws: sed_group_norm_ws_floats(..) floats of scratch (0: null will do).  No pointer needs more than its element's alignment; results
+ * do not overlap operands.  N, S, C >= 1, C % G == 0, N G < 2^25, N times the workgroups of a sample (one up to 16 KB) below 2^24. */
 long sed_group_norm_ws_floats(int dtype, long N, long S, int C, int G, int backward);
 int sed_group_norm_fwd(const void* x, const void* weight, const void* bias, int dtype, int wdtype, long N, long S, int C, int G,
                        float eps, int act, void* y, float* mean, float* rstd, float* ws, sed_stream_t stream);
@@ -505,9 +505,10 @@ int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const 
  * sed_linear_bwd: gz = gy act'(z) (z nullable without an activation);  gx = gz W [M][K];  gweight = gz^T x [N][K];  gbias = sum gz [N]
  * of bdtype; each nullable (x only serves gweight, weight only gx).  gz is rounded to `dtype` for the two products, gbias is summed
  * before that.
- * ws: 16-byte aligned scratch of sed_linear_*_ws_bytes bytes (0: none).  M, N, K >= 1; N, K <= 2^21.  The tensors need no more than
- * their element's alignment; lines of a multiple of 16 bytes at 16-byte addresses are read in place, others are copied into ws first
- * (not in the forward product of up to 64 rows and lines of up to 16 KB). */
+ * ws: 16-byte aligned scratch of sed_linear_*_ws_bytes bytes (0: none).  M, N, K >= 1; M < 2^31 - 256; N, K <= 2^21; x, W and y
+ * below 2^38 elements.  Results do not overlap operands.  The tensors need no more than their element's alignment; lines of a multiple
+ * of 16 bytes at 16-byte addresses are read in place, others are copied into ws first (not in the forward product of up to 64 rows
+ * with lines of up to 1 KB, 32 rows with 4 KB, 16 rows with 16 KB). */
 long sed_linear_kept_elements(long M, long N);
 long sed_linear_fwd_ws_bytes(const void* x, const void* weight, int dtype, long M, long N, long K);
 int sed_linear_fwd(const void* x, const void* weight, const void* bias, const void* residual, int dtype, int bdtype, long M, long N,
@@ -525,6 +526,7 @@ int sed_linear_bwd(const void* x, const void* weight, const void* gy, const void
  * every tensor once.  Moments: flat buffers padded to 256 elements per tensor -- float (state_bits 32), or signed / unsigned bytes
  * (state_bits 8) with one float of m_scale / v_scale per 256 elements: m = sign(q) (|q| / 127)^2 scale, v = (q / 255)^4 scale.
  * hyper (HOST): per group five doubles {lr, beta1, beta2, eps, weight_decay}, at most 16 groups; grad_scale multiplies the gradient.
+ * master: where a 16-bit parameter is not the rounding of its copy, the step goes on from the parameter.
  * skip_flag (nullable, device): non-zero leaves everything untouched and adds 1 to *skipped, as in sed_adam_amsgrad.
  * sed_adamw_moments: the values that 8-bit moments stand for, n elements (a multiple of 256). */
 int sed_adamw_chunk(void);

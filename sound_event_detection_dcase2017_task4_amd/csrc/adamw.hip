@@ -4,7 +4,10 @@
 //
 // The work is a list of chunks of 4096 elements, each inside one tensor: a 28-tensor model and a single 240-million-element matrix
 // fill the chip alike, and no tensor costs a launch.  Bound by HBM: 28 bytes an element with 32-bit moments (parameter, gradient, two
-// moments in; parameter, two moments out; a 16-bit parameter adds its 32-bit copy and saves as much), 16 bytes with 8-bit ones.
+// moments in; parameter, two moments out; 30 for a 16-bit parameter with its 32-bit copy), 16 (18) bytes with 8-bit ones.
+//
+// A 16-bit parameter is the rounding of its 32-bit copy.  Where it is not, somebody else wrote the parameter since the last step, and
+// the step goes on from the parameter: nothing has to be remembered about who wrote it, at two bytes an element.
 //
 // 8-bit moments: a block of 256 elements -- one wave, four elements a lane -- shares one scale, the block's largest magnitude, held
 // in 32 bits.  The codes are powers of a linear grid, because the moments of one block spread over decades and a relative error
@@ -153,7 +156,13 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void adamw_chunk(co
         if (e >= padded) continue;
         load4(g, e, n, wide, gv[i]);
         if (sizeof(T) == 4) load4(p, e, n, wide, pv[i]);
-        else load4(copy, e, padded, true, pv[i]);
+        else {
+            float q[4];
+            load4(copy, e, padded, true, pv[i]);
+            load4(p, e, n, wide, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pv[i][j] = (float)(T)pv[i][j] == q[j] ? pv[i][j] : q[j];
+        }
         if (EIGHT) {
             const char4 qm = reinterpret_cast<const char4*>(a.m)[(off + e) >> 2];
             const uchar4 qv = reinterpret_cast<const uchar4*>(a.v)[(off + e) >> 2];
@@ -237,7 +246,7 @@ SED_API int sed_adamw_chunk(void) { return CHUNK; }
 SED_API int sed_adamw(const long* rows, const int* chunks, long nchunks, void* m, void* v, float* m_scale, float* v_scale,
                       float* master, int state_bits, const double* hyper, int ngroups, int step, float grad_scale, const int* skip_flag,
                       int* skipped, sed_stream_t stream) {
-    if (!rows || !chunks || !m || !v || !hyper || nchunks < 1 || nchunks > 0x7fffffffL || ngroups < 1 || ngroups > MAX_GROUPS || step < 1)
+    if (!rows || !chunks || !m || !v || !hyper || nchunks < 1 || nchunks >= 1L << 24 || ngroups < 1 || ngroups > MAX_GROUPS || step < 1)
         return SED_EINVAL;
     if (state_bits != 32 && (state_bits != 8 || !m_scale || !v_scale)) return SED_EINVAL;
     if (skip_flag && !skipped) return SED_EINVAL;

@@ -344,8 +344,8 @@ class FusedAdamW(object):
 
     state_bits: 32 -- the two moments as float32; 8 -- as 8-bit codes with one float32 scale per 256 elements (csrc/adamw.hip), a
     quarter of the memory.  The update itself is computed in 32 bits either way.  16-bit parameters get a 32-bit copy (`master`, flat,
-    in the order of those parameters) that the step updates and rounds once into the parameter; a parameter that torch changes in
-    place (`load_state_dict` of its model, clipping) is copied back into it at the next step.
+    in the order of those parameters) that the step updates and rounds once into the parameter; where a parameter is not the rounding of
+    its copy (its model was loaded, it was clipped or broadcast), the step goes on from the parameter.
 
     `exp_avg`, `exp_avg_sq` (and `exp_avg_scale`, `exp_avg_sq_scale`) are flat buffers in which every tensor begins at a multiple of
     256 elements (`offsets`).  In a data-parallel job reduce the gradients first and pass `step(grad_scale=1 / world_size)`.  The step
@@ -396,7 +396,6 @@ class FusedAdamW(object):
         self.exp_avg_scale = zeros(total // STATE_BLOCK, torch.float32) if state_bits == 8 else None
         self.exp_avg_sq_scale = zeros(total // STATE_BLOCK, torch.float32) if state_bits == 8 else None
         self.master = zeros(copied, torch.float32) if copied else None
-        self._versions = [None] * len(self.params)
         self.step_count = 0
         self.skipped_steps = 0
         self._skipped = zeros(1, torch.int32)
@@ -412,7 +411,10 @@ class FusedAdamW(object):
         count = -(-self._rows[:, 4] // per)
         first = np.repeat(np.cumsum(count) - count, count)
         chunks = np.stack([np.repeat(np.arange(len(count)), count), np.arange(len(first)) - first], axis=1).astype(np.int32)
-        self._chunks = torch.from_numpy(chunks).to(dev)     # complete when this returns: any stream may read it
+        self._chunks = torch.from_numpy(chunks).to(dev)
+        if self.master is not None:
+            self._refresh_copies()
+        torch.cuda.current_stream(dev).synchronize()        # the buffers are complete when this returns: any stream may use them
 
     def _hyper(self):
         rows = []
@@ -450,31 +452,33 @@ class FusedAdamW(object):
                 else:
                     p.grad.detach_().zero_()
 
+    @torch.no_grad()
     def _refresh_copies(self):
-        """Take parameters that torch wrote since the last step (or never seen) into their 32-bit copies."""
-        for i, p in enumerate(self.params):
-            if p.dtype != torch.float32 and self._versions[i] != (p._version, p.data_ptr()):
-                self.master[self._copy_at[i]:self._copy_at[i] + p.numel()].copy_(p.detach().reshape(-1))
-                self._versions[i] = (p._version, p.data_ptr())
+        """Take parameters that are not the rounding of their 32-bit copies into these, as the step does."""
+        for at, p in zip(self._copy_at, self.params):
+            if p.dtype != torch.float32:
+                copy, now = self.master[at:at + p.numel()], p.detach().reshape(-1)
+                copy.copy_(torch.where(copy.to(p.dtype) == now, copy, now.float()))
 
     def _table(self):
         """Device table of this step's tensors; the gradients it points to are returned with it and stay alive until the launch."""
         grads = [p.grad for p in self.params]
         if not all([g is None or g.is_contiguous() for g in grads]):
             grads = [g if g is None else g.contiguous() for g in grads]
-        at = [p.data_ptr() for p in self.params], [p.numel() for p in self.params], [0 if g is None else g.data_ptr() for g in grads], ops._stream()
-        if at == self._sent:                       # every address and size as in the table that the kernel read last, on the same stream
+        now = [(p.data_ptr(), p.numel(), p.dtype, p.is_contiguous()) for p in self.params]
+        at = now, [0 if g is None else g.data_ptr() for g in grads], ops._stream()
+        if at == self._sent:                       # all that the table holds is as in the one that the kernel read last, on the same stream
             return grads
         rows = self._rows
-        if self._sent is None or at[:2] != self._sent[:2]:
+        if self._sent is None or now != self._sent[0]:
             self._check_params()
-            if at[1] != rows[:, 4].tolist() or [ops.DTYPE_CODES[p.dtype] for p in self.params] != (rows[:, 5] >> 32).tolist():
+            if [t[1] for t in now] != rows[:, 4].tolist() or [ops.DTYPE_CODES[p.dtype] for p in self.params] != (rows[:, 5] >> 32).tolist():
                 raise ValueError("FusedAdamW: a parameter changed its size or type since the optimiser was made")
         for p, g in zip(self.params, grads):
             if g is not None and (g.dtype != p.dtype or g.device != p.device or g.numel() != p.numel()):
                 raise ValueError("FusedAdamW: a gradient %s of type %s on %s for a parameter %s of type %s on %s"
                                  % (tuple(g.shape), g.dtype, g.device, tuple(p.shape), p.dtype, p.device))
-        rows[:, 0], rows[:, 1] = at[0], at[2]
+        rows[:, 0], rows[:, 1] = [t[0] for t in now], at[1]
         # uploaded on the stream that reads it, into new memory: a step still in flight keeps the table it was given
         self._dev_rows = ops.upload_small(rows, self.device, torch.int64)
         self._sent = at
@@ -490,8 +494,6 @@ class FusedAdamW(object):
         ops.check_device_errors()
 
     def _update(self, hyper, grad_scale):
-        if self.master is not None:
-            self._refresh_copies()
         grads = self._table()
         self.step_count += 1
         if len(self._chunks):
@@ -516,7 +518,7 @@ class FusedAdamW(object):
 
     def load_state_dict(self, sd):
         """Takes over the step counter, the moments and the 32-bit copies of a state_dict() of the same tensors and state_bits; a
-        'master' of None (or none at all) takes the copies from the parameters.  lr / betas / eps / weight_decay stay those of this
+        'master' of None (or none at all) takes the copies from the parameters, as does one that they are not the rounding of.  lr / betas / eps / weight_decay stay those of this
         optimiser.  Anything that does not fit is refused (ValueError) before anything is changed."""
         if "step" not in sd or "exp_avg" not in sd or "exp_avg_sq" not in sd:
             raise ValueError("unknown optimiser state layout (keys: %s): expected a FusedAdamW.state_dict()" % sorted(sd.keys()))
@@ -540,4 +542,3 @@ class FusedAdamW(object):
             for k, have in new.items():
                 getattr(self, k).copy_(have.reshape(-1))
         self.step_count = step
-        self._versions = [(p._version, p.data_ptr()) if "master" in new else None for p in self.params]

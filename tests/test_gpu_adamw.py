@@ -220,6 +220,32 @@ def test_copy_follows_a_parameter_that_torch_changed():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copy_follows_a_parameter_that_was_written_through_data(dtype, bits):
+    """A write that no version counter records: elements that are not the rounding of their copy are taken, the others keep their bits."""
+    p = torch.nn.Parameter(torch.linspace(-2.0, 2.0, 1001, device="cuda").to(dtype)[1:])          # 16-bit vectors begin beside 8 bytes
+    p.grad = torch.full_like(p, 0.3)
+    opt = optim.FusedAdamW([p], lr=1e-3, weight_decay=0.0, state_bits=bits)
+    for _ in range(3):
+        opt.step()
+    kept = opt.master[:1000].clone()
+    assert torch.equal(kept.to(dtype), p.detach()) and not torch.equal(kept.to(dtype).float(), kept)
+    p.data[100:200] = 5.0
+    p.data[300] = float("nan")
+    p.grad.zero_()
+    opt.param_groups[0]["lr"] = 0.0
+    assert float(opt.state_dict()["master"][150]) == 5.0
+    opt.master[:1000] = kept                               # the step does the same by itself
+    opt.step()
+    want = kept.clone()
+    want[100:200] = 5.0
+    want[300] = float("nan")
+    assert torch.equal(opt.master[:1000].nan_to_num(99.0), want.nan_to_num(99.0))
+    assert torch.equal(p.detach().nan_to_num(99.0), want.to(dtype).nan_to_num(99.0))
+
+
+@gpu
 def test_gradients_of_any_layout_moved_between_steps_and_other_streams():
     p, q = (torch.nn.Parameter(torch.ones(33, 40, device="cuda")) for _ in range(2))
     grads = [torch.randn(40, 33, device="cuda").t() for _ in range(4)]
