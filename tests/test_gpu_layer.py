@@ -1,0 +1,156 @@
+"""A residual layer of ops.group_norm_act and ops.linear_act, trained by optim.FusedAdamW: the operators together, as a model uses them.
+
+    h = silu(norm(x));  u = gelu(h W1^T + b1);  y = x + u W2^T + b2
+
+Each step is checked from where it starts: the gradients against those of the formulas in 64 bits at the step's own parameters, and the
+parameters and moments behind it against the formula with the step's own gradients.
+
+Tolerances.  Normwise, a rounding of a tensor to a type with half a step e moves what depends on it by at most e times a gain; the gains of
+these layers (random matrices of unit gain, derivatives of at most 1.2, the norm's backward projection) are below 2.  A gradient depends on
+at most eight rounded tensors: h, u, y's gradient as given, gz and gx of two products, z kept twice (2^-11 at most), its own rounding.  In
+32 bits the roundings are those of the sums behind each: (0.5 count + 16) 2^-24 for the longest sum."""
+import copy
+
+import pytest
+import torch
+
+from sound_event_detection_dcase2017_task4_amd import ops, optim
+
+H = 2.0 ** -24
+gpu = pytest.mark.gpu
+F = torch.nn.functional
+GROUPS, C, HIDDEN = 8, 96, 136
+
+
+class Layer(torch.nn.Module):
+    def __init__(self, seed, dtype, tied=False):
+        super().__init__()
+        g = torch.Generator().manual_seed(seed)
+        par = lambda t, d=dtype: torch.nn.Parameter(t.to(d).cuda())  # noqa: E731
+        hidden = C if tied else HIDDEN
+        self.nw, self.nb = par(1 + 0.1 * torch.randn(C, generator=g), torch.float32), par(0.1 * torch.randn(C, generator=g), torch.float32)
+        self.w1, self.b1 = par(torch.randn(hidden, C, generator=g) / C ** 0.5), par(0.1 * torch.randn(hidden, generator=g))
+        self.w2 = self.w1 if tied else par(torch.randn(C, hidden, generator=g) / hidden ** 0.5)
+        self.b2 = par(0.1 * torch.randn(C, generator=g))
+
+    def forward(self, x):
+        h = ops.group_norm_act(x, GROUPS, self.nw, self.nb, activation="silu")
+        u = ops.linear_act(h, self.w1, self.b1, "gelu")
+        return ops.linear_act(u, self.w2, self.b2, residual=x)
+
+
+def _gradients_64(layer, x, gy):
+    names = [n for n, _ in layer.named_parameters()]
+    p = {n: t.detach().double().cpu().requires_grad_(True) for n, t in layer.named_parameters()}
+    x = x.detach().double().cpu().requires_grad_(True)
+    h = F.silu(F.group_norm(x.transpose(1, 2), GROUPS, p["nw"], p["nb"]).transpose(1, 2))
+    u = F.gelu(h @ p["w1"].t() + p["b1"])
+    y = x + u @ p.get("w2", p["w1"]).t() + p["b2"]
+    grads = torch.autograd.grad(y, [x] + [p[n] for n in names], gy.double().cpu())
+    return y.detach(), grads[0], dict(zip(names, grads[1:]))
+
+
+def _near(got, want, tol):
+    return float((got.detach().double().cpu() - want).norm()) <= tol * float(want.norm())
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,tied", [(torch.float32, False), (torch.bfloat16, False), (torch.float16, False), (torch.float32, True)])
+def test_training_steps_against_64_bits(dtype, tied, bits):
+    layer = Layer(1, dtype, tied)
+    lr, betas, eps, wd = 2e-3, (0.9, 0.99), 1e-7, 0.05
+    opt = optim.FusedAdamW(layer, lr=lr, betas=betas, eps=eps, weight_decay=wd, state_bits=bits)
+    e = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else (0.5 * 3 * 70 + 16) * H
+    g = torch.Generator().manual_seed(2)
+    flat = lambda t, k: t[opt.offsets[k]:opt.offsets[k] + opt.params[k].numel()].double()  # noqa: E731
+    value = lambda k, p: (p.detach().reshape(-1) if p.dtype == torch.float32 else opt.master[opt._copy_at[k]:opt._copy_at[k] + p.numel()]).double()  # noqa: E731
+    for t in range(1, 4):
+        x = torch.randn(3, 70, C, generator=g).to(dtype).cuda().requires_grad_(True)
+        gy = torch.randn(3, 70, C, generator=g).to(dtype).cuda()
+        opt.zero_grad()
+        y = layer(x)
+        y.backward(gy)
+        wy, wx, wp = _gradients_64(layer, x, gy)
+        tol = 8 * 2 * e
+        assert _near(y, wy, tol) and _near(x.grad, wx, tol)
+        for n, p in layer.named_parameters():
+            assert p.grad.dtype == p.dtype and _near(p.grad, wp[n], tol), n
+        before = [value(k, p).clone() for k, p in enumerate(opt.params)]
+        m0, v0 = (s.clone() for s in opt.moments())
+        opt.step()
+        m1, v1 = opt.moments()
+        for k, p in enumerate(opt.params):
+            gd = p.grad.double().reshape(-1)
+            m, v = betas[0] * flat(m0, k) + (1 - betas[0]) * gd, betas[1] * flat(v0, k) + (1 - betas[1]) * gd * gd
+            step = lr / (1 - betas[0] ** t) * m / (v.sqrt() / (1 - betas[1] ** t) ** 0.5 + eps)
+            want = before[k] * (1 - lr * wd) - step
+            # a few roundings of the parameter, and of the update: its moments' (m may cancel: relative to its terms), root, quotient, constants
+            terms = lr / (1 - betas[0] ** t) * (betas[0] * flat(m0, k).abs() + (1 - betas[0]) * gd.abs()) / (v.sqrt() / (1 - betas[1] ** t) ** 0.5 + eps)
+            assert (value(k, p) - want).abs().le(4 * H * (want.abs() + step.abs()) + 24 * H * terms).all()
+            if p.dtype != torch.float32:
+                assert torch.equal(p.detach().reshape(-1), value(k, p).float().to(p.dtype))
+            if bits == 32:
+                assert (flat(m1, k) - m).abs().le(5 * H * (flat(m0, k).abs() + gd.abs())).all() and (flat(v1, k) - v).abs().le(6 * H * v).all()
+    assert opt.step_count == 3
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_passes_with_the_step_behind_the_replay(dtype):
+    eager, layer = Layer(3, dtype), Layer(3, dtype)
+    opts = [optim.FusedAdamW(m, lr=1e-2, state_bits=8) for m in (eager, layer)]
+    x, gy = torch.randn(2, 50, C, device="cuda").to(dtype), torch.randn(2, 50, C, device="cuda").to(dtype)
+    run = lambda m: torch.autograd.grad(m(x), list(m.parameters()), gy)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(layer)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = run(layer)
+    for p, q in zip(layer.parameters(), grads):
+        p.grad = q
+    for k in range(4):
+        with torch.no_grad():
+            x.normal_()
+            gy.normal_()
+        graph.replay()
+        opts[1].step()
+        for p, q in zip(eager.parameters(), run(eager)):
+            p.grad = q
+        opts[0].step()
+        for (n, p), q in zip(eager.named_parameters(), layer.parameters()):
+            assert torch.equal(p.grad, q.grad) and torch.equal(p.detach(), q.detach()), (k, n)
+
+
+@gpu
+def test_under_the_other_optimiser_and_in_two_passes():
+    """FusedAdamAmsgrad keeps its gradients in one flat buffer: two passes of the layer add up there as autograd adds them."""
+    layer = Layer(4, torch.float32)
+    twin = copy.deepcopy(layer)
+    opt = optim.FusedAdamAmsgrad(layer, lr=1e-3)
+    xs = [torch.randn(2, 40, C, device="cuda") for _ in range(2)]
+    opt.zero_grad()
+    for x in xs:
+        layer(x).square().sum().backward()
+        twin(x).square().sum().backward()
+    for p, q in zip(layer.parameters(), twin.parameters()):
+        assert torch.equal(p.grad, q.grad)
+    before = [p.detach().clone() for p in layer.parameters()]
+    opt.step()
+    for p, q, b in zip(layer.parameters(), twin.parameters(), before):
+        # the first step of Adam is lr sign(g) where |g| is far above eps
+        assert (p.detach() - (b - 1e-3 * q.grad / (q.grad.abs() + 1e-8))).abs().max() <= 8 * H * (1 + float(b.abs().max()))
+
+
+@gpu
+def test_recorded_again_under_checkpointing():
+    from torch.utils.checkpoint import checkpoint
+    layer = Layer(5, torch.bfloat16)
+    x = torch.randn(2, 33, C, device="cuda").bfloat16().requires_grad_(True)
+    leaves = [x] + list(layer.parameters())
+    plain = torch.autograd.grad(layer(x).sum(), leaves)
+    again = torch.autograd.grad(checkpoint(layer, x, use_reentrant=False).sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
