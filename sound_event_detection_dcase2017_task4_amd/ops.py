@@ -1960,6 +1960,8 @@ def _act_code(activation):
 
 def _chk_operand(name, t, shape, dtype, other, device):
     """A further operand of an operator whose first one fixes device and sizes; `other`: a second type it may have."""
+    if t.shape == shape and (t.dtype is dtype or t.dtype is other) and t.device == device:
+        return
     if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     if t.dtype is not dtype and t.dtype is not other:
@@ -1968,8 +1970,8 @@ def _chk_operand(name, t, shape, dtype, other, device):
         raise ValueError("%s is on %s, the input on %s" % (name, t.device, device))
 
 
-def _bytes(n, device):
-    return torch.empty((n,), dtype=torch.uint8, device=device) if n else None
+def _bytes(n, like):
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def _contiguous(t):
@@ -1981,9 +1983,9 @@ def _group_norm_fwd(x, weight, bias, groups, eps, act):
     N = x.shape[0]
     S = x.numel() // (N * C)
     y = torch.empty_like(x)
-    stats = torch.empty((2 * N * groups,), dtype=torch.float32, device=x.device)           # mean, 1 / sigma
+    stats = x.new_empty(2 * N * groups, dtype=torch.float32)           # mean, 1 / sigma
     at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
-    ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, groups, 0), x.device)
+    ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, groups, 0), x)
     par = weight if weight is not None else bias
     _call("sed_group_norm_fwd", x.data_ptr(), _ptr(weight), _ptr(bias), dt, DTYPE_CODES[par.dtype] if par is not None else 0,
           N, S, C, groups, eps, act, y.data_ptr(), at, at + 4 * N * groups, _ptr(ws), _stream())
@@ -2001,7 +2003,7 @@ def _group_norm_bwd(ctx, gy):
     gw = torch.empty_like(weight) if want[1] else None
     gb = torch.empty_like(bias) if want[2] else None
     at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
-    ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, G, 1), x.device)
+    ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, G, 1), x)
     _call("sed_group_norm_bwd", x.data_ptr(), gy.data_ptr(), _ptr(weight), _ptr(bias), dt,
           DTYPE_CODES[par.dtype] if par is not None else 0, N, S, C, G, ctx.act, at, at + 4 * N * G, _ptr(gx), _ptr(gw), _ptr(gb),
           _ptr(ws), _stream())
@@ -2067,13 +2069,13 @@ def _linear_fwd(x, weight, bias, residual, act, keep):
     N, K = weight.shape
     M, dt = x.numel() // K, DTYPE_CODES[x.dtype]
     h = _lib.lib()
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape[:-1] + (N,))
     z = None
     if keep and act:
-        z = torch.empty((h.sed_linear_kept_elements(M, N),), dtype=torch.float16 if dt else torch.float32, device=x.device)
+        z = x.new_empty(h.sed_linear_kept_elements(M, N), dtype=torch.float16 if dt else torch.float32)
     px, pw = x.data_ptr(), weight.data_ptr()
     need = h.sed_linear_fwd_ws_bytes(px, pw, dt, M, N, K)
-    ws = _bytes(need, x.device)
+    ws = _bytes(need, x)
     _call("sed_linear_fwd", px, pw, _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt, M, N, K, act,
           y.data_ptr(), _ptr(z), _ptr(ws), need, _stream())
     return y, z
@@ -2089,10 +2091,10 @@ def _linear_bwd(ctx, gy):
     M, dt = x.numel() // K, DTYPE_CODES[x.dtype]
     gx = torch.empty_like(x) if want[0] else None
     gw = torch.empty_like(weight) if want[1] else None
-    gb = torch.empty((N,), dtype=ctx.btype, device=x.device) if want[2] else None
+    gb = x.new_empty(N, dtype=ctx.btype) if want[2] else None
     px, pw, pg = x.data_ptr(), weight.data_ptr(), g.data_ptr()
     need = _lib.lib().sed_linear_bwd_ws_bytes(px, pw, pg, dt, M, N, K, ctx.act, want[0], want[1], want[2])
-    ws = _bytes(need, x.device)
+    ws = _bytes(need, x)
     _call("sed_linear_bwd", px, pw, pg, _ptr(z), dt, DTYPE_CODES[ctx.btype] if want[2] else dt, M, N, K, ctx.act, _ptr(gx), _ptr(gw),
           _ptr(gb), _ptr(ws), need, _stream())
     return gx, gw, gb, gy if want[3] else None, None
