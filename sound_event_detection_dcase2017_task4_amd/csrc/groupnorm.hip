@@ -11,7 +11,7 @@
 // folded to groups afterwards.  A row that is not a multiple of V channels ends in a vector that overlaps its neighbour (the twice
 // computed channels are written twice with the same value, and counted once), and loads need no more than element alignment.
 #include "common.h"
-#include "sed_hip.h"
+#include "sed_hip_test.h"
 
 SED_OBJECT_FLAGS(groupnorm)
 
@@ -78,6 +78,16 @@ __device__ __forceinline__ void store_param(void* p, int type, int c, float v) {
     if (type == SED_F32) reinterpret_cast<float*>(p)[c] = v;
     else if (type == SED_F16) reinterpret_cast<_Float16*>(p)[c] = (_Float16)v;
     else reinterpret_cast<__bf16*>(p)[c] = (__bf16)v;
+}
+
+// the groups of V consecutive channels, by one division
+template <int V> __device__ __forceinline__ void groups_of(int c0, int cg, int (&g)[V]) {
+    int q = c0 / cg, r = c0 - q * cg;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        g[j] = q;
+        if (++r == cg) { r = 0; ++q; }
+    }
 }
 
 // where this thread works: sample, chunk, first channel, row lane
@@ -202,12 +212,13 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
     if (!q.on) return;
     const T* const x = reinterpret_cast<const T*>(p.x) + q.n * p.S * p.C + q.c0;
     T* const y = reinterpret_cast<T*>(p.y) + q.n * p.S * p.C + q.c0;
-    const int cg = p.C / p.G;
+    int gr[V];
+    groups_of<V>(q.c0, p.C / p.G, gr);
     float m[V], a[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = q.c0 + j;
-        const long ng = q.n * p.G + c / cg;
+        const long ng = q.n * p.G + gr[j];
         m[j] = p.mean[ng];
         a[j] = p.rstd[ng] * load_param(p.w, p.wdtype, c, 1.f);
         b[j] = load_param(p.b, p.wdtype, c, 0.f);
@@ -235,12 +246,13 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
         const long at = q.n * p.S * p.C + q.c0;
         const T* const x = reinterpret_cast<const T*>(p.x) + at;
         const T* const gy = reinterpret_cast<const T*>(p.gy) + at;
-        const int cg = p.C / p.G;
+        int gr[V];
+        groups_of<V>(q.c0, p.C / p.G, gr);
         float m[V], r[V], w[V], b[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = q.c0 + j;
-            const long ng = q.n * p.G + c / cg;
+            const long ng = q.n * p.G + gr[j];
             m[j] = p.mean[ng];
             r[j] = p.rstd[ng];
             w[j] = load_param(p.w, p.wdtype, c, 1.f);
@@ -356,12 +368,13 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
     const T* const x = reinterpret_cast<const T*>(p.x) + at;
     const T* const gy = reinterpret_cast<const T*>(p.gy) + at;
     T* const gx = reinterpret_cast<T*>(p.y) + at;
-    const int cg = p.C / p.G;
+    int gr[V];
+    groups_of<V>(q.c0, p.C / p.G, gr);
     float m[V], r[V], w[V], b[V], c1[V], c2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = q.c0 + j;
-        const long ng = q.n * p.G + c / cg;
+        const long ng = q.n * p.G + gr[j];
         m[j] = p.mean[ng];
         r[j] = p.rstd[ng];
         w[j] = load_param(p.w, p.wdtype, c, 1.f);
@@ -392,7 +405,7 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
 }
 
 // ---- one pass: the rows of a bundle of whole groups stay in the registers of one workgroup, up to 128 KB (forward) or 2 x 64 KB
-// (backward), and are read once.  The statistics are then the plain two-step ones: mean, then squared deviations from it.
+// (backward), and are read once.
 struct OneP {
     const void* x;
     const void* gy;
@@ -404,6 +417,7 @@ struct OneP {
     float* chan;                         // backward: [N][2][C], sum gz and sum gz xhat
     long S;
     int C, G, per, bundles, wdtype;      // per: groups in a bundle
+    int glanes;                          // lanes that add up a group's channels: a power of two up to 64
     float eps;
 };
 constexpr int MAX_BUNDLE = 1024;         // channels of a bundle
@@ -472,66 +486,100 @@ template <typename F> __device__ __forceinline__ void group_sums(const float* ch
     __syncthreads();
 }
 
-template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS) void norm_one_kernel(OneP p) {
+// what a lane's 16 bytes hold must stay in 16-bit form between the passes over it: converted once, they would take twice the registers
+template <typename T, int V> __device__ __forceinline__ void keep(Vec<T, V>& v) {
+    floatx4 q = __builtin_bit_cast(floatx4, v);
+    asm volatile("" : "+v"(q));
+    v = __builtin_bit_cast(Vec<T, V>, q);
+}
+
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+// Mean and sum of squared deviations of each of `groups` groups of cg channels over `count` rows, from the sums of the deviations from the
+// first row and of their squares (chan[2][channels], LDS, overwritten) and the first row itself; `lanes` (a power of two) share a group,
+// and the first of them passes the two to write(group, mean, squares).
+template <typename F> __device__ __forceinline__ void group_stats(float* chan, const float* first, int groups, int cg, int count, int lanes, F write) {
+    const float inv = 1.f / (float)count, share = 1.f / (float)cg;
+    const int sub = threadIdx.x % lanes;
+    for (int g = threadIdx.x / lanes; g < groups; g += blockDim.x / lanes) {
+        float a = 0.f, q = 0.f;
+        for (int c = g * cg + sub; c < (g + 1) * cg; c += lanes) {
+            const float sum = chan[c], m = sum * inv, sq = chan[MAX_BUNDLE + c];
+            chan[c] = first[c] + m;
+            chan[MAX_BUNDLE + c] = fmaxf(fmaf(-sum, m, sq), 0.f) + (sq - sq);        // sq - sq: 0, or the NaN that fmaxf would drop
+            a += chan[c];
+        }
+        const float m = lanes_sum(a, lanes) * share;
+        for (int c = g * cg + sub; c < (g + 1) * cg; c += lanes) {
+            const float d = chan[c] - m;
+            q += fmaf((float)count * d, d, chan[MAX_BUNDLE + c]);
+        }
+        q = lanes_sum(q, lanes);
+        if (sub == 0) write(g, m, q);
+    }
+}
+
+template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS, 4) void norm_one_kernel(OneP p) {
     extern __shared__ float scratch[];             // 2 * blockDim * V floats
-    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE];
+    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE], row0[MAX_BUNDLE];
     const long n = blockIdx.x / p.bundles;
     const int g0 = (int)(blockIdx.x % p.bundles) * p.per, groups = min(p.per, p.G - g0), cg = p.C / p.G, width = groups * cg;
     const int K = (width + V - 1) / V, RT = blockDim.x / K, t = threadIdx.x, col = t % K, r0 = t / K;
-    const bool on = r0 < RT;
+    const int count = r0 < RT ? (int)p.S : 0;
     const int own = col * V, c0 = min(own, width - V);
     const long at = n * p.S * p.C + g0 * cg + c0;
     const T* const x = reinterpret_cast<const T*>(p.x) + at;
-    Vec<T, V> v[R];
+    Vec<T, V> v[R], k0 = load_vec<T, V>(x);        // deviations are taken from the first row, as in norm_stats_kernel
 #pragma unroll
     for (int u = 0; u < R; ++u)
-        if (on && r0 + u * RT < p.S) v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
-    const float scale = 1.f / ((float)p.S * (float)cg);
-    float s1[V] = {}, s2[V] = {}, m[V], r[V];
+        if (r0 + u * RT < count) v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
+    float s1[V] = {}, s2[V] = {};
 #pragma unroll
     for (int u = 0; u < R; ++u)
-        if (on && r0 + u * RT < p.S)
-#pragma unroll
-            for (int j = 0; j < V; ++j) s1[j] += (float)v[u].v[j];
-    channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
-    group_sums(chan, groups, cg, [](int) { return 1.f; }, grp);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        m[j] = grp[2 * ((c0 + j) / cg)] * scale;
-        s1[j] = 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < R; ++u)
-        if (on && r0 + u * RT < p.S)
+        if (r0 + u * RT < count) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = (float)v[u].v[j] - m[j];
-                s1[j] = fmaf(d, d, s1[j]);
+                const float d = (float)v[u].v[j] - (float)k0.v[j];
+                s1[j] += d;
+                s2[j] = fmaf(d, d, s2[j]);
             }
-    __syncthreads();                               // every thread has its mean
-    if (t < groups) p.mean[n * p.G + g0 + t] = grp[2 * t] * scale;
-    __syncthreads();
+            keep(v[u]);
+        }
+    if (t < K)
+#pragma unroll
+        for (int j = 0; j < V; ++j) row0[c0 + j] = (float)k0.v[j];
     channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
-    group_sums(chan, groups, cg, [](int) { return 1.f; }, grp);
-    if (t < groups) p.rstd[n * p.G + g0 + t] = 1.f / sqrtf(grp[2 * t] * scale + p.eps);
-    if (!on) return;
-    float b[V];
+    const float scale = 1.f / ((float)p.S * (float)cg);
+    group_stats(chan, row0, groups, cg, (int)p.S, p.glanes, [&](int g, float m, float q) {
+        const float r = 1.f / sqrtf(q * scale + p.eps);
+        grp[2 * g] = m;
+        grp[2 * g + 1] = r;
+        p.mean[n * p.G + g0 + g] = m;
+        p.rstd[n * p.G + g0 + g] = r;
+    });
+    __syncthreads();
+    int gr[V];
+    groups_of<V>(c0, cg, gr);
+    float m[V], a[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        r[j] = 1.f / sqrtf(grp[2 * ((c0 + j) / cg)] * scale + p.eps) * load_param(p.w, p.wdtype, g0 * cg + c0 + j, 1.f);
+        m[j] = grp[2 * gr[j]];
+        a[j] = grp[2 * gr[j] + 1] * load_param(p.w, p.wdtype, g0 * cg + c0 + j, 1.f);
         b[j] = load_param(p.b, p.wdtype, g0 * cg + c0 + j, 0.f);
     }
     T* const y = reinterpret_cast<T*>(p.y) + at;
 #pragma unroll
     for (int u = 0; u < R; ++u)
-        if (r0 + u * RT < p.S) {
+        if (r0 + u * RT < count) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[u].v[j] = (T)sed_act<ACT>(fmaf((float)v[u].v[j] - m[j], r[j], b[j]));
+            for (int j = 0; j < V; ++j) v[u].v[j] = (T)sed_act<ACT>(fmaf((float)v[u].v[j] - m[j], a[j], b[j]));
             store_vec<T, V>(y + (long)(r0 + u * RT) * p.C, v[u]);
         }
 }
 
-template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS) void norm_one_bwd_kernel(OneP p) {
+template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS, 4) void norm_one_bwd_kernel(OneP p) {
     extern __shared__ float scratch[];
     __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE];
     const long n = blockIdx.x / p.bundles;
@@ -550,10 +598,12 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
             g[u] = load_vec<T, V>(gy + (long)(r0 + u * RT) * p.C);
         }
     float s1[V] = {}, s2[V] = {}, m[V], r[V], w[V], b[V];
+    int gr[V];
+    groups_of<V>(c0, cg, gr);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = g0 * cg + c0 + j;
-        const long ng = n * p.G + c / cg;
+        const long ng = n * p.G + g0 + gr[j];
         m[j] = p.mean[ng];
         r[j] = p.rstd[ng];
         w[j] = load_param(p.w, p.wdtype, c, 1.f);
@@ -561,7 +611,7 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
     }
 #pragma unroll
     for (int u = 0; u < R; ++u)
-        if (on && r0 + u * RT < p.S)
+        if (on && r0 + u * RT < p.S) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float xh = ((float)v[u].v[j] - m[j]) * r[j];
@@ -569,6 +619,9 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
                 s1[j] += gz;
                 s2[j] = fmaf(gz, xh, s2[j]);
             }
+            keep(v[u]);
+            keep(g[u]);
+        }
     channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
     for (int k = t; k < width; k += blockDim.x) {
         p.chan[n * 2 * p.C + g0 * cg + k] = chan[k];
@@ -579,18 +632,221 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
     if (!on) return;
     const float scale = 1.f / ((float)p.S * (float)cg);
     T* const gx = reinterpret_cast<T*>(p.y) + at;
+    float c1[V], c2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        c1[j] = grp[2 * gr[j]] * scale;
+        c2[j] = grp[2 * gr[j] + 1] * scale;
+    }
 #pragma unroll
     for (int u = 0; u < R; ++u)
         if (r0 + u * RT < p.S) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const int gr = (c0 + j) / cg;
                 const float xh = ((float)v[u].v[j] - m[j]) * r[j];
                 const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
-                v[u].v[j] = (T)(r[j] * (fmaf(gz, w[j], -grp[2 * gr] * scale) - xh * (grp[2 * gr + 1] * scale)));
+                v[u].v[j] = (T)(r[j] * (fmaf(gz, w[j], -c1[j]) - xh * c2[j]));
             }
             store_vec<T, V>(gx + (long)(r0 + u * RT) * p.C, v[u]);
         }
+}
+
+// ---- one pass over samples that a single workgroup cannot hold (forward): the rows of a sample lie in the registers of up to 128
+// workgroups, 128 KB each.  Each publishes the statistics of its rows; the one that arrives last joins the sample's and publishes them;
+// the others wait for that, and write their rows from registers.  Nothing rests on the workgroups of a sample running together: one that
+// has waited WAIT_TICKS gives up (and with it all that wait later), and a second kernel, which normally finds nothing to do, writes
+// what was left, from memory.  The results are the same bits either way.
+// Taken from 384 MB on: below 256 MB the caches serve the second reading of the two passes.  256 x 64064 x 64 float16 (2.1 GB) takes
+// 1062 us, in two passes 1255; 64 x 64064 x 64 float32 459 and 667; 262 MB of either type 149 to 201 and 163 to 179; 131 MB 85 and 80.
+// (Backward, with x and gy in registers, it lost: 65 M bfloat16 elements 190 us, in two passes 146 -- a sample then has twice the workgroups,
+// and the last one adds up a row of channels from each.)
+constexpr long SHARED_LEAST = 384l << 20;          // bytes of x
+constexpr int SHARED_MOST = 128;                   // workgroups of a sample, of the 512 that are resident
+constexpr long WAIT_TICKS = 200000;                // of the 100 MHz clock: 2 ms
+long g_wait_ticks = WAIT_TICKS;
+struct SharedP {
+    const void* x;
+    const void* w;
+    const void* b;
+    void* y;
+    float* mean;
+    float* rstd;
+    unsigned long long* stats;           // [N][G][chunks] {mean, sum of squared deviations}
+    int* state;                          // zeroed: [N] arrived, [N] ready, given up, [N][chunks] written
+    long N, S, wait;
+    int rows, chunks, C, G, wdtype;
+    int glanes, clanes;                  // lanes that add up a group's channels, and a group's chunks: powers of two up to 64
+    float eps;
+};
+__device__ __forceinline__ float get(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// every store of the workgroup has reached the memory that all XCDs share
+__device__ __forceinline__ void published() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+// true in the workgroup of a sample that arrives last
+__device__ __forceinline__ bool arrive(const SharedP& p, long n, int* word) {
+    published();
+    if (threadIdx.x == 0) *word = __hip_atomic_fetch_add(p.state + n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.chunks - 1;
+    __syncthreads();
+    const bool last = *word;
+    __syncthreads();
+    return last;
+}
+__device__ __forceinline__ void announce(const SharedP& p, long n) {
+    published();
+    if (threadIdx.x == 0) __hip_atomic_store(p.state + p.N + n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// waits for the sample's sums; false: given up
+__device__ __forceinline__ bool await(const SharedP& p, long n, int* word) {
+    if (threadIdx.x == 0) {
+        const long until = wall_clock64() + p.wait;
+        int ok = 0;
+        while (!(ok = __hip_atomic_load(p.state + p.N + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) {
+            if (__hip_atomic_load(p.state + 2 * p.N, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) break;
+            if ((long)wall_clock64() >= until) {
+                __hip_atomic_store(p.state + 2 * p.N, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                break;
+            }
+            __builtin_amdgcn_s_sleep(8);
+        }
+        *word = ok;
+    }
+    __syncthreads();
+    return *word != 0;
+}
+__device__ __forceinline__ void written(const SharedP& p) {
+    if (threadIdx.x == 0) p.state[2 * p.N + 1 + blockIdx.x] = 1;
+}
+template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS, 4) void norm_shared_kernel(SharedP p) {
+    extern __shared__ float scratch[];             // 2 * ONE_THREADS * V floats
+    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE];
+    __shared__ int word;
+    const long n = blockIdx.x / p.chunks;
+    const int chunk = (int)(blockIdx.x % p.chunks), cg = p.C / p.G, K = (p.C + V - 1) / V, RT = ONE_THREADS / K;
+    const int t = threadIdx.x, col = t % K, r0 = t / K, c0 = min(col * V, p.C - V);
+    const long s0 = (long)chunk * p.rows;
+    const int count = r0 < RT ? (int)min((long)p.rows, p.S - s0) : 0, all = (int)min((long)p.rows, p.S - s0);
+    const long first = (n * p.S + s0) * p.C, at = first + c0;
+    const T* const x = reinterpret_cast<const T*>(p.x) + at;
+    Vec<T, V> v[R], k0 = load_vec<T, V>(x);        // deviations are taken from the chunk's first row, as in norm_stats_kernel
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (r0 + u * RT < count) v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
+    float s1[V] = {}, s2[V] = {};
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (r0 + u * RT < count) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = (float)v[u].v[j] - (float)k0.v[j];
+                s1[j] += d;
+                s2[j] = fmaf(d, d, s2[j]);
+            }
+            keep(v[u]);
+        }
+    if (t < K)
+#pragma unroll
+        for (int j = 0; j < V; ++j) grp[c0 + j] = (float)k0.v[j];
+    channel_sums<V>(K, RT, K, p.C, s1, s2, scratch, chan);
+    group_stats(chan, grp, p.G, cg, all, p.glanes, [&](int g, float m, float q) {
+        __hip_atomic_store(p.stats + (n * p.G + g) * p.chunks + chunk, (unsigned long long)__float_as_uint(q) << 32 | __float_as_uint(m), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    });
+    if (arrive(p, n, &word)) {
+        const float scale = 1.f / (float)p.S, share = 1.f / (float)cg;
+        const int L = p.clanes, sub = t % L;
+#pragma unroll 2
+        for (int g = t / L; g < p.G; g += ONE_THREADS / L) {
+            float m[SHARED_MOST / 64], q[SHARED_MOST / 64], cnt[SHARED_MOST / 64], a = 0.f, b = 0.f;
+#pragma unroll
+            for (int i = 0; i < SHARED_MOST / 64; ++i) {
+                const int k = i * L + sub;
+                unsigned long long e = 0;
+                if (k < p.chunks) e = __hip_atomic_load(p.stats + (n * p.G + g) * p.chunks + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                cnt[i] = k < p.chunks ? (float)min((long)p.rows, p.S - (long)k * p.rows) * scale : 0.f;
+                m[i] = __uint_as_float((unsigned)e);
+                q[i] = __uint_as_float((unsigned)(e >> 32));
+                a = fmaf(cnt[i], m[i], a);
+            }
+            const float mean = lanes_sum(a, L);
+#pragma unroll
+            for (int i = 0; i < SHARED_MOST / 64; ++i) {
+                const float d = m[i] - mean;
+                b += fmaf(cnt[i] * d, d, q[i] * share * scale);
+            }
+            b = lanes_sum(b, L);
+            if (sub == 0) {
+                grp[2 * g] = mean;
+                grp[2 * g + 1] = 1.f / sqrtf(b + p.eps);
+                put(p.mean + n * p.G + g, mean);
+                put(p.rstd + n * p.G + g, grp[2 * g + 1]);
+            }
+        }
+        announce(p, n);
+    } else {
+        if (!await(p, n, &word)) return;
+        for (int g = t; g < p.G; g += ONE_THREADS) {
+            grp[2 * g] = get(p.mean + n * p.G + g);
+            grp[2 * g + 1] = get(p.rstd + n * p.G + g);
+        }
+        __syncthreads();
+    }
+    written(p);
+    int gr[V];
+    groups_of<V>(c0, cg, gr);
+    float m[V], a[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        m[j] = grp[2 * gr[j]];
+        a[j] = grp[2 * gr[j] + 1] * load_param(p.w, p.wdtype, c0 + j, 1.f);
+        b[j] = load_param(p.b, p.wdtype, c0 + j, 0.f);
+    }
+    T* const y = reinterpret_cast<T*>(p.y) + at;
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (r0 + u * RT < count) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u].v[j] = (T)sed_act<ACT>(fmaf((float)v[u].v[j] - m[j], a[j], b[j]));
+            store_vec<T, V>(y + (long)(r0 + u * RT) * p.C, v[u]);
+        }
+}
+
+// the rows of the chunks that were given up
+template <typename T, int V, int ACT> __global__ __launch_bounds__(ONE_THREADS) void norm_rest_kernel(SharedP p) {
+    __shared__ int list[ONE_THREADS], left;
+    const long total = p.N * p.chunks;
+    const int t = threadIdx.x, K = (p.C + V - 1) / V, RT = ONE_THREADS / K, c0 = min(t % K * V, p.C - V), r0 = t / K;
+    int gr[V];
+    groups_of<V>(c0, p.C / p.G, gr);
+    for (long base = (long)blockIdx.x * ONE_THREADS; base < total; base += (long)gridDim.x * ONE_THREADS) {
+        __syncthreads();
+        if (t == 0) left = 0;
+        __syncthreads();
+        if (base + t < total && !p.state[2 * p.N + 1 + base + t]) list[atomicAdd(&left, 1)] = (int)(base + t);
+        __syncthreads();
+        for (int i = 0; i < left; ++i) {
+            const long n = list[i] / p.chunks, s0 = (long)(list[i] % p.chunks) * p.rows, at = (n * p.S + s0) * p.C + c0;
+            const int count = r0 < RT ? (int)min((long)p.rows, p.S - s0) : 0;
+            float m[V], a[V], b[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                m[j] = p.mean[n * p.G + gr[j]];
+                a[j] = p.rstd[n * p.G + gr[j]] * load_param(p.w, p.wdtype, c0 + j, 1.f);
+                b[j] = load_param(p.b, p.wdtype, c0 + j, 0.f);
+            }
+            for (int s = r0; s < count; s += RT) {
+                auto v = load_vec<T, V>(reinterpret_cast<const T*>(p.x) + at + (long)s * p.C);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v.v[j] = (T)sed_act<ACT>(fmaf((float)v.v[j] - m[j], a[j], b[j]));
+                store_vec<T, V>(reinterpret_cast<T*>(p.y) + at + (long)s * p.C, v);
+            }
+        }
+    }
+}
+__global__ __launch_bounds__(256) void norm_zero_kernel(int* p, long n) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) p[i] = 0;
 }
 
 int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
@@ -622,12 +878,38 @@ One one_of(long N, long S, int C, int G, int esize, int most) {
     else o.R = each <= 4 ? 4 : most;
     return o;
 }
+// How the kernels that share a sample cut: chunks of rows that fit a workgroup.  chunks = 0: not for them.
+struct Shared {
+    int rows, chunks;
+};
+Shared shared_of(long N, long S, int C, int esize) {
+    const int V = 16 / esize;
+    const long K = (C + V - 1) / V, RT = ONE_THREADS / K;
+    if (C < V || C > MAX_BUNDLE || N * S * C * esize < SHARED_LEAST) return {0, 0};
+    const long most = RT * ONE_FWD, chunks = (S + most - 1) / most;
+    if (chunks > SHARED_MOST || N * chunks >= (1L << 32) / ONE_THREADS) return {0, 0};
+    const long rows = ((S + chunks - 1) / chunks + RT - 1) / RT * RT;        // even shares
+    return {(int)rows, (int)((S + rows - 1) / rows)};
+}
+int lanes_of(int n) {
+    int l = 1;
+    while (l < n && l < 64) l *= 2;
+    return l;
+}
+long state_ints(long N, int chunks) { return 2 * N + 1 + N * chunks; }
 NormP params_of(const Cut& c, const void* x, const void* w, const void* b, int wdtype, long S, int C, int G, float* ws) {
     NormP p{};
     p.x = x; p.w = w; p.b = b; p.wdtype = wdtype;
     p.S = S; p.rows = c.rows; p.chunks = c.chunks; p.C = C; p.G = G; p.CT = c.CT; p.RT = c.RT; p.tiles = c.tiles; p.K = c.K;
     p.parts = ws;
     return p;
+}
+
+// the counters and flags of a launch, cleared; workgroups of the kernel behind it
+unsigned clear(const SharedP& p, hipStream_t stream) {
+    const long ints = state_ints(p.N, p.chunks), nb = (ints + 255) / 256, rest = (p.N * p.chunks + ONE_THREADS - 1) / ONE_THREADS;
+    hipLaunchKernelGGL(norm_zero_kernel, dim3((unsigned)(nb > 1024 ? 1024 : nb)), dim3(256), 0, stream, p.state, ints);
+    return (unsigned)(rest > 1024 ? 1024 : rest);
 }
 
 #define NORM_ACT(KERNEL, T, V)                                                                              \
@@ -661,6 +943,16 @@ NormP params_of(const Cut& c, const void* x, const void* w, const void* b, int w
     if (dtype == SED_F32) { ONE_ACT(KERNEL, MOST, float, 4) }         \
     else if (dtype == SED_F16) { ONE_ACT(KERNEL, MOST, _Float16, 8) } \
     else { ONE_ACT(KERNEL, MOST, __bf16, 8) }
+#define SHARED(T, V, ACT)                                                                                                                             \
+    hipLaunchKernelGGL((norm_shared_kernel<T, V, ACT, ONE_FWD>), dim3((unsigned)(N * sh.chunks)), dim3(ONE_THREADS), 2 * ONE_THREADS * V * 4, stream, p); \
+    hipLaunchKernelGGL((norm_rest_kernel<T, V, ACT>), dim3(rest), dim3(ONE_THREADS), 0, stream, p);
+#define SHARED_ACT(T, V)                        \
+    switch (act) {                              \
+        case SED_ACT_NONE: SHARED(T, V, 0) break; \
+        case SED_ACT_RELU: SHARED(T, V, 1) break; \
+        case SED_ACT_SILU: SHARED(T, V, 2) break; \
+        default: SHARED(T, V, 3)                \
+    }
 #define NORM_PLAIN(KERNEL, T, V) hipLaunchKernelGGL((KERNEL<T, V>), grid, dim3(THREADS), 0, stream, p);
 
 }  // namespace
@@ -668,6 +960,8 @@ NormP params_of(const Cut& c, const void* x, const void* w, const void* b, int w
 SED_API long sed_group_norm_ws_floats(int dtype, long N, long S, int C, int G, int backward) {
     if (bad_shape(dtype, SED_F32, N, S, C, G, 0)) return 0;
     if (one_of(N, S, C, G, esize_of(dtype), backward ? ONE_BWD : ONE_FWD).threads) return backward ? N * 2 * C : 0;
+    const Shared sh = shared_of(N, S, C, esize_of(dtype));
+    if (!backward && sh.chunks) return 1 + N * G * sh.chunks * 2 + state_ints(N, sh.chunks);
     const long parts = N * cut_of(N, S, C, esize_of(dtype)).chunks * 2 * C;
     return backward ? parts + N * 2 * C + N * 2 * G : parts;
 }
@@ -679,8 +973,20 @@ SED_API int sed_group_norm_fwd(const void* x, const void* weight, const void* bi
     if (!one.threads && !ws) return SED_EINVAL;
     if (one.threads) {
         const dim3 grid((unsigned)(N * one.bundles));
-        OneP p{x, nullptr, weight, bias, y, mean, rstd, nullptr, S, C, G, one.per, one.bundles, wdtype, eps};
+        OneP p{x, nullptr, weight, bias, y, mean, rstd, nullptr, S, C, G, one.per, one.bundles, wdtype, lanes_of(C / G), eps};
         ONE_TYPE(norm_one_kernel, ONE_FWD)
+        SED_LAUNCH_CHECK();
+        return 0;
+    }
+    const Shared sh = shared_of(N, S, C, esize_of(dtype));
+    if (sh.chunks) {
+        float* const stats = ws + (reinterpret_cast<uintptr_t>(ws) & 7) / 4;          // 8-byte numbers
+        const SharedP p{x, weight, bias, y, mean, rstd, reinterpret_cast<unsigned long long*>(stats), reinterpret_cast<int*>(stats + N * G * sh.chunks * 2),
+                        N, S, g_wait_ticks, sh.rows, sh.chunks, C, G, wdtype, lanes_of(C / G), lanes_of(sh.chunks), eps};
+        const unsigned rest = clear(p, stream);
+        if (dtype == SED_F32) { SHARED_ACT(float, 4) }
+        else if (dtype == SED_F16) { SHARED_ACT(_Float16, 8) }
+        else { SHARED_ACT(__bf16, 8) }
         SED_LAUNCH_CHECK();
         return 0;
     }
@@ -702,7 +1008,7 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
     const One one = one_of(N, S, C, G, esize_of(dtype), ONE_BWD);
     if (one.threads) {
         const dim3 grid((unsigned)(N * one.bundles));
-        OneP p{x, gy, weight, bias, gx, const_cast<float*>(mean), const_cast<float*>(rstd), ws, S, C, G, one.per, one.bundles, wdtype, 0.f};
+        OneP p{x, gy, weight, bias, gx, const_cast<float*>(mean), const_cast<float*>(rstd), ws, S, C, G, one.per, one.bundles, wdtype, 0, 0.f};
         ONE_TYPE(norm_one_bwd_kernel, ONE_BWD)
         if (gweight || gbias)
             hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, ws, N, C, gweight, gbias, wdtype);
@@ -723,5 +1029,10 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
         hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, chan, N, C, gweight, gbias, wdtype);
     if (gx) { NORM_TYPE(NORM_ACT, norm_bwd_apply_kernel) }
     SED_LAUNCH_CHECK();
+    return 0;
+}
+
+SED_API int sed_group_norm_set_wait(long ticks) {
+    g_wait_ticks = ticks < 0 ? WAIT_TICKS : ticks;
     return 0;
 }

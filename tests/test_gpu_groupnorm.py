@@ -275,3 +275,89 @@ def test_c_entries_refuse_bad_arguments():
     assert fwd(S=1 << 20, ws=None) == -22
     assert h.sed_group_norm_ws_floats(0, 2, 3, 8, 3, 0) == 0 and h.sed_group_norm_ws_floats(0, 2, 3, 8, 2, 1) > 0
     assert h.sed_group_norm_ws_floats(0, 2, 1 << 20, 8, 2, 0) > 0
+
+
+def _large(n, rows, channels, dtype, seed):
+    torch.manual_seed(seed)
+    x = torch.empty((n, rows, channels), dtype=dtype, device="cuda").normal_()
+    x.mul_(torch.linspace(0.5, 2.0, channels, device="cuda").to(dtype)).add_(torch.linspace(-2.0, 3.0, channels, device="cuda").to(dtype))
+    return x, 1 + 0.2 * torch.randn(channels, device="cuda"), 0.2 * torch.randn(channels, device="cuda")
+
+
+LARGE = [(torch.float16, 9, 63337, 384, 8), (torch.bfloat16, 300, 8003, 91, 7), (torch.float32, 64, 16001, 128, 32), (torch.float32, 1030, 100, 1000, 1),
+         (torch.float16, 40, 20011, 257, 257)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n,rows,channels,groups", LARGE)
+def test_samples_shared_by_many_workgroups(dtype, n, rows, channels, groups):
+    """Inputs beyond 384 MB: the rows of a sample stay in several workgroups.  Against 64 bits, and bit for bit where they give up at once
+    and the second kernel writes the rows, in three launches that follow each other and in two that run side by side."""
+    from sound_event_detection_dcase2017_task4_amd import _lib
+    x, w, b = _large(n, rows, channels, dtype, 3)
+    run = lambda: ops.group_norm_act(x, groups, w, b, activation="silu")  # noqa: E731
+    with torch.no_grad():
+        y = run()
+        for k in {0, n // 2, n - 1}:
+            xd = x[k].double().reshape(rows, groups, -1)
+            mean, var = xd.mean(dim=(0, 2), keepdim=True), xd.var(dim=(0, 2), keepdim=True, unbiased=False)
+            z = ((xd - mean) / torch.sqrt(var + 1e-5)).reshape(rows, channels) * w.double() + b.double()
+            want = F.silu(z)
+            dev = float((xd - xd[:1]).abs().max() / var.min().sqrt())     # of a channel from its first row
+            far = float((mean.abs() / var.sqrt()).max())
+            # sums of at most 16 rows a thread, then trees and the joined chunks, as in _check
+            zerr = (100 + 8 * dev + 2 * far) * H * float(w.abs().max())
+            tol = HALF[dtype] * want.abs() * (1 + 2.0 ** -8) + 1.2 * zerr + 12 * H * (1 + want.abs()) + (6e-8 if dtype == torch.float16 else 0)
+            assert ((y[k].double() - want).abs() <= tol).all()
+        hooks = _lib.test_hooks()
+        try:
+            for wait in (0, -1, 0):
+                hooks.sed_group_norm_set_wait(wait)
+                assert torch.equal(run(), y), wait
+        finally:
+            hooks.sed_group_norm_set_wait(-1)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            a = run()
+        c = run()
+        torch.cuda.synchronize()
+        assert torch.equal(a, y) and torch.equal(c, y)
+
+
+@gpu
+def test_shared_samples_in_a_graph_and_in_training():
+    x, w, b = _large(70, 25000, 128, torch.bfloat16, 5)
+    with torch.no_grad():
+        ops.group_norm_act(x, 8, w, b)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.group_norm_act(x, 8, w, b)
+        for _ in range(3):
+            x.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, ops.group_norm_act(x, 8, w, b))
+    gy = torch.empty_like(x).normal_()
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(ops.group_norm_act(x, 8, w, b, activation="gelu"), leaves, gy)
+    part = torch.autograd.grad(ops.group_norm_act(x[:20], 8, w, b, activation="gelu"), leaves, gy[:20])        # 128 MB: in two passes
+    # x's gradient: statistics that differ by a few H, then one rounding to bfloat16 each: a step of it apart at most, and mostly equal
+    d, s = (got[0][:20].float() - part[0][:20].float()).abs(), part[0][:20].float().abs()
+    assert (d <= 2 * HALF[torch.bfloat16] * 1.01 * s + 1e-5 * s.max()).all() and (d > 0).float().mean() < 0.01
+
+
+@gpu
+def test_a_nan_and_an_infinity_stay_in_their_sample_when_shared():
+    x, w, b = _large(70, 25000, 128, torch.bfloat16, 6)
+    with torch.no_grad():
+        clean = ops.group_norm_act(x, 8, w, b, activation="relu")
+        x[3, 24999, 5], x[40, 0, 127] = float("nan"), float("inf")
+        y = ops.group_norm_act(x, 8, w, b, activation="relu")
+    bad = torch.zeros(70, 8, dtype=torch.bool, device="cuda")
+    bad[3, 0], bad[40, 7] = True, True
+    nan = torch.isnan(y).reshape(70, 25000, 8, 16)
+    assert torch.equal(nan.all(dim=3).all(dim=1), bad) and torch.equal(nan.any(dim=3).any(dim=1), bad)
+    keep = ~bad.view(70, 1, 8, 1).expand(70, 25000, 8, 16).reshape(y.shape)
+    assert torch.equal(y[keep], clean[keep])
