@@ -70,6 +70,9 @@ static inline hipError_t sed_amax_clear(float* amax_out, hipStream_t stream) {
                                                             : hipSuccess;
 }
 
+// the bound of waits between workgroups, as sed_gru_set_spin_limit leaves it
+long sed_spin_limit__();
+
 // Split-f16 operand format (csrc/conv_sf16.hip): x = (hi + lo) / s with hi = f16(s*x), lo = f16(s*x - hi), s = the power of two
 // that brings the tensor's amax (or an upper BOUND of it) to [2^13, 2^14).  A tensor stored "as pairs" holds, per channel
 // pair, two dwords {hi0 | hi1 << 16, lo0 | lo1 << 16}: the bytes of the fp32 tensor, and the consumers' staging is a copy.

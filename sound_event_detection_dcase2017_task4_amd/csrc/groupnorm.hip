@@ -11,7 +11,7 @@
 // folded to groups afterwards.  A row that is not a multiple of V channels ends in a vector that overlaps its neighbour (the twice
 // computed channels are written twice with the same value, and counted once), and loads need no more than element alignment.
 #include "common.h"
-#include "sed_hip_test.h"
+#include "sed_hip.h"
 
 SED_OBJECT_FLAGS(groupnorm)
 
@@ -663,7 +663,6 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
 constexpr long SHARED_LEAST = 384l << 20;          // bytes of x
 constexpr int SHARED_MOST = 128;                   // workgroups of a sample, of the 512 that are resident
 constexpr long WAIT_TICKS = 200000;                // of the 100 MHz clock: 2 ms
-long g_wait_ticks = WAIT_TICKS;
 struct SharedP {
     const void* x;
     const void* w;
@@ -982,7 +981,7 @@ SED_API int sed_group_norm_fwd(const void* x, const void* weight, const void* bi
     if (sh.chunks) {
         float* const stats = ws + (reinterpret_cast<uintptr_t>(ws) & 7) / 4;          // 8-byte numbers
         const SharedP p{x, weight, bias, y, mean, rstd, reinterpret_cast<unsigned long long*>(stats), reinterpret_cast<int*>(stats + N * G * sh.chunks * 2),
-                        N, S, g_wait_ticks, sh.rows, sh.chunks, C, G, wdtype, lanes_of(C / G), lanes_of(sh.chunks), eps};
+                        N, S, sed_spin_limit__() < WAIT_TICKS ? sed_spin_limit__() : WAIT_TICKS, sh.rows, sh.chunks, C, G, wdtype, lanes_of(C / G), lanes_of(sh.chunks), eps};
         const unsigned rest = clear(p, stream);
         if (dtype == SED_F32) { SHARED_ACT(float, 4) }
         else if (dtype == SED_F16) { SHARED_ACT(_Float16, 8) }
@@ -1029,10 +1028,5 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
         hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, chan, N, C, gweight, gbias, wdtype);
     if (gx) { NORM_TYPE(NORM_ACT, norm_bwd_apply_kernel) }
     SED_LAUNCH_CHECK();
-    return 0;
-}
-
-SED_API int sed_group_norm_set_wait(long ticks) {
-    g_wait_ticks = ticks < 0 ? WAIT_TICKS : ticks;
     return 0;
 }

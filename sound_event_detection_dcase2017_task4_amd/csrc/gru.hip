@@ -630,6 +630,8 @@ SED_API int sed_gru_seq_supported(int B, int Hd) {
 SED_API long sed_gru_seq_ws_floats(void) { return GRU_FLAG_INTS; }
 SED_API int sed_gru_seq_row_block(void) { return GRU_RB; }
 SED_API long sed_gru_seq_saves_floats(int B, int T) { return B > 0 && T > 0 ? 2L * T * sed_cdiv(B, GRU_RB) * GRU_RB * 4 * GH : 0; }
+long sed_spin_limit__() { return g_spin_limit; }
+
 SED_API int sed_gru_set_spin_limit(long spins) {
     g_spin_limit = spins > 0 ? spins : (1L << 23);
     return 0;

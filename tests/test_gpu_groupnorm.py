@@ -311,11 +311,11 @@ def test_samples_shared_by_many_workgroups(dtype, n, rows, channels, groups):
             assert ((y[k].double() - want).abs() <= tol).all()
         hooks = _lib.test_hooks()
         try:
-            for wait in (0, -1, 0):
-                hooks.sed_group_norm_set_wait(wait)
+            for wait in (1, 0, 1):                         # one tick, the default, one tick
+                hooks.sed_gru_set_spin_limit(wait)
                 assert torch.equal(run(), y), wait
         finally:
-            hooks.sed_group_norm_set_wait(-1)
+            hooks.sed_gru_set_spin_limit(0)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):

@@ -154,3 +154,37 @@ def test_recorded_again_under_checkpointing():
     plain = torch.autograd.grad(layer(x).sum(), leaves)
     again = torch.autograd.grad(checkpoint(layer, x, use_reentrant=False).sum(), leaves)
     assert all(torch.equal(a, b) for a, b in zip(plain, again))
+
+
+@gpu
+def test_a_model_of_the_package_under_adamw():
+    """Cnn_9layers_FrameAvg without a flat buffer: its gradients reach p.grad, the step is AdamW's, and the packed weights follow it."""
+    import numpy as np
+
+    from oracle import model as om
+    from sound_event_detection_dcase2017_task4_amd.pytorch import models
+    from sound_event_detection_dcase2017_task4_amd.pytorch.losses import clip_bce
+    build = lambda: models.Cnn_9layers_FrameAvg(32000, 1024, 320, 64, 50, 14000, 17)  # noqa: E731
+    model = build()
+    model.load_state_dict(om.recipe_state("Cnn_9layers_FrameAvg", 5))
+    model = model.cuda().train()
+    rs = np.random.RandomState(1)
+    x, y = torch.from_numpy((rs.randn(4, 32000) * 0.1).astype(np.float32)).cuda(), torch.from_numpy((rs.rand(4, 17) < 0.2).astype(np.float32)).cuda()
+    opt = optim.FusedAdamW(model, lr=1e-3, weight_decay=0.01)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in opt.params]
+    want = torch.optim.AdamW(twins, lr=1e-3, weight_decay=0.01, eps=1e-8)
+    for _ in range(2):
+        opt.zero_grad()
+        clip_bce(model(x), {"target": y}).backward()
+        for p, q in zip(opt.params, twins):
+            q.grad = None if p.grad is None else p.grad.detach().clone()
+        opt.step()
+        want.step()
+        for p, q in zip(opt.params, twins):                # both count the same roundings: of the parameter and of an update of up to lr
+            assert (p.detach() - q.detach()).abs().max() <= 16 * H * (float(q.detach().abs().max()) + 1e-3) + 1e-3 * 64 * H
+    model.eval()
+    fresh = build()
+    fresh.load_state_dict(model.state_dict())
+    fresh = fresh.cuda().eval()
+    with torch.no_grad():
+        assert torch.equal(model(x)["clipwise_output"], fresh(x)["clipwise_output"])
