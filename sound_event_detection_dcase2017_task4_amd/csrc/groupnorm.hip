@@ -31,9 +31,10 @@ Cut cut_of(long N, long S, int C, int esize) {
     Cut c;
     c.V = C >= 16 / esize ? 16 / esize : 1;
     c.K = (C + c.V - 1) / c.V;
-    c.CT = c.K < THREADS ? c.K : THREADS;
+    // up to 1 KB of a row, so that a chunk has many rows: its sums, which are written and read again, are then little beside them
+    c.tiles = (c.K + 63) / 64;
+    c.CT = (c.K + c.tiles - 1) / c.tiles;
     c.RT = THREADS / c.CT;
-    c.tiles = (c.K + c.CT - 1) / c.CT;
     // enough workgroups to fill 256 CUs eight times over, at least UNROLL rows per thread, at most 64 so that a sum's chain stays short
     const long want = (2048 + N * c.tiles - 1) / (N * c.tiles);
     long rows = (S + want - 1) / want;
@@ -173,37 +174,85 @@ template <typename T, int V> __global__ __launch_bounds__(THREADS) void norm_sta
     });
 }
 
+// The kernels that join a sample's chunks take a bundle of groups each, all of a workgroup's threads on channels x chunks: f(chunk, channel)
+// summed over the chunks, per channel, into out[channel - c0] (LDS) for the channels from c0 to c1.  scratch: JOIN floats.
+constexpr int JOIN = 1024;
+constexpr int MAX_BUNDLE = 1024;         // channels of a bundle, and of a group that is held in LDS
+template <typename F, typename W> __device__ __forceinline__ void chunk_sums(long chunks, int c0, int c1, float* scratch, F f, W write) {
+    const int t = threadIdx.x, T = blockDim.x, lanes = min(T, c1 - c0), share = T / lanes, lane = t % lanes, first = t / lanes;
+    for (int c = c0; c < c1; c += lanes) {
+        const int k = c + lane;
+        float a = 0.f;
+        if (first < share && k < c1)
+#pragma unroll 4
+            for (long i = first; i < chunks; i += share) a += f(i, k);
+        __syncthreads();
+        scratch[t] = a;
+        // halves of the lanes' shares, added pairwise
+        for (int n = share; n > 1;) {
+            const int half = (n + 1) / 2;
+            __syncthreads();
+            if (first + half < n) scratch[t] += scratch[t + half * lanes];
+            n = half;
+        }
+        __syncthreads();
+        if (t < lanes && k < c1) write(k, scratch[t]);
+    }
+    __syncthreads();
+}
+// How they cut: 64 channels' worth of groups in a workgroup, as far as there are 256 workgroups, and a thread for eight numbers
+struct Join {
+    int per, threads;
+    long blocks;
+};
+Join join_of(long N, long chunks, int C, int G) {
+    const int cg = C / G;
+    Join j;
+    j.per = cg >= 64 ? 1 : 64 / cg < G ? 64 / cg : G;
+    const long most = N * G / 256;
+    if (j.per > most) j.per = most > 1 ? (int)most : 1;
+    const long want = chunks * j.per * cg / 8;
+    j.threads = 64;
+    while (j.threads < JOIN && j.threads < want) j.threads *= 2;
+    j.blocks = N * ((G + j.per - 1) / j.per);
+    return j;
+}
+
 // mean and 1 / sqrt(variance + eps) of a group from its chunks' means and squared deviations: two passes over numbers in the caches
-__global__ __launch_bounds__(128) void norm_finalize_kernel(const float* parts, long S, long rows, long chunks, int C, int G, float eps, float* mean, float* rstd) {
-    __shared__ float red[2];
-    const long n = blockIdx.x / G;
-    const int g = (int)(blockIdx.x % G), cg = C / G;
-    const float* const base = parts + n * chunks * 2 * C + g * cg;
-    const long total = chunks * cg;
+__global__ __launch_bounds__(JOIN) void norm_finalize_kernel(const float* parts, long S, long rows, long chunks, int C, int G, int per, float eps, float* mean, float* rstd) {
+    __shared__ float scratch[JOIN], chan[MAX_BUNDLE], means[64];
+    const int bundles = (G + per - 1) / per, cg = C / G;
+    const long n = blockIdx.x / bundles;
+    const int g0 = (int)(blockIdx.x % bundles) * per, g1 = min(G, g0 + per), t = threadIdx.x;
+    const float* const base = parts + n * chunks * 2 * C;
     const float scale = 1.f / ((float)S * (float)cg);
-    float a = 0.f;
-    for (long e = threadIdx.x; e < total; e += 128) {
-        const long i = e / cg;
-        const float cnt = (float)min(rows, S - i * rows);
-        a = fmaf(cnt * scale, base[i * 2 * C + e % cg], a);
+    auto count = [&](long i) { return (float)min(rows, S - i * rows); };
+    // sums over a group's channels; a channel beyond the LDS is added to the one that it shares a place with
+    auto group_sum = [&](int g) {
+        float a = 0.f;
+        for (int k = t & 63; k < min(cg, MAX_BUNDLE); k += 64) a += chan[(g - g0) * cg + k];
+        return wave_sum(a);
+    };
+    auto add = [&](int k, float v) {
+        const int at = k - g0 * cg;
+        chan[at % MAX_BUNDLE] = at < MAX_BUNDLE ? v : chan[at % MAX_BUNDLE] + v;
+    };
+    chunk_sums(chunks, g0 * cg, g1 * cg, scratch, [&](long i, int c) { return count(i) * scale * base[i * 2 * C + c]; }, add);
+    for (int g = g0 + (t >> 6); g < g1; g += (int)blockDim.x / 64) {
+        const float m = group_sum(g);
+        if ((t & 63) == 0) means[g - g0] = m;
     }
-    a = wave_sum(a);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    const float m = red[0] + red[1];
-    __syncthreads();
-    float v = 0.f;
-    for (long e = threadIdx.x; e < total; e += 128) {
-        const long i = e / cg;
-        const float cnt = (float)min(rows, S - i * rows), d = base[i * 2 * C + e % cg] - m;
-        v += fmaf(cnt * d, d, base[i * 2 * C + C + e % cg]) * scale;
-    }
-    v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        mean[blockIdx.x] = m;
-        rstd[blockIdx.x] = 1.f / sqrtf(red[0] + red[1] + eps);
+    chunk_sums(chunks, g0 * cg, g1 * cg, scratch, [&](long i, int c) {
+        const float k = count(i), d = base[i * 2 * C + c] - means[per == 1 ? 0 : c / cg - g0];
+        return fmaf(k * d, d, base[i * 2 * C + C + c]) * scale;
+    }, add);
+    for (int g = g0 + (t >> 6); g < g1; g += (int)blockDim.x / 64) {
+        const float v = group_sum(g);
+        if ((t & 63) == 0) {
+            mean[n * G + g] = means[g - g0];
+            rstd[n * G + g] = 1.f / sqrtf(v + eps);
+        }
     }
 }
 
@@ -285,39 +334,19 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
     });
 }
 
-// per (sample, bundle of `per` groups): the chunks' sums per channel, chan [N][2][C], and the groups' two means, coef [N][G][2].  A channel's
-// chunks are shared out to as many threads as there are for it.
-__global__ __launch_bounds__(256) void norm_bwd_fold_kernel(const float* parts, long S, long chunks, int C, int G, int per, const void* w, int wdtype, float* chan, float* coef) {
-    __shared__ float red[2][256];
+// per (sample, bundle of `per` groups): the chunks' sums per channel, chan [N][2][C], and the groups' two means, coef [N][G][2]
+__global__ __launch_bounds__(JOIN) void norm_bwd_fold_kernel(const float* parts, long S, long chunks, int C, int G, int per, const void* w, int wdtype, float* chan, float* coef) {
+    __shared__ float scratch[JOIN];
     const int bundles = (G + per - 1) / per, cg = C / G;
     const long n = blockIdx.x / bundles;
-    const int g0 = (int)(blockIdx.x % bundles) * per, c0 = g0 * cg, c1 = min(G, g0 + per) * cg, t = threadIdx.x;
+    const int g0 = (int)(blockIdx.x % bundles) * per, g1 = min(G, g0 + per), t = threadIdx.x;
     const float* const base = parts + n * chunks * 2 * C;
-    const int lanes = min(256, c1 - c0), share = 256 / lanes, lane = t % lanes, first = t / lanes;
-    for (int c = c0; c < c1; c += lanes) {         // more than 256 channels only where per is 1
-        float a = 0.f, b = 0.f;
-        const int k = c + lane;
-        if (first < share && k < c1)
-#pragma unroll 4
-            for (long i = first; i < chunks; i += share) {
-                a += base[i * 2 * C + k];
-                b += base[i * 2 * C + C + k];
-            }
-        __syncthreads();
-        red[0][t] = a;
-        red[1][t] = b;
-        __syncthreads();
-        if (t < lanes && k < c1) {
-            for (int i = 1; i < share; ++i) {
-                a += red[0][i * lanes + t];
-                b += red[1][i * lanes + t];
-            }
-            chan[n * 2 * C + k] = a;
-            chan[n * 2 * C + C + k] = b;
-        }
-    }
-    __syncthreads();                               // the workgroup's own stores to chan are read back below
-    for (int g = g0 + (t >> 6); g < min(G, g0 + per); g += 4) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+        chunk_sums(chunks, g0 * cg, g1 * cg, scratch, [&](long i, int c) { return base[(i * 2 + which) * C + c]; },
+                   [&](int c, float v) { chan[(n * 2 + which) * C + c] = v; });
+    // the workgroup's own stores to chan are read back
+    for (int g = g0 + (t >> 6); g < g1; g += (int)blockDim.x / 64) {
         float a = 0.f, b = 0.f;
         for (int k = t & 63; k < cg; k += 64) {
             const int c = g * cg + k;
@@ -420,7 +449,6 @@ struct OneP {
     int glanes;                          // lanes that add up a group's channels: a power of two up to 64
     float eps;
 };
-constexpr int MAX_BUNDLE = 1024;         // channels of a bundle
 constexpr int ONE_THREADS = 512, ONE_FWD = 16, ONE_BWD = 8;        // threads, and 16-byte vectors of x that one of them holds
 
 // Sums of a[V], b[V] over the row lanes of each of the bundle's channels, left in out[2][channels] (LDS).  scratch: 2 * blockDim * V floats.
@@ -851,7 +879,7 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(int* p, long n) {
 int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
 bool bad_shape(int dtype, int wdtype, long N, long S, int C, int G, int act) {
     return dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2 || N < 1 || S < 1 || C < 1 || G < 1 || C % G || act < 0 || act > 3 ||
-           N * G >= 1L << 25 || cut_of(N, S, C, esize_of(dtype)).blocks >= 1L << 24;         // a launch takes fewer than 2^32 threads
+           N * G >= 1L << 22 || cut_of(N, S, C, esize_of(dtype)).blocks >= 1L << 24;         // a launch takes fewer than 2^32 threads
 }
 // How the one-pass kernels cut: bundles of whole groups with at least 128 bytes of a row (or all of it), a workgroup of so many threads
 // that each holds up to R vectors.  threads = 0: the rows do not fit, or a row has fewer channels than a vector.
@@ -994,7 +1022,8 @@ SED_API int sed_group_norm_fwd(const void* x, const void* weight, const void* bi
     NormP p = params_of(c, x, weight, bias, wdtype, S, C, G, ws);
     p.y = y; p.mean = mean; p.rstd = rstd;
     NORM_TYPE(NORM_PLAIN, norm_stats_kernel)
-    hipLaunchKernelGGL(norm_finalize_kernel, dim3((unsigned)(N * G)), dim3(128), 0, stream, ws, S, c.rows, c.chunks, C, G, eps, mean, rstd);
+    const Join j = join_of(N, c.chunks, C, G);
+    hipLaunchKernelGGL(norm_finalize_kernel, dim3((unsigned)j.blocks), dim3(j.threads), 0, stream, ws, S, c.rows, c.chunks, C, G, j.per, eps, mean, rstd);
     NORM_TYPE(NORM_ACT, norm_apply_kernel)
     SED_LAUNCH_CHECK();
     return 0;
@@ -1021,9 +1050,8 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
     float* const coef = chan + N * 2 * C;
     p.gy = gy; p.y = gx; p.mean = mean; p.rstd = rstd; p.coef = coef;
     NORM_TYPE(NORM_ACT, norm_bwd_sums_kernel)
-    const int cg = C / G, per = cg >= 64 ? 1 : 64 / cg < G ? 64 / cg : G;
-    hipLaunchKernelGGL(norm_bwd_fold_kernel, dim3((unsigned)(N * ((G + per - 1) / per))), dim3(256), 0, stream, ws, S, c.chunks, C, G, per, weight, wdtype,
-                       chan, coef);
+    const Join j = join_of(N, c.chunks, C, G);
+    hipLaunchKernelGGL(norm_bwd_fold_kernel, dim3((unsigned)j.blocks), dim3(j.threads), 0, stream, ws, S, c.chunks, C, G, j.per, weight, wdtype, chan, coef);
     if (gweight || gbias)
         hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, chan, N, C, gweight, gbias, wdtype);
     if (gx) { NORM_TYPE(NORM_ACT, norm_bwd_apply_kernel) }
