@@ -2154,14 +2154,14 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
 
 def adamw_(rows, chunks, nchunks, m, v, m_scale, v_scale, master, state_bits, hyper, step, grad_scale=1.0, guard=None, skipped=None):
     """One AdamW step over the tensors of `rows` (device int64 (tensors, 6)) in one launch: see include/sed_hip.h, sed_adamw.
-    hyper: host float64 array (groups, 5).  guard (default: on while the split-f16 kernels are in use): the step is refused when a
+    hyper: array.array('d') of five a group.  guard (default: on while the split-f16 kernels are in use): the step is refused when a
     split-f16 kernel met a NaN / inf operand; see NonFiniteOperand.  optim.FusedAdamW keeps the tables."""
     _chk_dev(rows, chunks, m, v)
     if guard is None:
         guard = USE_SF16 and skipped is not None
     invalidate_weight_caches()                     # parameters change through raw pointers: `_version` does not see it
     _call("sed_adamw", _ptr(rows), _ptr(chunks), nchunks, _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), _ptr(master), state_bits,
-          hyper.ctypes.data, hyper.shape[0], step, grad_scale, _sf16_err_dev_ptr(m.device) if guard else None,
+          hyper.buffer_info()[0], len(hyper) // 5, step, grad_scale, _sf16_err_dev_ptr(m.device) if guard else None,
           _ptr(skipped) if guard else None, _stream())
 
 

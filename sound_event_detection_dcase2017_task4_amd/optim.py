@@ -13,6 +13,7 @@ therefore never move, which equals torch.optim.Adam skipping `grad is None` para
 `direct_grads=True` means "this backward pass DEFINES the gradient" (what zero_grad() + backward() gives); accumulating
 several backward passes into one step needs `direct_grads=False` (plain autograd accumulation into the same views).
 """
+import array
 import collections
 
 import numpy as np
@@ -417,13 +418,14 @@ class FusedAdamW(object):
         torch.cuda.current_stream(dev).synchronize()        # the buffers are complete when this returns: any stream may use them
 
     def _hyper(self):
+        """lr, beta1, beta2, eps, weight_decay of every group as one array of doubles, which the launch copies."""
         rows = []
         for g in self.param_groups:
             lr, (b1, b2), eps, wd = float(g["lr"]), g["betas"], float(g["eps"]), float(g["weight_decay"])
             if not (lr >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and wd >= 0.0):
                 raise ValueError("invalid lr / betas / eps / weight_decay: %r" % ((lr, (b1, b2), eps, wd),))
-            rows.append((lr, b1, b2, eps, wd))
-        return np.array(rows, dtype=np.float64)
+            rows += (lr, b1, b2, eps, wd)
+        return array.array("d", rows)
 
     def _check_params(self):
         dev, spans = self.params[0].device, []

@@ -295,3 +295,13 @@ def test_c_entries_refuse_bad_arguments():
         assert bwd(**bad) == -22, bad
     assert h.sed_linear_fwd_ws_bytes(16, 16, 1, 100, 8, 9) > 0 and h.sed_linear_fwd_ws_bytes(16, 16, 1, 64, 8, 9) == 0
     assert h.sed_linear_fwd_ws_bytes(16, 16, 1, 0, 8, 9) == 0 and h.sed_linear_kept_elements(3, 9) == 48
+
+
+def test_c_entries_refuse_what_a_launch_cannot_hold():
+    from sound_event_detection_dcase2017_task4_amd import _lib
+    h = _lib.lib()
+    for t in (0, 1, 2):
+        for m, n, k in ((1 << 30, 4096, 8), (1 << 30, 8, 4096), (1 << 21, 1 << 21, 8), (8, 1 << 21, 1 << 21), ((1 << 31) - 256, 8, 8)):
+            assert h.sed_linear_fwd_ws_bytes(16, 16, t, m, n, k) == 0
+            assert h.sed_linear_fwd(16, 16, None, None, t, t, m, n, k, 0, 16, None, 16, 1 << 60, None) == -22
+            assert h.sed_linear_bwd(16, 16, 16, None, t, t, m, n, k, 0, 16, None, None, 16, 1 << 60, None) == -22
