@@ -138,14 +138,73 @@ template <int V, typename F> __device__ __forceinline__ void fold_rows(const Nor
     }
 }
 
-// per chunk and channel: mean and sum of squared deviations.  The sums run over x - (the channel's value in the chunk's first row): a
-// member of the set, so that the square of a large common offset never enters a sum.
+// Statistics of a column of numbers in one reading: the sums run over d = x - k0, k0 the column's first number.  A column is what one
+// thread reads of a channel, 64 rows at most: whatever k0 is -- a padded row, an outlier -- the squares that cancel are at most 64 times
+// what k0 itself adds to the group's squares, and the variance keeps 32 - 6 bits' worth of it.
+template <int V> __device__ __forceinline__ void column_stats(int count, const float (&k0)[V], float (&s1)[V], float (&s2)[V]) {      // -> mean, squared deviations
+    const float inv = count ? 1.f / (float)count : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float d = s1[j] * inv;
+        s2[j] = fmaxf(fmaf(-s1[j], d, s2[j]), 0.f) + (s2[j] - s2[j]);         // the difference: 0, or the NaN that fmaxf would drop
+        s1[j] = count ? k0[j] + d : 0.f;
+    }
+}
+// Means and squared deviations of every thread's columns, joined over the row lanes: write(channel, mean, squares).  `count` rows are dealt
+// out to RT lanes; scratch holds 2 * T * V floats, part T.
+template <int V, typename F> __device__ __forceinline__ void join_columns(int T, int CT, int RT, int count, const float (&mean)[V], const float (&sq)[V], float* scratch, float* part, F write) {
+    const int t = threadIdx.x, NC = CT * V, share = max(1, min(T / NC, 16)), lane = NC < T ? t / NC : 0, full = count / RT, more = count % RT;
+    float* const ra = scratch;
+    float* const rb = scratch + T * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        ra[t * V + j] = mean[j];
+        rb[t * V + j] = sq[j];
+    }
+    __syncthreads();
+    const float inv = 1.f / (float)count;
+    for (int base = 0; base < NC; base += T) {     // once where there is more than one thread for a channel
+        const int k = base + (NC < T ? t % NC : t);
+        const bool on = lane < share && k < NC;
+        // means are averaged as differences from one of them: a common offset is rounded once, not with every term
+        const float ref = on ? ra[k] : 0.f;
+        float m = 0.f, q = 0.f;
+        if (on)
+            for (int r = lane; r < RT; r += share) m = fmaf((float)(full + (r < more)) * inv, ra[r * NC + k] - ref, m);
+        if (share > 1) {
+            part[t] = m;
+            __syncthreads();
+            m = 0.f;
+            if (on)
+                for (int i = 0; i < share; ++i) m += part[i * NC + k];
+            __syncthreads();
+        }
+        m += ref;
+        if (on)
+            for (int r = lane; r < RT; r += share) {
+                const float d = ra[r * NC + k] - m;
+                q += fmaf((float)(full + (r < more)) * d, d, rb[r * NC + k]);
+            }
+        if (share > 1) {
+            part[t] = q;
+            __syncthreads();
+            if (on && lane == 0)
+                for (int i = 1; i < share; ++i) q += part[i * NC + k];
+        }
+        if (on && lane == 0) write(k, m, q);
+    }
+    __syncthreads();
+}
+
+// per chunk and channel: mean and sum of squared deviations
 template <typename T, int V> __global__ __launch_bounds__(THREADS) void norm_stats_kernel(NormP p) {
+    __shared__ float scratch[2 * THREADS * V], part[THREADS];
     const Place q = place_of<V>(p);
     const T* const x = reinterpret_cast<const T*>(p.x) + q.n * p.S * p.C + q.c0;
-    float s1[V] = {}, s2[V] = {}, k0[V];
-    if (q.on) {
-        const auto f = load_vec<T, V>(x + q.s0 * p.C);
+    float s1[V] = {}, s2[V] = {}, k0[V] = {};
+    const int rows = (int)(q.s1 - q.s0);
+    if (q.on && q.r < rows) {
+        const auto f = load_vec<T, V>(x + (q.s0 + q.r) * p.C);
 #pragma unroll
         for (int j = 0; j < V; ++j) k0[j] = (float)f.v[j];
         for (long s = q.s0 + q.r; s < q.s1; s += (long)p.RT * UNROLL) {
@@ -164,13 +223,15 @@ template <typename T, int V> __global__ __launch_bounds__(THREADS) void norm_sta
                     }
         }
     }
-    const float inv = 1.f / (float)(q.s1 - q.s0);
+    column_stats<V>(q.r < rows ? (rows - 1 - q.r) / p.RT + 1 : 0, k0, s1, s2);
     float* const out = p.parts + (q.n * p.chunks + q.chunk) * 2 * p.C;
-    const T* const first = reinterpret_cast<const T*>(p.x) + (q.n * p.S + q.s0) * p.C;
-    fold_rows<V>(p, q, s1, s2, [&](int c, float a, float b) {
-        const float m = a * inv;
-        out[c] = (float)first[c] + m;
-        out[p.C + c] = fmaxf(fmaf(-a, m, b), 0.f) + (b - b);              // b - b: 0, or the NaN that fmaxf would drop
+    const int tile = (int)(blockIdx.x % p.tiles);
+    join_columns<V>(THREADS, p.CT, p.RT, rows, s1, s2, scratch, part, [&](int k, float m, float sq) {
+        const int col = tile * p.CT + k / V, own = col * V, c = min(own, p.C - V) + k % V;
+        if (col < p.K && c >= own) {
+            out[c] = m;
+            out[p.C + c] = sq;
+        }
     });
 }
 
@@ -237,9 +298,9 @@ __global__ __launch_bounds__(JOIN) void norm_finalize_kernel(const float* parts,
         const int at = k - g0 * cg;
         chan[at % MAX_BUNDLE] = at < MAX_BUNDLE ? v : chan[at % MAX_BUNDLE] + v;
     };
-    chunk_sums(chunks, g0 * cg, g1 * cg, scratch, [&](long i, int c) { return count(i) * scale * base[i * 2 * C + c]; }, add);
+    chunk_sums(chunks, g0 * cg, g1 * cg, scratch, [&](long i, int c) { return count(i) * scale * (base[i * 2 * C + c] - base[per == 1 ? g0 * cg : c / cg * cg]); }, add);
     for (int g = g0 + (t >> 6); g < g1; g += (int)blockDim.x / 64) {
-        const float m = group_sum(g);
+        const float m = group_sum(g) + base[g * cg];          // averaged as differences from the first chunk's first channel
         if ((t & 63) == 0) means[g - g0] = m;
     }
     __syncthreads();
@@ -525,21 +586,16 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-// Mean and sum of squared deviations of each of `groups` groups of cg channels over `count` rows, from the sums of the deviations from the
-// first row and of their squares (chan[2][channels], LDS, overwritten) and the first row itself; `lanes` (a power of two) share a group,
-// and the first of them passes the two to write(group, mean, squares).
-template <typename F> __device__ __forceinline__ void group_stats(float* chan, const float* first, int groups, int cg, int count, int lanes, F write) {
-    const float inv = 1.f / (float)count, share = 1.f / (float)cg;
+// Mean and sum of squared deviations of each of `groups` groups of cg channels over `count` rows, from its channels' (chan, LDS: the means,
+// and MAX_BUNDLE further the squares); `lanes` (a power of two) share a group, and the first of them passes the two to write.
+template <typename F> __device__ __forceinline__ void group_stats(const float* chan, int groups, int cg, int count, int lanes, F write) {
+    const float share = 1.f / (float)cg;
     const int sub = threadIdx.x % lanes;
     for (int g = threadIdx.x / lanes; g < groups; g += blockDim.x / lanes) {
         float a = 0.f, q = 0.f;
-        for (int c = g * cg + sub; c < (g + 1) * cg; c += lanes) {
-            const float sum = chan[c], m = sum * inv, sq = chan[MAX_BUNDLE + c];
-            chan[c] = first[c] + m;
-            chan[MAX_BUNDLE + c] = fmaxf(fmaf(-sum, m, sq), 0.f) + (sq - sq);        // sq - sq: 0, or the NaN that fmaxf would drop
-            a += chan[c];
-        }
-        const float m = lanes_sum(a, lanes) * share;
+        const float ref = chan[g * cg];
+        for (int c = g * cg + sub; c < (g + 1) * cg; c += lanes) a += chan[c] - ref;
+        const float m = fmaf(lanes_sum(a, lanes), share, ref);
         for (int c = g * cg + sub; c < (g + 1) * cg; c += lanes) {
             const float d = chan[c] - m;
             q += fmaf((float)count * d, d, chan[MAX_BUNDLE + c]);
@@ -551,7 +607,7 @@ template <typename F> __device__ __forceinline__ void group_stats(float* chan, c
 
 template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS, 4) void norm_one_kernel(OneP p) {
     extern __shared__ float scratch[];             // 2 * blockDim * V floats
-    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE], row0[MAX_BUNDLE];
+    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE], part[ONE_THREADS];
     const long n = blockIdx.x / p.bundles;
     const int g0 = (int)(blockIdx.x % p.bundles) * p.per, groups = min(p.per, p.G - g0), cg = p.C / p.G, width = groups * cg;
     const int K = (width + V - 1) / V, RT = blockDim.x / K, t = threadIdx.x, col = t % K, r0 = t / K;
@@ -559,28 +615,34 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
     const int own = col * V, c0 = min(own, width - V);
     const long at = n * p.S * p.C + g0 * cg + c0;
     const T* const x = reinterpret_cast<const T*>(p.x) + at;
-    Vec<T, V> v[R], k0 = load_vec<T, V>(x);        // deviations are taken from the first row, as in norm_stats_kernel
+    Vec<T, V> v[R];
 #pragma unroll
     for (int u = 0; u < R; ++u)
         if (r0 + u * RT < count) v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
-    float s1[V] = {}, s2[V] = {};
+    float s1[V] = {}, s2[V] = {}, k0[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) k0[j] = r0 < count ? (float)v[0].v[j] : 0.f;
 #pragma unroll
     for (int u = 0; u < R; ++u)
         if (r0 + u * RT < count) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = (float)v[u].v[j] - (float)k0.v[j];
+                const float d = (float)v[u].v[j] - k0[j];
                 s1[j] += d;
                 s2[j] = fmaf(d, d, s2[j]);
             }
             keep(v[u]);
         }
-    if (t < K)
-#pragma unroll
-        for (int j = 0; j < V; ++j) row0[c0 + j] = (float)k0.v[j];
-    channel_sums<V>(K, RT, K, width, s1, s2, scratch, chan);
+    column_stats<V>(r0 < count ? (count - 1 - r0) / RT + 1 : 0, k0, s1, s2);
+    join_columns<V>(blockDim.x, K, RT, (int)p.S, s1, s2, scratch, part, [&](int k, float m, float sq) {
+        const int own = k / V * V, c = min(own, width - V) + k % V;
+        if (c >= own) {
+            chan[c] = m;
+            chan[MAX_BUNDLE + c] = sq;
+        }
+    });
     const float scale = 1.f / ((float)p.S * (float)cg);
-    group_stats(chan, row0, groups, cg, (int)p.S, p.glanes, [&](int g, float m, float q) {
+    group_stats(chan, groups, cg, (int)p.S, p.glanes, [&](int g, float m, float q) {
         const float r = 1.f / sqrtf(q * scale + p.eps);
         grp[2 * g] = m;
         grp[2 * g + 1] = r;
@@ -748,7 +810,7 @@ __device__ __forceinline__ void written(const SharedP& p) {
 }
 template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_THREADS, 4) void norm_shared_kernel(SharedP p) {
     extern __shared__ float scratch[];             // 2 * ONE_THREADS * V floats
-    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE];
+    __shared__ float chan[2 * MAX_BUNDLE], grp[2 * MAX_BUNDLE], part[ONE_THREADS];
     __shared__ int word;
     const long n = blockIdx.x / p.chunks;
     const int chunk = (int)(blockIdx.x % p.chunks), cg = p.C / p.G, K = (p.C + V - 1) / V, RT = ONE_THREADS / K;
@@ -757,27 +819,33 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
     const int count = r0 < RT ? (int)min((long)p.rows, p.S - s0) : 0, all = (int)min((long)p.rows, p.S - s0);
     const long first = (n * p.S + s0) * p.C, at = first + c0;
     const T* const x = reinterpret_cast<const T*>(p.x) + at;
-    Vec<T, V> v[R], k0 = load_vec<T, V>(x);        // deviations are taken from the chunk's first row, as in norm_stats_kernel
+    Vec<T, V> v[R];
 #pragma unroll
     for (int u = 0; u < R; ++u)
         if (r0 + u * RT < count) v[u] = load_vec<T, V>(x + (long)(r0 + u * RT) * p.C);
-    float s1[V] = {}, s2[V] = {};
+    float s1[V] = {}, s2[V] = {}, k0[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) k0[j] = r0 < count ? (float)v[0].v[j] : 0.f;
 #pragma unroll
     for (int u = 0; u < R; ++u)
         if (r0 + u * RT < count) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = (float)v[u].v[j] - (float)k0.v[j];
+                const float d = (float)v[u].v[j] - k0[j];
                 s1[j] += d;
                 s2[j] = fmaf(d, d, s2[j]);
             }
             keep(v[u]);
         }
-    if (t < K)
-#pragma unroll
-        for (int j = 0; j < V; ++j) grp[c0 + j] = (float)k0.v[j];
-    channel_sums<V>(K, RT, K, p.C, s1, s2, scratch, chan);
-    group_stats(chan, grp, p.G, cg, all, p.glanes, [&](int g, float m, float q) {
+    column_stats<V>(r0 < count ? (count - 1 - r0) / RT + 1 : 0, k0, s1, s2);
+    join_columns<V>(ONE_THREADS, K, RT, all, s1, s2, scratch, part, [&](int k, float m, float sq) {
+        const int own = k / V * V, c = min(own, p.C - V) + k % V;
+        if (c >= own) {
+            chan[c] = m;
+            chan[MAX_BUNDLE + c] = sq;
+        }
+    });
+    group_stats(chan, p.G, cg, all, p.glanes, [&](int g, float m, float q) {
         __hip_atomic_store(p.stats + (n * p.G + g) * p.chunks + chunk, (unsigned long long)__float_as_uint(q) << 32 | __float_as_uint(m), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
     });
@@ -795,9 +863,11 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
                 cnt[i] = k < p.chunks ? (float)min((long)p.rows, p.S - (long)k * p.rows) * scale : 0.f;
                 m[i] = __uint_as_float((unsigned)e);
                 q[i] = __uint_as_float((unsigned)(e >> 32));
-                a = fmaf(cnt[i], m[i], a);
             }
-            const float mean = lanes_sum(a, L);
+            const float ref = __shfl(m[0], (t & 63) - sub, 64);          // the first chunk's
+#pragma unroll
+            for (int i = 0; i < SHARED_MOST / 64; ++i) a = fmaf(cnt[i], m[i] - ref, a);
+            const float mean = lanes_sum(a, L) + ref;
 #pragma unroll
             for (int i = 0; i < SHARED_MOST / 64; ++i) {
                 const float d = m[i] - mean;

@@ -371,3 +371,23 @@ def test_c_entries_refuse_what_a_launch_cannot_hold():
             assert h.sed_group_norm_ws_floats(t, n, s, c, g, 1) == 0
             assert h.sed_group_norm_fwd(16, None, None, t, 0, n, s, c, g, 1e-5, 0, 16, 16, 16, 16, None) == -22
             assert h.sed_group_norm_bwd(16, 16, None, None, t, 0, n, s, c, g, 0, 16, 16, None, None, None, 16, None) == -22
+
+
+@gpu
+@pytest.mark.parametrize("shape,groups", [((3, 300, 64), 4), ((2, 1000, 24), 3), ((2, 9000, 40), 5), ((1, 40000, 16), 2), ((7, 8, 8), 1), ((6, 125000, 256), 8)])
+@pytest.mark.parametrize("where", [0, -1, 17])
+def test_a_row_far_from_the_others(shape, groups, where):
+    """One row of zeros (a padded frame) beside rows around 1000 sigma: the variance is that row's, but for its sixteenth digit the rest's.
+    A thread reads at most 64 rows of a channel, and sums squares of distances from the first of them: 64 D^2, each product and sum
+    rounded (3 H), against the D^2 that the row adds to the group -- 200 H of the variance at most, half of that of 1 / sigma; the mean is rounded
+    for a thread, a workgroup, a group and a sample, and is off by 6 H of itself at most, which is up to sqrt(rows) sigma."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = 1000.0 + torch.randn(shape, generator=g, device="cuda")
+    x[:, where % shape[1]] = 0.0
+    with torch.no_grad():
+        y = ops.group_norm_act(x, groups)
+    xd = x.double().reshape(shape[0], shape[1], groups, -1)
+    mean, var = xd.mean(dim=(1, 3), keepdim=True), xd.var(dim=(1, 3), keepdim=True, unbiased=False)
+    want = ((xd - mean) / torch.sqrt(var + 1e-5)).reshape(shape)
+    far = float((mean.abs() / var.sqrt()).max())
+    assert ((y.double() - want).abs() <= 100 * H * want.abs() + 6 * H * far + 4 * H).all()
