@@ -381,13 +381,40 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gem
     __shared__ __attribute__((aligned(16))) unsigned char lds[5 * BM * 128];
     gemm_tile<T, PROWS, QROWS, BM, BN, WM, WN, CUT, ACT>(a, blockIdx.x, gridDim.x, lds);
 }
-// both products of a backward pass in one launch, where both are cut into tiles of 64: the first w.tiles workgroups take gz^T x, whose
-// tiles are the longer ones where there are more rows than columns, the others gz W.  Forward and backward of 4000 x 512 x 512 bf16
+// gb [N] of `type` = the column sums of sums [chunks][ld]: 16 columns x ROWS lanes, a power of two
+struct ColumnsP {
+    const float* sums;
+    long chunks;
+    int ld, N;
+    void* gb;
+    int type, blocks;
+};
+template <int ROWS> __device__ __forceinline__ void column_sums(const ColumnsP& p, int bid, float* red) {       // red: ROWS * 17
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = bid * 16 + lane;
+    float v = 0.f;
+    if (c < p.N) {
+#pragma unroll 4
+        for (long i = row; i < p.chunks; i += ROWS) v += p.sums[i * p.ld + c];
+    }
+    red[row * 17 + lane] = v;
+    __syncthreads();
+    for (int s = ROWS / 2; s > 0; s >>= 1) {
+        if (row < s) red[row * 17 + lane] += red[(row + s) * 17 + lane];
+        __syncthreads();
+    }
+    if (row == 0 && c < p.N) store_typed(p.gb, p.type, c, red[lane]);
+}
+
+// both products of a backward pass, and the bias gradient's last sums, in one launch, where both are cut into tiles of 64: the first
+// c.blocks workgroups take the sums, the next `first` gz^T x, whose tiles are the longer ones where there are more rows than columns,
+// the others gz W.  Forward and backward of 4000 x 512 x 512 bf16
 // 44.9 -> 39.8 us, of 4000 x 512 x 2048 86 -> 72, of 500 x 96 x 136 fp32 29.1 -> 24.3.
-template <typename T, bool CUTW, bool CUTX> __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(GemmP w, GemmP x, int first) {
+template <typename T, bool CUTW, bool CUTX> __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(GemmP w, GemmP x, int first, ColumnsP c) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[5 * 64 * 128];
-    if ((int)blockIdx.x < first) gemm_tile<T, true, true, 64, 64, 2, 2, CUTW, 0>(w, blockIdx.x, first, lds);
-    else gemm_tile<T, true, false, 64, 64, 2, 2, CUTX, 0>(x, blockIdx.x - first, gridDim.x - first, lds);
+    const int bid = (int)blockIdx.x - c.blocks;
+    if (bid < 0) column_sums<16>(c, blockIdx.x, reinterpret_cast<float*>(lds));
+    else if (bid < first) gemm_tile<T, true, true, 64, 64, 2, 2, CUTW, 0>(w, bid, first, lds);
+    else gemm_tile<T, true, false, 64, 64, 2, 2, CUTX, 0>(x, bid - first, gridDim.x - c.blocks - first, lds);
 }
 
 // the slices of a cut product, added in order, and the epilogue
@@ -569,22 +596,9 @@ template <typename T, bool WHOLE> void launch_act_grad(const GradP& p, unsigned 
         default: hipLaunchKernelGGL((act_grad_kernel<T, 3, WHOLE>), dim3(blocks), dim3(256), 0, stream, p);
     }
 }
-// gb [N] of `type` = the column sums of sums [chunks][ld]: 16 columns x 64 lanes
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float* sums, long chunks, int ld, int N, void* gb, int type) {
-    __shared__ float red[64][17];
-    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
-    float v = 0.f;
-    if (c < N) {
-#pragma unroll 4
-        for (long i = row; i < chunks; i += 64) v += sums[i * ld + c];
-    }
-    red[row][lane] = v;
-    __syncthreads();
-    for (int s = 32; s > 0; s >>= 1) {
-        if (row < s) red[row][lane] += red[row + s][lane];
-        __syncthreads();
-    }
-    if (row == 0 && c < N) store_typed(gb, type, c, red[0][lane]);
+__global__ __launch_bounds__(1024) void column_sums_kernel(ColumnsP p) {
+    __shared__ float red[64 * 17];
+    column_sums<64>(p, blockIdx.x, red);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -657,18 +671,18 @@ template <typename T, bool PROWS, bool QROWS> void launch_gemm(GemmP a, const Pl
     else if constexpr (sizeof(T) == 2) launch_edge<T, PROWS, QROWS, 256>(a, q, stream);
     launch_join<T>(a, q, stream);
 }
-bool pairs(const Plan& w, const Plan& x) { return w.edge == 64 && x.edge == 64 && (long)w.tm * w.tn * w.slices + (long)x.tm * x.tn * x.slices < 1L << 24; }
-template <typename T> void launch_pair(GemmP w, const Plan& qw, GemmP x, const Plan& qx, float* part, hipStream_t stream) {
+bool pairs(const Plan& w, const Plan& x) { return w.edge == 64 && x.edge == 64 && (long)w.tm * w.tn * w.slices + (long)x.tm * x.tn * x.slices < (1L << 24) - (1L << 17); }
+template <typename T> void launch_pair(GemmP w, const Plan& qw, GemmP x, const Plan& qx, const ColumnsP& c, float* part, hipStream_t stream) {
     place(w, qw, part);
     place(x, qx, part + qw.part_bytes / 4);
     const int first = qw.tm * qw.tn * qw.slices;
-    const dim3 grid((unsigned)(first + qx.tm * qx.tn * qx.slices));
+    const dim3 grid((unsigned)(c.blocks + first + qx.tm * qx.tn * qx.slices));
     if (qw.slices > 1) {
-        if (qx.slices > 1) hipLaunchKernelGGL((gemm_pair_kernel<T, true, true>), grid, dim3(256), 0, stream, w, x, first);
-        else hipLaunchKernelGGL((gemm_pair_kernel<T, true, false>), grid, dim3(256), 0, stream, w, x, first);
+        if (qx.slices > 1) hipLaunchKernelGGL((gemm_pair_kernel<T, true, true>), grid, dim3(256), 0, stream, w, x, first, c);
+        else hipLaunchKernelGGL((gemm_pair_kernel<T, true, false>), grid, dim3(256), 0, stream, w, x, first, c);
     } else {
-        if (qx.slices > 1) hipLaunchKernelGGL((gemm_pair_kernel<T, false, true>), grid, dim3(256), 0, stream, w, x, first);
-        else hipLaunchKernelGGL((gemm_pair_kernel<T, false, false>), grid, dim3(256), 0, stream, w, x, first);
+        if (qx.slices > 1) hipLaunchKernelGGL((gemm_pair_kernel<T, false, true>), grid, dim3(256), 0, stream, w, x, first, c);
+        else hipLaunchKernelGGL((gemm_pair_kernel<T, false, false>), grid, dim3(256), 0, stream, w, x, first, c);
     }
     launch_join<T>(w, qw, stream);
     launch_join<T>(x, qx, stream);
@@ -787,7 +801,6 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         if (N % (16 / es) == 0) launch_act_grad<T, true>(p, (unsigned)(c.chunks * c.tiles), stream);
         else launch_act_grad<T, false>(p, (unsigned)(c.chunks * c.tiles), stream);
     }
-    if (gb && c.chunks > 1) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)sed_cdiv(N, 16)), dim3(1024), 0, stream, sums, c.chunks, (int)ldn, (int)N, gb, btype);
     const void* const dz = gz ? gz : gy;
     pad<T>(x, M, d.px, w, N, d.pw, K, ws, stream);
     const bool wide = K % (16 / es) == 0;
@@ -810,8 +823,10 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         pw = plan_of(N, K, M, es);
     }
     float* const part = reinterpret_cast<float*>(ws);
-    if (gx && gw && pairs(pw, px)) launch_pair<T>(w_, pw, x_, px, part, stream);
+    ColumnsP columns{sums, c.chunks, (int)ldn, (int)N, gb, btype, gb && c.chunks > 1 ? sed_cdiv(N, 16) : 0};
+    if (gx && gw && pairs(pw, px)) launch_pair<T>(w_, pw, x_, px, columns, part, stream);
     else {
+        if (columns.blocks) hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)columns.blocks), dim3(1024), 0, stream, columns);
         if (gx) launch_gemm<T, true, false>(x_, px, part, stream);
         if (gw) launch_gemm<T, true, true>(w_, pw, part, stream);
     }
