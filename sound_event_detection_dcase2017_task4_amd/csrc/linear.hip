@@ -505,13 +505,13 @@ struct PadP {
     const void* src[2];
     void* dst[2];
     long R[2];
-    int C, ld;
+    int C, ld, blocks;                             // blocks: workgroups that share them, 0 where there is nothing to copy
 };
-template <typename T> __global__ __launch_bounds__(256) void pad_kernel(PadP p) {
+template <typename T> __device__ __forceinline__ void pad_lines(const PadP& p) {
     constexpr int E = 16 / sizeof(T);
     const int per = p.ld / E;
     const long first = p.R[0] * per, total = first + p.R[1] * per;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)p.blocks * 256) {
         const int which = i >= first;
         const long r = (i - which * first) / per;
         const int c = (int)(i % per) * E;
@@ -524,9 +524,10 @@ template <typename T> __global__ __launch_bounds__(256) void pad_kernel(PadP p) 
         __builtin_memcpy(reinterpret_cast<T*>(p.dst[which]) + r * p.ld + c, v, 16);
     }
 }
+template <typename T> __global__ __launch_bounds__(256) void pad_kernel(PadP p) { pad_lines<T>(p); }
 
 // gz [M][ld] = gy act'(z) (null: only the sums) and per chunk of rows the column sums of gz in 32 bits, before it is rounded.
-// A thread owns E columns (16 bytes) of every RT-th row of a chunk.
+// A thread owns E columns (16 bytes) of every RT-th row of a chunk.  The first pad.blocks workgroups copy the operands that need it.
 struct GradP {
     const void* gy;
     const void* z;
@@ -536,13 +537,16 @@ struct GradP {
     int btype;
     long M, rows;
     int N, ld, CT, RT, tiles, act;
+    PadP pad;
 };
 template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) void act_grad_kernel(GradP p) {       // WHOLE: N is a multiple of E
     constexpr int E = 16 / sizeof(T), U = 4;
     typedef typename Kept<T>::type Z;
     __shared__ float red[256 * E];
-    const int tile = (int)(blockIdx.x % p.tiles), t = threadIdx.x, col = tile * p.CT + t % p.CT, r = t / p.CT, c = col * E;
-    const long chunk = blockIdx.x / p.tiles, s0 = chunk * p.rows, s1 = min(p.M, s0 + p.rows);
+    if ((int)blockIdx.x < p.pad.blocks) { pad_lines<T>(p.pad); return; }
+    const unsigned bid = blockIdx.x - p.pad.blocks;
+    const int tile = (int)(bid % p.tiles), t = threadIdx.x, col = tile * p.CT + t % p.CT, r = t / p.CT, c = col * E;
+    const long chunk = bid / p.tiles, s0 = chunk * p.rows, s1 = min(p.M, s0 + p.rows);
     const T* const gy = reinterpret_cast<const T*>(p.gy) + c;
     const Z* const kept = reinterpret_cast<const Z*>(p.z) + c;
     float sum[E] = {};
@@ -687,10 +691,10 @@ template <typename T> void launch_pair(GemmP w, const Plan& qw, GemmP x, const P
     launch_join<T>(w, qw, stream);
     launch_join<T>(x, qx, stream);
 }
-// x [M][C] and w [N][C] with lines of a multiple of 16 bytes, those of them that need it, in one launch
-template <typename T> void pad(const void*& x, long M, bool px, const void*& w, long N, bool pw, long C, char*& ws, hipStream_t stream) {
-    if (!px && !pw) return;
+// x [M][C] and w [N][C] with lines of a multiple of 16 bytes, those of them that need it: from here on they are what lies in ws
+template <typename T> PadP pad_of(const void*& x, long M, bool px, const void*& w, long N, bool pw, long C, char*& ws) {
     PadP p{};
+    if (!px && !pw) return p;
     p.C = (int)C; p.ld = (int)padded(C, sizeof(T));
     auto take = [&](int i, const void*& src, long R) {
         p.src[i] = src; p.R[i] = R; p.dst[i] = ws;
@@ -701,7 +705,11 @@ template <typename T> void pad(const void*& x, long M, bool px, const void*& w, 
     if (px) take(used++, x, M);
     if (pw) take(used++, w, N);
     const long nb = ((p.R[0] + p.R[1]) * (p.ld * (long)sizeof(T) / 16) + 255) / 256;
-    hipLaunchKernelGGL((pad_kernel<T>), dim3((unsigned)(nb > 16384 ? 16384 : nb)), dim3(256), 0, stream, p);
+    p.blocks = (int)(nb > 16384 ? 16384 : nb);
+    return p;
+}
+template <typename T> void launch_pad(const PadP& p, hipStream_t stream) {
+    if (p.blocks) hipLaunchKernelGGL((pad_kernel<T>), dim3((unsigned)p.blocks), dim3(256), 0, stream, p);
 }
 
 // rows and columns that 32-bit offsets inside a tile and the tiles of one launch can hold: 2^38 elements of x, W or y at most
@@ -746,7 +754,7 @@ int linear_fwd(const void* x, const void* w, const void* bias, const void* res, 
         return 0;
     }
     const long ld = padded(K, sizeof(T));
-    pad<T>(x, M, needs_pad(x, K, sizeof(T)), w, N, needs_pad(w, K, sizeof(T)), K, ws, stream);
+    launch_pad<T>(pad_of<T>(x, M, needs_pad(x, K, sizeof(T)), w, N, needs_pad(w, K, sizeof(T)), K, ws), stream);
     GemmP a{};
     a.M = (int)M; a.N = (int)N; a.K = ld; a.e = e;
     a.q = {x, ld, (int)M};
@@ -795,14 +803,15 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         sums = reinterpret_cast<float*>(ws);
         ws += up256(c.chunks * ldn * 4);
     }
-    if (gz || gb) {
+    const PadP pad = pad_of<T>(x, M, d.px, w, N, d.pw, K, ws);
+    if (!gz && !gb) launch_pad<T>(pad, stream);
+    else {
         const bool one = gb && c.chunks == 1;
-        GradP p{gy, z, gz, one ? nullptr : sums, one ? gb : nullptr, btype, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act};
-        if (N % (16 / es) == 0) launch_act_grad<T, true>(p, (unsigned)(c.chunks * c.tiles), stream);
-        else launch_act_grad<T, false>(p, (unsigned)(c.chunks * c.tiles), stream);
+        GradP p{gy, z, gz, one ? nullptr : sums, one ? gb : nullptr, btype, M, c.rows, (int)N, (int)ldn, c.CT, c.RT, c.tiles, act, pad};
+        if (N % (16 / es) == 0) launch_act_grad<T, true>(p, (unsigned)(pad.blocks + c.chunks * c.tiles), stream);
+        else launch_act_grad<T, false>(p, (unsigned)(pad.blocks + c.chunks * c.tiles), stream);
     }
     const void* const dz = gz ? gz : gy;
-    pad<T>(x, M, d.px, w, N, d.pw, K, ws, stream);
     const bool wide = K % (16 / es) == 0;
     GemmP x_{}, w_{};
     Plan px{}, pw{};
