@@ -97,9 +97,9 @@ struct Place {
     int c0, own, r;                      // first channel; channels below `own` belong to the neighbour; row lane
     bool on;
 };
-template <int V> __device__ __forceinline__ Place place_of(const NormP& p) {
+template <int V> __device__ __forceinline__ Place place_of(const NormP& p, unsigned bid) {
     Place q;
-    long id = blockIdx.x;
+    long id = bid;
     const int tile = (int)(id % p.tiles);
     id /= p.tiles;
     q.chunk = id % p.chunks;
@@ -199,7 +199,7 @@ template <int V, typename F> __device__ __forceinline__ void join_columns(int T,
 // per chunk and channel: mean and sum of squared deviations
 template <typename T, int V> __global__ __launch_bounds__(THREADS) void norm_stats_kernel(NormP p) {
     __shared__ float scratch[2 * THREADS * V], part[THREADS];
-    const Place q = place_of<V>(p);
+    const Place q = place_of<V>(p, blockIdx.x);
     const T* const x = reinterpret_cast<const T*>(p.x) + q.n * p.S * p.C + q.c0;
     float s1[V] = {}, s2[V] = {}, k0[V] = {};
     const int rows = (int)(q.s1 - q.s0);
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(JOIN) void norm_finalize_kernel(const float* parts,
 }
 
 template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void norm_apply_kernel(NormP p) {
-    const Place q = place_of<V>(p);
+    const Place q = place_of<V>(p, blockIdx.x);
     if (!q.on) return;
     const T* const x = reinterpret_cast<const T*>(p.x) + q.n * p.S * p.C + q.c0;
     T* const y = reinterpret_cast<T*>(p.y) + q.n * p.S * p.C + q.c0;
@@ -350,7 +350,7 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
 
 // per chunk and channel: sum gz and sum gz xhat
 template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void norm_bwd_sums_kernel(NormP p) {
-    const Place q = place_of<V>(p);
+    const Place q = place_of<V>(p, blockIdx.x);
     float s1[V] = {}, s2[V] = {};
     if (q.on) {
         const long at = q.n * p.S * p.C + q.c0;
@@ -425,34 +425,45 @@ __global__ __launch_bounds__(JOIN) void norm_bwd_fold_kernel(const float* parts,
     }
 }
 
-// gbias, gweight [C] of wdtype: the sums of chan [N][2][C] over the samples; 16 channels x 64 sample lanes per workgroup
-__global__ __launch_bounds__(1024) void norm_bwd_params_kernel(const float* chan, long N, int C, void* gw, void* gb, int wdtype) {
-    __shared__ float red[2][64][17];
-    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
+// gbias, gweight [C] of wdtype: the sums of chan [N][2][C] over the samples; 16 channels x ROWS sample lanes per workgroup
+struct ParamsP {
+    const float* chan;
+    long N;
+    int C, wdtype;
+    void* gw;
+    void* gb;
+    int blocks;                          // 0: neither is wanted
+};
+template <int ROWS> __device__ __forceinline__ void param_sums(const ParamsP& p, int bid) {
+    __shared__ float red[2][ROWS][17];
+    const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = bid * 16 + lane;
     float a = 0.f, b = 0.f;
-    if (c < C)
-        for (long n = row; n < N; n += 64) {
-            a += chan[n * 2 * C + c];
-            b += chan[n * 2 * C + C + c];
+    if (c < p.C)
+        for (long n = row; n < p.N; n += ROWS) {
+            a += p.chan[n * 2 * p.C + c];
+            b += p.chan[n * 2 * p.C + p.C + c];
         }
     red[0][row][lane] = a;
     red[1][row][lane] = b;
     __syncthreads();
-    for (int s = 32; s > 0; s >>= 1) {
+    for (int s = ROWS / 2; s > 0; s >>= 1) {
         if (row < s) {
             red[0][row][lane] += red[0][row + s][lane];
             red[1][row][lane] += red[1][row + s][lane];
         }
         __syncthreads();
     }
-    if (row == 0 && c < C) {
-        if (gb) store_param(gb, wdtype, c, red[0][0][lane]);
-        if (gw) store_param(gw, wdtype, c, red[1][0][lane]);
+    if (row == 0 && c < p.C) {
+        if (p.gb) store_param(p.gb, p.wdtype, c, red[0][0][lane]);
+        if (p.gw) store_param(p.gw, p.wdtype, c, red[1][0][lane]);
     }
 }
+__global__ __launch_bounds__(1024) void norm_bwd_params_kernel(ParamsP p) { param_sums<64>(p, blockIdx.x); }
 
-template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void norm_bwd_apply_kernel(NormP p) {
-    const Place q = place_of<V>(p);
+// gx; the first params.blocks workgroups add up the parameters' gradients
+template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void norm_bwd_apply_kernel(NormP p, ParamsP params) {
+    if ((int)blockIdx.x < params.blocks) { param_sums<THREADS / 16>(params, blockIdx.x); return; }
+    const Place q = place_of<V>(p, blockIdx.x - params.blocks);
     if (!q.on) return;
     const long at = q.n * p.S * p.C + q.c0;
     const T* const x = reinterpret_cast<const T*>(p.x) + at;
@@ -949,7 +960,7 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(int* p, long n) {
 int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
 bool bad_shape(int dtype, int wdtype, long N, long S, int C, int G, int act) {
     return dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2 || N < 1 || S < 1 || C < 1 || G < 1 || C % G || act < 0 || act > 3 ||
-           N * G >= 1L << 22 || cut_of(N, S, C, esize_of(dtype)).blocks >= 1L << 24;         // a launch takes fewer than 2^32 threads
+           N * G >= 1L << 22 || cut_of(N, S, C, esize_of(dtype)).blocks + C / 16 + 1 >= 1L << 24;         // a launch takes fewer than 2^32 threads
 }
 // How the one-pass kernels cut: bundles of whole groups with at least 128 bytes of a row (or all of it), a workgroup of so many threads
 // that each holds up to R vectors.  threads = 0: the rows do not fit, or a row has fewer channels than a vector.
@@ -1015,6 +1026,16 @@ unsigned clear(const SharedP& p, hipStream_t stream) {
         case SED_ACT_RELU: hipLaunchKernelGGL((KERNEL<T, V, 1>), grid, dim3(THREADS), 0, stream, p); break; \
         case SED_ACT_SILU: hipLaunchKernelGGL((KERNEL<T, V, 2>), grid, dim3(THREADS), 0, stream, p); break; \
         default: hipLaunchKernelGGL((KERNEL<T, V, 3>), grid, dim3(THREADS), 0, stream, p);                  \
+    }
+#define NORM_APPLY(KERNEL, T, V)                                                                                          \
+    {                                                                                                                     \
+        const dim3 with((unsigned)(params.blocks + c.blocks));                                                            \
+        switch (act) {                                                                                                    \
+            case SED_ACT_NONE: hipLaunchKernelGGL((KERNEL<T, V, 0>), with, dim3(THREADS), 0, stream, p, params); break; \
+            case SED_ACT_RELU: hipLaunchKernelGGL((KERNEL<T, V, 1>), with, dim3(THREADS), 0, stream, p, params); break; \
+            case SED_ACT_SILU: hipLaunchKernelGGL((KERNEL<T, V, 2>), with, dim3(THREADS), 0, stream, p, params); break; \
+            default: hipLaunchKernelGGL((KERNEL<T, V, 3>), with, dim3(THREADS), 0, stream, p, params);                  \
+        }                                                                                                                 \
     }
 #define NORM_TYPE(WHAT, ...)                                                                     \
     if (c.V == 1) {                                                                              \
@@ -1108,8 +1129,8 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
         const dim3 grid((unsigned)(N * one.bundles));
         OneP p{x, gy, weight, bias, gx, const_cast<float*>(mean), const_cast<float*>(rstd), ws, S, C, G, one.per, one.bundles, wdtype, 0, 0.f};
         ONE_TYPE(norm_one_bwd_kernel, ONE_BWD)
-        if (gweight || gbias)
-            hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, ws, N, C, gweight, gbias, wdtype);
+        const ParamsP params{ws, N, C, wdtype, gweight, gbias, gweight || gbias ? sed_cdiv(C, 16) : 0};
+        if (params.blocks) hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)params.blocks), dim3(1024), 0, stream, params);
         SED_LAUNCH_CHECK();
         return 0;
     }
@@ -1122,9 +1143,9 @@ SED_API int sed_group_norm_bwd(const void* x, const void* gy, const void* weight
     NORM_TYPE(NORM_ACT, norm_bwd_sums_kernel)
     const Join j = join_of(N, c.chunks, C, G);
     hipLaunchKernelGGL(norm_bwd_fold_kernel, dim3((unsigned)j.blocks), dim3(j.threads), 0, stream, ws, S, c.chunks, C, G, j.per, weight, wdtype, chan, coef);
-    if (gweight || gbias)
-        hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)sed_cdiv(C, 16)), dim3(1024), 0, stream, chan, N, C, gweight, gbias, wdtype);
-    if (gx) { NORM_TYPE(NORM_ACT, norm_bwd_apply_kernel) }
+    const ParamsP params{chan, N, C, wdtype, gweight, gbias, gweight || gbias ? sed_cdiv(C, 16) : 0};
+    if (gx) { NORM_TYPE(NORM_APPLY, norm_bwd_apply_kernel) }
+    else if (params.blocks) hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((unsigned)params.blocks), dim3(1024), 0, stream, params);
     SED_LAUNCH_CHECK();
     return 0;
 }
