@@ -4,8 +4,9 @@
 //   gz = gy act'(z);  gw = sum gz xhat;  gb = sum gz;  h = gz w;  gx = rstd (h - mean_g(h) - xhat mean_g(h xhat))
 //
 // Bound by HBM.  The statistics of a group need every row of a sample before any element of it can be written.  Where the rows of some
-// groups fit the registers of a workgroup they are read once (the one-pass kernels); beyond that a first pass leaves sums per chunk
-// of rows and channel, a small kernel adds them up, and a second pass reads the rows again.
+// groups fit the registers of a workgroup they are read once (the one-pass kernels); beyond that a first pass leaves statistics per
+// chunk of rows and channel, a small kernel joins them, and a second pass reads the rows again -- forward, and from 384 MB on, only where
+// a sample does not fit the registers of 128 workgroups either.
 //
 // A thread owns V channels (16 bytes) of every RT-th row of a chunk of rows, whatever the group width: sums are held per channel and
 // folded to groups afterwards.  A row that is not a multiple of V channels ends in a vector that overlaps its neighbour (the twice
@@ -506,7 +507,8 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
 }
 
 // ---- one pass: the rows of a bundle of whole groups stay in the registers of one workgroup, up to 128 KB (forward) or 2 x 64 KB
-// (backward), and are read once.
+// (backward), and are read once.  16-bit rows stay packed: 1000 x 300 x 512 bfloat16 takes 192 us forward and 300 backward, with rows that
+// the compiler holds as floats (and half the workgroups on a CU) 489 and 573.
 struct OneP {
     const void* x;
     const void* gy;
