@@ -501,7 +501,8 @@ int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const 
 /* ---- matrix product with bias, activation and residual in its epilogue -----------------------------------------------
  * z = x W^T + b;  y = act(z) + residual:  x [M][K], weight [N][K], residual (nullable), y [M][N] of `dtype` (SED_F32 / SED_F16 /
  * SED_BF16), bias (nullable) [N] of bdtype.  Products are summed in 32 bits and rounded once; 32-bit ones run on the fp32 matrix
- * instructions.  z (nullable): what the backward pass needs of z, sed_linear_kept_elements(M, N) floats (SED_F32) or 16-bit values.
+ * instructions.  z (nullable, 16-byte aligned): what the backward pass needs of z, sed_linear_kept_elements(M, N) floats, or as many
+ * 16-bit values for SED_ACT_RELU beside 16-bit tensors.
  * sed_linear_bwd: gz = gy act'(z) (z nullable without an activation);  gx = gz W [M][K];  gweight = gz^T x [N][K];  gbias = sum gz [N]
  * of bdtype; each nullable (x only serves gweight, weight only gx).  gz is rounded to `dtype` for the two products, gbias is summed
  * before that.

@@ -44,16 +44,13 @@ __device__ __forceinline__ void store_typed(void* p, int type, long i, float v) 
     else reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
 }
 
-// What is kept of z for the backward pass, which reads nothing but act'(z) from it.  16-bit tensors keep it as float16 whatever
-// their type: its 11 bits lose a sixteenth of what gz loses when it is rounded to bfloat16, and beyond +-60000 every derivative has
-// long been 0 or 1.  ReLU keeps 1 or 0, so that a z below the smallest float16 is not lost.
-template <typename T> struct Kept { typedef _Float16 type; };
-template <> struct Kept<float> { typedef float type; };
-template <typename T> __device__ __forceinline__ typename Kept<T>::type keep_z(float z, int act) {
-    if (act == SED_ACT_RELU) return (typename Kept<T>::type)(z > 0.f ? 1.f : 0.f);
-    if (sizeof(T) == 4) return (typename Kept<T>::type)z;
-    return (typename Kept<T>::type)(z > 60000.f ? 60000.f : (z < -60000.f ? -60000.f : z));
-}
+// What is kept of z for the backward pass, which reads nothing but act'(z) from it: z in 32 bits, whatever the tensors' type.  (A z of
+// 16 bits puts |act''(z) z| 2^-12 into a float16 gradient, as much as its own rounding, and as much into a bias gradient of 32 bits.)
+// ReLU keeps 1 or 0, in 16 bits beside 16-bit tensors.
+template <typename T> struct Mask { typedef _Float16 type; };
+template <> struct Mask<float> { typedef float type; };
+template <typename T, int ACT> struct Kept { typedef float type; };
+template <typename T> struct Kept<T, SED_ACT_RELU> { typedef typename Mask<T>::type type; };
 __device__ __forceinline__ float act_of(float z, int act) {
     switch (act) {
         case SED_ACT_RELU: return sed_act<1>(z);
@@ -98,14 +95,20 @@ template <typename T, int V> __device__ __forceinline__ void load_bias(const Epi
     }
 }
 template <typename T, int V, int ACT> __device__ __forceinline__ void finish(const Epilogue& e, long m, int n, int N, float (&v)[V], const float (&bias)[V], const float (&res)[V]) {
-    typedef typename Kept<T>::type Z;
 #pragma unroll
     for (int r = 0; r < V; ++r) v[r] += bias[r];
-    if (e.z) {
-        typename Wide<Z, V>::type k;
+    if (e.z) {                                     // ldz is a multiple of V
+        if ((ACT == RUNTIME ? e.act : ACT) == SED_ACT_RELU) {
+            typedef typename Mask<T>::type Z;
+            typename Wide<Z, V>::type k;
 #pragma unroll
-        for (int r = 0; r < V; ++r) k[r] = keep_z<T>(v[r], ACT == RUNTIME ? e.act : ACT);
-        *reinterpret_cast<typename Wide<Z, V>::type*>(reinterpret_cast<Z*>(e.z) + m * e.ldz + n) = k;      // ldz is a multiple of V
+            for (int r = 0; r < V; ++r) k[r] = (Z)(v[r] > 0.f ? 1.f : 0.f);
+            *reinterpret_cast<typename Wide<Z, V>::type*>(reinterpret_cast<Z*>(e.z) + m * e.ldz + n) = k;
+        } else {
+            float* const z = reinterpret_cast<float*>(e.z) + m * e.ldz + n;
+#pragma unroll
+            for (int r = 0; r < V; r += 4) *reinterpret_cast<floatx4*>(z + r) = floatx4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+        }
     }
 #pragma unroll
     for (int r = 0; r < V; ++r) v[r] = (ACT == RUNTIME ? act_of(v[r], e.act) : sed_act<ACT>(v[r])) + res[r];
@@ -541,7 +544,7 @@ struct GradP {
 };
 template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) void act_grad_kernel(GradP p) {       // WHOLE: N is a multiple of E
     constexpr int E = 16 / sizeof(T), U = 4;
-    typedef typename Kept<T>::type Z;
+    typedef typename Kept<T, ACT>::type Z;
     __shared__ float red[256 * E];
     if ((int)blockIdx.x < p.pad.blocks) { pad_lines<T>(p.pad); return; }
     const unsigned bid = blockIdx.x - p.pad.blocks;

@@ -2072,7 +2072,7 @@ def _linear_fwd(x, weight, bias, residual, act, keep):
     y = x.new_empty(x.shape[:-1] + (N,))
     z = None
     if keep and act:
-        z = x.new_empty(h.sed_linear_kept_elements(M, N), dtype=torch.float16 if dt else torch.float32)
+        z = x.new_empty(h.sed_linear_kept_elements(M, N), dtype=torch.float16 if dt and act == ACTIVATIONS["relu"] else torch.float32)
     px, pw = x.data_ptr(), weight.data_ptr()
     need = h.sed_linear_fwd_ws_bytes(px, pw, dt, M, N, K)
     ws = _bytes(need, x)

@@ -305,3 +305,20 @@ def test_c_entries_refuse_what_a_launch_cannot_hold():
             assert h.sed_linear_fwd_ws_bytes(16, 16, t, m, n, k) == 0
             assert h.sed_linear_fwd(16, 16, None, None, t, t, m, n, k, 0, 16, None, 16, 1 << 60, None) == -22
             assert h.sed_linear_bwd(16, 16, 16, None, t, t, m, n, k, 0, 16, None, None, 16, 1 << 60, None) == -22
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [1, 5, 70, 700])
+def test_bias_gradient_of_16_bit_tensors_has_the_bits_of_its_own_type(m, dtype, act):
+    """A 32-bit bias beside 16-bit tensors: the derivative is that of z in 32 bits, so the roundings of the tensors' type do not enter."""
+    x, w, b, _, gy = _inputs(m, 96, 40, dtype, torch.float32, 31, residual=False)
+    b.requires_grad_(True)
+    got, = torch.autograd.grad(ops.linear_act(x, w, b, act), b, gy)
+    xd, wd, gd = x.double(), w.double(), gy.double()
+    z = (xd @ wd.t() + b.detach().double()).requires_grad_(True)
+    da, = torch.autograd.grad(ACTS[act](z).sum(), z)
+    zerr = _sum_err(96) * (xd.abs() @ wd.abs().t() + b.detach().double().abs()) + 4 * H
+    tol = (gd.abs() * (1.2 * zerr + 16 * H)).sum(0) + _sum_err(m) * (gd * da).abs().sum(0)
+    assert got.dtype == torch.float32 and ((got.double() - (gd * da).sum(0)).abs() <= tol).all()
