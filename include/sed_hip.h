@@ -504,8 +504,9 @@ int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const 
  * instructions.  z (nullable, 16-byte aligned): what the backward pass needs of z, sed_linear_kept_elements(M, N) floats, or as many
  * 16-bit values for SED_ACT_RELU beside 16-bit tensors.
  * sed_linear_bwd: gz = gy act'(z) (z nullable without an activation);  gx = gz W [M][K];  gweight = gz^T x [N][K];  gbias = sum gz [N]
- * of bdtype; each nullable (x only serves gweight, weight only gx).  gz is rounded to `dtype` for the two products, gbias is summed
- * before that.
+ * of bdtype; each nullable (x only serves gweight, weight only gx).  gz enters the two products of 16-bit tensors as the sum of two numbers
+ * of `dtype` where the activation gives it more bits than gy has (SILU, GELU), so that gx and gweight are rounded once; gbias is summed
+ * from gz in 32 bits.
  * ws: 16-byte aligned scratch of sed_linear_*_ws_bytes bytes (0: none).  M, N, K >= 1; M < 2^31 - 256; N, K <= 2^21; x, W and y
  * below 2^38 elements.  Results do not overlap operands.  The tensors need no more than their element's alignment; lines of a multiple
  * of 16 bytes at 16-byte addresses are read in place, others are copied into ws first (not in the forward product of up to 64 rows

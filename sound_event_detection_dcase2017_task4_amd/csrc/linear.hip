@@ -125,6 +125,20 @@ template <typename T, int V, int ACT> __device__ __forceinline__ void finish(con
     }
 }
 
+// One number as the sum of two of a 16-bit type: what is lost is 2^-18 of it in bfloat16, 2^-24 of it or 2^-36 in float16, which holds half of it
+// and the small part times 2^11.  An infinity or NaN is in the large part alone.
+template <typename T> struct Split;
+template <> struct Split<__bf16> { static constexpr float UNIT = 1.f, LOW = 1.f; };
+template <> struct Split<_Float16> { static constexpr float UNIT = 0.5f, LOW = 0x1p-11f; };
+template <typename T> __device__ __forceinline__ void split(float f, T& large, T& small) {
+    f *= Split<T>::UNIT;
+    large = (T)f;
+    const float rest = f - (float)large;
+    small = rest - rest == 0.f ? (T)(rest * (1.f / Split<T>::LOW)) : (T)0.f;
+}
+// SiLU and GELU beside 16-bit tensors: their gz has more bits than the tensors
+template <typename T> bool in_parts(int act) { return sizeof(T) == 2 && (act == SED_ACT_SILU || act == SED_ACT_GELU); }
+
 // ---- 16 bytes of k of every row: one instruction in 16 bits, four in 32 (they take the k of a lane in any order, as long as P and Q agree)
 template <typename T> struct Frag;
 template <> struct Frag<_Float16> { typedef half8 type; };
@@ -151,15 +165,26 @@ __device__ __forceinline__ floatx16 mma(floatx4 p, floatx4 q, floatx16 c) {
 // A step takes 128 bytes of k: 64 elements in 16 bits, 32 in 32.  One operand's tile of R rows is R * 128 bytes.
 //   k contiguous: [R][128 bytes];  rows contiguous: [k][R elements];  16-byte piece c of a line lies at place c ^ swizzle(line), so that
 //   the lanes that are served together lie in different banks.
+// The backward products of 16-bit tensors behind a SiLU or GELU take gz as the sum of two numbers of the tensors' type, the rounding of gz and
+// what it leaves: gx and gW then carry their own rounding only (gz rounded once put as much again into them, and in float16 lost what is
+// below 6e-8).  k runs over the small parts first and over the large ones behind them, 0 .. K and half .. half + K, half the next
+// multiple of the step.  float16 holds gz / 2, which cannot overflow, and the small part times 2^11, which does not underflow: the sums are
+// multiplied by `low` between the parts and by `scale` at the end, powers of two (the float16 kernels of edge 256 spill there, outside the
+// loop).  It doubles the two products: forward and backward of 32000 x 2048 x 2048 bf16 take 1302 us, for 848 with gz and z in 16
+// bits, of 4000 x 512 x 2048 125 for 116; the error against 64 bits is 1.7e-3 for 2.4e-3, that of the output's rounding.
 struct Operand {
     const void* base;
     long ld;                                       // elements from one line to the next
     int rows;                                      // rows (m or n)
+    long part;                                     // elements from the small parts to the large ones; 0: the same for both
 };
+constexpr long ONE_PART = 1L << 62;                // a `half` that k does not reach
 struct GemmP {
     Operand p, q;
     int M, N;
     long K;
+    long half, end;                                // first k of the second part, end of the last one
+    float low, scale;
     long kslice;                                   // k of one slice, a multiple of the step
     int tm, tn;                                    // tiles
     float* part;                                   // [slices][M][ldp] where the product is cut along k
@@ -188,10 +213,15 @@ template <typename T, int R, bool ROWS, int THREADS, bool RUNS> struct Stage {
         }
     }
     // where the step that begins at k lies, and how much of it: what is behind K lies outside and comes as zeros -- all of a step
-    // behind the end, the lines behind K, or, where the last step ends inside the lines, the pieces that are taken out of `off` for good
-    __device__ __forceinline__ static uint4v descriptor(const Operand& o, int row0, long k, long K, unsigned (&off)[PER]) {
-        const unsigned long at = reinterpret_cast<unsigned long>(reinterpret_cast<const T*>(o.base) + (ROWS ? k * o.ld + row0 : row0 * o.ld + k));
-        const int left = (int)max(0l, min(K - k, (long)STEP));
+    // behind `stop`, the lines behind K, or, where the last step of a part ends inside the lines, the pieces that are taken out of `off`
+    // until the next part begins
+    template <bool PARTS> __device__ __forceinline__ static uint4v descriptor(const Operand& o, int row0, long k, long stop, long K, long half, unsigned (&off)[PER]) {
+        const bool second = PARTS && k >= half;
+        const long in = second ? k - half : k;
+        const T* const base = reinterpret_cast<const T*>(o.base) + (second ? o.part : 0);
+        const unsigned long at = reinterpret_cast<unsigned long>(base + (ROWS ? in * o.ld + row0 : row0 * o.ld + in));
+        const int left = k < stop ? (int)min(K - in, (long)STEP) : 0;
+        if (PARTS && !ROWS && k == half) offsets(o, row0, off);
         if (!ROWS && left > 0 && left < STEP)
 #pragma unroll
             for (int i = 0; i < PER; ++i) off[i] = piece_of(0) * E < left ? off[i] : OUTSIDE;
@@ -262,7 +292,8 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
     // tiles in groups of eight rows of tiles: the 32 that an XCD works on share 8 + 4 operand tiles, not 32 + 1
     const int group = tile / (8 * a.tn), gm = min(8, a.tm - 8 * group), in = tile - group * 8 * a.tn;
     const int m0 = (8 * group + in % gm) * BM, n0 = in / gm * BN;
-    const long k0 = CUT ? slice * a.kslice : 0, k1 = CUT ? min(a.K, k0 + a.kslice) : a.K;
+    constexpr bool PARTS = PROWS && sizeof(T) == 2;          // the backward products
+    const long end = PARTS ? a.end : a.K, k0 = CUT ? slice * a.kslice : 0, k1 = CUT ? min(end, k0 + a.kslice) : end;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
     unsigned poff[SP::PER], qoff[SQ::PER];
@@ -300,7 +331,8 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
     };
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const uint4v dp = SP::descriptor(a.p, n0, k0 + t * SP::STEP, k1, poff), dq = SQ::descriptor(a.q, m0, k0 + t * SP::STEP, k1, qoff);
+        const uint4v dp = SP::template descriptor<PARTS>(a.p, n0, k0 + t * SP::STEP, k1, a.K, a.half, poff);
+        const uint4v dq = SQ::template descriptor<PARTS>(a.q, m0, k0 + t * SP::STEP, k1, a.K, a.half, qoff);
 #pragma unroll
         for (int o = 0; o < SP::PER; ++o) ask_p(dp, 2 * t, o);
 #pragma unroll
@@ -311,8 +343,9 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
     for (int o = 0; o < FRAGS; ++o) read(0, 1, 0, 0, o);
     int ps = 0;                                    // P(t)'s slot; the next ones follow around the ring
     auto ring = [&](int i) { return ps + i < 5 ? ps + i : ps + i - 5; };
-    for (long k = k0; k < k1; k += SP::STEP) {
-        const uint4v dp = SP::descriptor(a.p, n0, k + 2 * SP::STEP, k1, poff), dq = SQ::descriptor(a.q, m0, k + 2 * SP::STEP, k1, qoff);
+    auto step = [&](long k) {
+        const uint4v dp = SP::template descriptor<PARTS>(a.p, n0, k + 2 * SP::STEP, k1, a.K, a.half, poff);
+        const uint4v dq = SQ::template descriptor<PARTS>(a.q, m0, k + 2 * SP::STEP, k1, a.K, a.half, qoff);
         const int qs = ring(1), pn = ring(2), qn = ring(3), spare = ring(4);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
@@ -332,6 +365,19 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
             }
         }
         ps = pn;
+    };
+    if constexpr (PARTS) {
+        long k = k0;
+        do {
+            const long stop = min(k1, k < a.half ? a.half : k1);
+            for (; k < stop; k += SP::STEP) step(k);
+            if constexpr (Split<T>::LOW != 1.f)
+                if (a.low != 1.f && k <= a.half)
+#pragma unroll
+                    for (int f = 0; f < MFMAS; ++f) acc[f / NI][f % NI] *= a.low;
+        } while (k < k1);
+    } else {
+        for (long k = k0; k < k1; k += SP::STEP) step(k);
     }
     arrived<0>();                                  // no request is in flight when the workgroup ends
     if (!EARLY) fetch();
@@ -357,7 +403,7 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
             for (int h = 0; h < V / 4; ++h) {
                 const floatx4 q = *reinterpret_cast<const floatx4*>(mine + (PASS * it + lane / LINE) * PITCH + place(lane % LINE * (V / 4) + h));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * h + j] = q[j];
+                for (int j = 0; j < 4; ++j) v[4 * h + j] = PARTS ? q[j] * a.scale : q[j];
             }
             const int m = row(i, it);
             if (m >= a.M || n >= a.N) continue;
@@ -529,7 +575,8 @@ template <typename T> __device__ __forceinline__ void pad_lines(const PadP& p) {
 }
 template <typename T> __global__ __launch_bounds__(256) void pad_kernel(PadP p) { pad_lines<T>(p); }
 
-// gz [M][ld] = gy act'(z) (null: only the sums) and per chunk of rows the column sums of gz in 32 bits, before it is rounded.
+// gz [M][ld] = gy act'(z) (null: only the sums), its small parts [M][ld] in front of it where it is in parts, and per chunk of rows the column
+// sums of gz in 32 bits, before it is rounded.
 // A thread owns E columns (16 bytes) of every RT-th row of a chunk.  The first pad.blocks workgroups copy the operands that need it.
 struct GradP {
     const void* gy;
@@ -552,6 +599,7 @@ template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) voi
     const long chunk = bid / p.tiles, s0 = chunk * p.rows, s1 = min(p.M, s0 + p.rows);
     const T* const gy = reinterpret_cast<const T*>(p.gy) + c;
     const Z* const kept = reinterpret_cast<const Z*>(p.z) + c;
+    constexpr bool PARTS = sizeof(T) == 2 && (ACT == SED_ACT_SILU || ACT == SED_ACT_GELU);
     float sum[E] = {};
     if (r < p.RT && c < p.ld)
         for (long s = s0 + r; s < s1; s += U * p.RT) {
@@ -571,6 +619,7 @@ template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) voi
             for (int u = 0; u < U; ++u) {
                 const long at = s + u * p.RT;
                 if (at >= s1) continue;
+                T small[E];
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     float f = (float)g[u][j];
@@ -578,9 +627,12 @@ template <typename T, int ACT, bool WHOLE> __global__ __launch_bounds__(256) voi
                     else if (ACT) f *= sed_act_grad<ACT>((float)z[u][j]);
                     if (!WHOLE && c + j >= p.N) f = 0.f;   // z is not written there
                     sum[j] += f;
-                    g[u][j] = (T)f;
+                    if constexpr (PARTS) split<T>(f, g[u][j], small[j]);
+                    else g[u][j] = (T)f;
                 }
-                if (p.gz) __builtin_memcpy(reinterpret_cast<T*>(p.gz) + at * p.ld + c, g[u], 16);
+                if (!p.gz) continue;
+                if constexpr (PARTS) __builtin_memcpy(reinterpret_cast<T*>(p.gz) + at * p.ld + c, small, 16);
+                __builtin_memcpy(reinterpret_cast<T*>(p.gz) + ((PARTS ? p.M : 0) + at) * p.ld + c, g[u], 16);
             }
         }
     if (!p.sums && !p.gb) return;
@@ -614,6 +666,17 @@ long padded(long n, int esize) { return (n + 16 / esize - 1) / (16 / esize) * (1
 long up256(long bytes) { return (bytes + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool needs_pad(const void* p, long ld, int esize) { return !aligned16(p) || ld % (16 / esize); }
+
+long whole_steps(long k, int esize) { const long step = 128 / esize; return (k + step - 1) / step * step; }
+// k of a product whose Q is in two parts, or in one
+template <typename T> void set_k(GemmP& a, long K, bool parts) {
+    a.K = K;
+    a.half = parts ? whole_steps(K, sizeof(T)) : ONE_PART;
+    a.end = parts ? 2 * a.half : K;
+    a.low = a.scale = 1.f;
+    if constexpr (sizeof(T) == 2)
+        if (parts) { a.low = Split<T>::LOW; a.scale = 1.f / Split<T>::UNIT; }
+}
 
 // How a product is cut: tile edge, and slices along k that a second pass adds.  The cut with the least time by what was measured on an
 // MI355X: a step of 128 bytes of k takes a tile of 64, 128 or 256 the microseconds below when 1, 2, .. of them share a CU (LDS holds 4, 2
@@ -759,9 +822,10 @@ int linear_fwd(const void* x, const void* w, const void* bias, const void* res, 
     const long ld = padded(K, sizeof(T));
     launch_pad<T>(pad_of<T>(x, M, needs_pad(x, K, sizeof(T)), w, N, needs_pad(w, K, sizeof(T)), K, ws), stream);
     GemmP a{};
-    a.M = (int)M; a.N = (int)N; a.K = ld; a.e = e;
-    a.q = {x, ld, (int)M};
-    a.p = {w, ld, (int)N};
+    a.M = (int)M; a.N = (int)N; a.e = e;
+    set_k<T>(a, ld, false);
+    a.q = {x, ld, (int)M, 0};
+    a.p = {w, ld, (int)N, 0};
     launch_gemm<T, false, false>(a, plan_of(M, N, ld, sizeof(T)), reinterpret_cast<float*>(ws), stream);
     SED_LAUNCH_CHECK();
     return 0;
@@ -782,9 +846,10 @@ BwdNeeds bwd_needs(const void* x, const void* w, const void* gy, int esize, long
 long bwd_ws(const void* x, const void* w, const void* gy, int esize, long M, long N, long K, int act, bool gx, bool gw, bool gb) {
     const BwdNeeds d = bwd_needs(x, w, gy, esize, N, K, act, gx, gw);
     const long ldn = padded(N, esize), ldk = padded(K, esize);
-    long b = (d.gz ? up256(M * ldn * esize) : 0) + (d.px ? up256(M * ldk * esize) : 0) + (d.pw ? up256(N * ldk * esize) : 0);
+    const bool parts = esize == 2 && in_parts<_Float16>(act);
+    long b = (d.gz ? up256((parts ? 2 : 1) * M * ldn * esize) : 0) + (d.px ? up256(M * ldk * esize) : 0) + (d.pw ? up256(N * ldk * esize) : 0);
     if (gb) b += up256(grad_cut(M, ldn, esize).chunks * ldn * 4);
-    const Plan px = gx ? plan_of(M, K, ldn, esize) : Plan{}, pw = gw ? plan_of(N, K, M, esize) : Plan{};
+    const Plan px = gx ? plan_of(M, K, parts ? 2 * whole_steps(N, esize) : ldn, esize) : Plan{}, pw = gw ? plan_of(N, K, parts ? 2 * whole_steps(M, esize) : M, esize) : Plan{};
     if (gx && gw && pairs(pw, px)) return b + pw.part_bytes + px.part_bytes;
     return b + (px.part_bytes > pw.part_bytes ? px.part_bytes : pw.part_bytes);
 }
@@ -796,10 +861,11 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
     const BwdNeeds d = bwd_needs(x, w, gy, es, N, K, act, gx != nullptr, gw != nullptr);
     const long ldn = padded(N, es), ldk = padded(K, es);
     const GradCut c = grad_cut(M, ldn, es);
+    const bool parts = in_parts<T>(act);
     T* gz = nullptr;
     if (d.gz) {
         gz = reinterpret_cast<T*>(ws);
-        ws += up256(M * ldn * es);
+        ws += up256((parts ? 2 : 1) * M * ldn * es);
     }
     float* sums = nullptr;
     if (gb) {
@@ -821,18 +887,19 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
     if (gx) {
         x_.M = (int)M; x_.N = (int)K;
         x_.e.y = gx; x_.e.wide = wide && aligned16(gx);
-        x_.q = {dz, ldn, (int)M};
-        x_.p = {w, ldk, (int)ldk};
+        x_.q = {dz, ldn, (int)M, M * ldn};
+        x_.p = {w, ldk, (int)ldk, 0};
         // gz has zeros behind its N-th column, W has no line there: k ends at N for W's lines and at ldn for gz's pieces
-        x_.K = N;
-        px = plan_of(M, K, ldn, es);
+        set_k<T>(x_, N, parts);
+        px = plan_of(M, K, parts ? x_.end : ldn, es);
     }
     if (gw) {
-        w_.M = (int)N; w_.N = (int)K; w_.K = M;
+        w_.M = (int)N; w_.N = (int)K;
+        set_k<T>(w_, M, parts);
         w_.e.y = gw; w_.e.wide = wide && aligned16(gw);
-        w_.q = {dz, ldn, (int)ldn};
-        w_.p = {x, ldk, (int)ldk};
-        pw = plan_of(N, K, M, es);
+        w_.q = {dz, ldn, (int)ldn, M * ldn};
+        w_.p = {x, ldk, (int)ldk, 0};
+        pw = plan_of(N, K, w_.end, es);
     }
     float* const part = reinterpret_cast<float*>(ws);
     ColumnsP columns{sums, c.chunks, (int)ldn, (int)N, gb, btype, gb && c.chunks > 1 ? sed_cdiv(N, 16) : 0};

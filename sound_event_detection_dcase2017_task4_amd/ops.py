@@ -2124,8 +2124,9 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     """y = act(x W^T + b) + residual in one product: x (..., K), weight (N, K), bias (N,), residual and y (..., N).
 
     x, weight and residual: float32, float16 or bfloat16, all of one type (any strides; non-contiguous ones are copied); bias: that
-    type or float32.  activation: 'none', 'relu', 'silu', 'gelu' (z Phi(z)).  Sums are held in 32 bits and y is rounded once; the
-    backward pass rounds gz = gy act'(z) to x's type for its two products.  A few rows are one pass over W (single frames of a
+    type or float32.  activation: 'none', 'relu', 'silu', 'gelu' (z Phi(z)).  Sums are held in 32 bits, y and
+    the gradients are rounded once: z is kept in 32 bits for the backward pass, and gz = gy act'(z) enters its two products with twice the
+    bits of x's type (SiLU and GELU beside 16-bit tensors; 4 M N bytes each in memory).  A few rows are one pass over W (single frames of a
     stream); an x without rows gives a y without rows."""
     act = _act_code(activation)
     dtype, device = x.dtype, x.device

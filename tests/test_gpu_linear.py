@@ -322,3 +322,57 @@ def test_bias_gradient_of_16_bit_tensors_has_the_bits_of_its_own_type(m, dtype, 
     zerr = _sum_err(96) * (xd.abs() @ wd.abs().t() + b.detach().double().abs()) + 4 * H
     tol = (gd.abs() * (1.2 * zerr + 16 * H)).sum(0) + _sum_err(m) * (gd * da).abs().sum(0)
     assert got.dtype == torch.float32 and ((got.double() - (gd * da).sum(0)).abs() <= tol).all()
+
+
+def _gradients(x, w, gy, act):
+    """gx and gw of linear_act, those of the formula in 64 bits, and gz."""
+    leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+    got = torch.autograd.grad(ops.linear_act(*leaves, activation=act), leaves, gy)
+    z = (x.double() @ w.double().t()).requires_grad_(True)
+    gz = gy.double() * torch.autograd.grad(ACTS[act](z).sum(), z)[0]
+    return got, (gz @ w.double(), gz.t() @ x.double()), gz
+
+
+PARTS = [(70, 40, 24), (64, 128, 64), (129, 72, 257), (300, 136, 65), (1001, 520, 127), (4000, 512, 200), (20000, 64, 48), (65, 9, 7), (3, 200, 33)]
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n", PARTS)
+def test_gradients_of_16_bit_tensors_carry_one_rounding(m, k, n, dtype, act):
+    """gz enters the products as the sum of two numbers of the type: off by e^2 of itself (float16: and 2^-36), e half a step of the type.  What
+    is left beside the sums' roundings is the gradient's own."""
+    x, w, _, _, gy = _inputs(m, k, n, dtype, dtype, 37, residual=False)
+    e, tiny = HALF[dtype], TINY[dtype]
+    for scale in (1.0, 2.0 ** -18):                         # the second one: a large share of the gradient is below float16's normal numbers
+        g = (gy.float() * scale).to(dtype)
+        got, want, gz = _gradients(x, w, g, act)
+        zerr = _sum_err(k) * (x.double().abs() @ w.double().abs().t()) + 4 * H
+        gzerr = g.double().abs() * (1.2 * zerr + 16 * H) + e * e * gz.abs() + (2.0 ** -36 if dtype == torch.float16 else 0)
+        for a, b, err, terms in ((got[0], want[0], gzerr @ w.double().abs(), _sum_err(2 * n) * (gz.abs() @ w.double().abs())),
+                                 (got[1], want[1], gzerr.t() @ x.double().abs(), _sum_err(2 * m) * (gz.abs().t() @ x.double().abs()))):
+            assert ((a.double() - b).abs() <= err + terms + e * 1.01 * b.abs() + tiny).all()
+            # and in the norm: within a twentieth of what rounding the right gradient leaves
+            assert (a.double() - b).norm() <= 1.05 * (b.to(dtype).double() - b).norm()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_at_the_ends_of_the_range(dtype):
+    x, w, _, _, gy = _inputs(150, 64, 96, dtype, dtype, 41, residual=False)
+    gy = torch.zeros_like(gy)
+    x[5], w[7] = 2.0 ** -6, 1.5                             # z = 1.5, where GELU's derivative is 1.13: gz is beyond float16's largest number
+    gy[5, 7] = 60000.0
+    got, want, gz = _gradients(x, w, gy, "gelu")
+    assert float(gz[5, 7]) > 65504
+    assert torch.equal(got[1], want[1].to(dtype)) and torch.equal(got[0][:5], torch.zeros_like(got[0][:5]))
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        x, w, _, _, gy = _inputs(150, 64, 96, dtype, dtype, 43, residual=False)
+        clean = _gradients(x, w, gy, "silu")[0]
+        gy[5, 7] = bad
+        got, want, _ = _gradients(x, w, gy, "silu")
+        for a, b, c, at in ((got[0], want[0], clean[0], 5), (got[1], want[1], clean[1], 7)):
+            keep = torch.arange(len(a), device="cuda") != at
+            assert torch.equal(a[keep], c[keep]) and not torch.isfinite(a[at]).any()
+            assert torch.equal(a[at].double().nan_to_num(1.0, 2.0, 3.0), b[at].nan_to_num(1.0, 2.0, 3.0))
