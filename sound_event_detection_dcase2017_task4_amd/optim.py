@@ -352,8 +352,9 @@ class FusedAdamW(object):
     256 elements (`offsets`).  In a data-parallel job reduce the gradients first and pass `step(grad_scale=1 / world_size)`.  The step
     number is an argument of the launch, so step() refuses to be captured into a graph: it belongs behind the graph.
 
-    Found-non-finite guard: as FusedAdamAmsgrad, the kernel refuses a step behind a split-f16 kernel that met a NaN / inf operand;
-    the gradients themselves are not scanned (a NaN gradient makes a NaN parameter, as in torch)."""
+    Found-non-finite guard: the kernel refuses a step behind a split-f16 kernel that reported a NaN / inf operand, and the BatchNorm
+    statistics of the forward passes since the last step are taken back, as FusedAdamAmsgrad does.  Unlike there the gradients themselves
+    are not scanned: a NaN gradient that no kernel reported makes a NaN parameter, as in torch."""
 
     DEFAULTS = ("lr", "betas", "eps", "weight_decay")
 
@@ -502,6 +503,7 @@ class FusedAdamW(object):
             ops.adamw_(self._dev_rows, self._chunks, len(self._chunks), self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
                        self.exp_avg_sq_scale, self.master, self.state_bits, hyper, self.step_count, grad_scale, skipped=self._skipped)
         del grads
+        ops.restore_bn_if_refused()        # a step refused after its forward pass takes the BatchNorm statistics back too
 
     def moments(self):
         """(exp_avg, exp_avg_sq) as flat float32 buffers: the state itself with 32 bits, the values that the codes stand for with 8."""

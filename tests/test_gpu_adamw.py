@@ -377,3 +377,77 @@ def test_c_entries_refuse_bad_arguments():
         assert call(**bad) == -22, bad
     assert h.sed_adamw_moments(1, 1, 1, 1, 255, 1, 1, None) == -22 and h.sed_adamw_moments(1, 1, 1, 1, 0, 1, 1, None) == -22
     assert h.sed_adamw_moments(1, None, 1, 1, 256, 1, 1, None) == -22 and h.sed_adamw_chunk() % 256 == 0
+
+
+def _model(seed=5):
+    from oracle import model as om
+    from sound_event_detection_dcase2017_task4_amd.pytorch import models
+    m = models.Cnn_9layers_FrameAvg(32000, 1024, 320, 64, 50, 14000, 17)
+    m.load_state_dict(om.recipe_state("Cnn_9layers_FrameAvg", seed))
+    rs = np.random.RandomState(seed)
+    x, y = torch.from_numpy((rs.randn(4, 32000) * 0.1).astype(np.float32)).cuda(), torch.from_numpy((rs.rand(4, 17) < 0.2).astype(np.float32)).cuda()
+    return m.cuda().train(), x, y
+
+
+def _report():
+    """As a split-f16 kernel that met a NaN operand leaves the two words."""
+    ops._err_dev()[0] = 1
+    torch.cuda.synchronize()
+    ops._err_flag()[1] = 1
+
+
+def _statistics(m):
+    return {k: v.clone() for k, v in m.named_buffers() if "running" in k}
+
+
+@gpu
+@pytest.mark.parametrize("passes", [1, 2])
+def test_refused_step_takes_the_batchnorm_statistics_back(passes):
+    """Clean forward passes install their statistics; behind them a kernel reports an operand that is not finite, and the step is refused."""
+    from sound_event_detection_dcase2017_task4_amd.pytorch.losses import clip_bce
+    m, x, y = _model()
+    opt = optim.FusedAdamW(m, lr=1e-3)
+    ops.check_device_errors(synchronize=True)
+
+    def step(reported=False):
+        opt.zero_grad()
+        for k in range(passes):
+            clip_bce(m(x * (1 + k)), {"target": y}).backward()
+        if reported:
+            _report()
+        opt.step()
+        ops.check_device_errors(synchronize=True)
+    for _ in range(2):
+        step()
+        assert ops._BN_LAST is None                               # nothing of a settled step is kept
+    before, stats = [p.detach().clone() for p in opt.params], _statistics(m)
+    with pytest.raises(ops.NonFiniteOperand):
+        step(reported=True)
+    assert opt.step_count == 2 and opt.skipped_steps == 1
+    assert all(torch.equal(p.detach(), b) for p, b in zip(opt.params, before))
+    assert all(torch.equal(v, stats[k]) for k, v in _statistics(m).items())
+    ops.rollback_bn_counters(m, passes)
+    step()
+    assert opt.step_count == 3 and not torch.equal(m.bn0.running_mean, stats["bn0.running_mean"])
+
+
+@gpu
+def test_a_refused_step_of_the_other_optimiser_leaves_the_statistics_of_settled_steps():
+    from sound_event_detection_dcase2017_task4_amd.pytorch.losses import clip_bce
+    m, x, y = _model()
+    opt = optim.FusedAdamW(m, lr=1e-3)
+    ops.check_device_errors(synchronize=True)
+    for _ in range(2):
+        opt.zero_grad()
+        clip_bce(m(x), {"target": y}).backward()
+        opt.step()
+    stats = _statistics(m)
+    other, x2, y2 = _model(6)
+    flat = optim.FusedAdamAmsgrad(other, lr=1e-3)
+    flat.zero_grad()
+    clip_bce(other(x2), {"target": y2}).backward()
+    _report()
+    with pytest.raises(ops.NonFiniteOperand):
+        flat.step()
+        ops.check_device_errors(synchronize=True)
+    assert all(torch.equal(v, stats[k]) for k, v in _statistics(m).items())
