@@ -90,7 +90,9 @@ class GraphedTrainStep(object):
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         prev, buckets.deferred = getattr(buckets, "deferred", False), True   # no collective inside the graph
-        bn_before = ops._BN_LAST               # BatchNorm groups tracked before the capture (normally none: a step has just ended)
+        # BatchNorm groups tracked before the capture (normally none: a step has just ended) are put aside: the list is capped, so
+        # the captured ones could not be told apart behind a full one
+        bn_before, ops._BN_LAST = ops._BN_LAST, None
         try:
             # thread_local: only THIS thread's actions can invalidate the recording.  Other threads of the process make HIP calls
             # of their own all the time -- the NCCL watchdog polls its events, the input pipeline's producer thread synchronises
@@ -110,8 +112,7 @@ class GraphedTrainStep(object):
             # the forward pass that was only RECORDED tracked its BatchNorm entries (ops._BN_LAST) although nothing ran: their
             # `cand` tensors hold no statistics yet.  They belong to the replays (below), never to the eager bookkeeping -- a
             # step refused later must not 'restore' running statistics from them
-            captured_bn = (ops._BN_LAST or [])[len(bn_before or []):]
-            ops._BN_LAST = bn_before
+            captured_bn, ops._BN_LAST = ops._BN_LAST, bn_before
         if ops.pending_sink_indices():
             ops.drop_pending_wgrads()
             raise GraphCaptureError("GraphedTrainStep: side-stream weight gradients were left un-joined by the captured backward pass")
@@ -122,7 +123,7 @@ class GraphedTrainStep(object):
         # nothing and ZERO the slice the graph has just filled
         self._written = set(buckets.written)
         # ... and likewise the BatchNorm entries of the captured forward pass (ops.restore_bn_if_refused() after every replay)
-        self._bn_last = captured_bn or None
+        self._bn_last = captured_bn
 
     def _capture_together(self):
         """Capture, and agree on the outcome with the other ranks: a rank that fell back to the eager loop alone would fire its

@@ -91,3 +91,35 @@ def test_non_finite_batch_is_refused_under_the_graph():
     loss = step(*batches[4])                     # the next clean batch trains again
     assert np.isfinite(float(loss))
     assert opt.step_count == 5 and not torch.equal(opt.flat, before)
+
+
+def test_captured_statistics_are_found_behind_a_full_list_of_tracked_passes():
+    """Train-mode forward passes without an optimiser step fill the (capped) list of tracked BatchNorm groups; the groups of the
+    pass that is captured behind them are kept all the same, and a refused replay takes its statistics back."""
+    from sound_event_detection_dcase2017_task4_amd import ops
+    from sound_event_detection_dcase2017_task4_amd.graph import GraphedTrainStep
+    from sound_event_detection_dcase2017_task4_amd.optim import FusedAdamAmsgrad
+    from sound_event_detection_dcase2017_task4_amd.pytorch.losses import clip_bce
+    m = _build("Cnn_9layers_FrameAvg")
+    step = GraphedTrainStep(m, FusedAdamAmsgrad(m, lr=1e-3), clip_bce, mixup=True, eager_steps=1)
+    batches = _batches(4)
+    step(*batches[0])
+    ops._BN_LAST = [[] for _ in range(ops._BN_TRACK_MAX)]
+    step(*batches[1])                            # captured and replayed
+    assert step.replays == 1 and step._bn_last is not None and len(step._bn_last) == 1 and len(step._bn_last[0]) > 0
+    step(*batches[2])
+    ops.check_device_errors(synchronize=True)
+    stats = {k: v.clone() for k, v in m.named_buffers() if "running" in k}
+    poison = step.opt.flat_grad                  # a NaN that arises behind the forward pass
+    replay, step.graph = step.graph, None
+
+    class Poisoned:
+        @staticmethod
+        def replay():
+            replay.replay()
+            poison[0] = float("nan")
+    step.graph = Poisoned
+    with pytest.raises(ops.NonFiniteOperand):
+        step(*batches[3])
+        ops.check_device_errors(synchronize=True)
+    assert all(torch.equal(v, stats[k]) for k, v in m.named_buffers() if "running" in k)
