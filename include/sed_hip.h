@@ -530,11 +530,15 @@ int sed_linear_bwd(const void* x, const void* weight, const void* gy, const void
  * hyper (HOST): per group five doubles {lr, beta1, beta2, eps, weight_decay}, at most 16 groups; grad_scale multiplies the gradient.
  * master: where a 16-bit parameter is not the rounding of its copy, the step goes on from the parameter.
  * skip_flag (nullable, device): non-zero leaves everything untouched and adds 1 to *skipped, as in sed_adam_amsgrad.
+ * sed_guard_collect, in front of it: a *rank_flag (nullable; see sed_guard_publish) other than 0 raises *skip_flag and the nullable
+ * host-mapped *err_host; the nullable host-mapped *status_host receives *skipped, and one more where *skip_flag is raised: the refused
+ * steps up to the one that follows.
  * sed_adamw_moments: the values that 8-bit moments stand for, n elements (a multiple of 256). */
 int sed_adamw_chunk(void);
 int sed_adamw(const long* rows, const int* chunks, long nchunks, void* m, void* v, float* m_scale, float* v_scale, float* master,
               int state_bits, const double* hyper, int ngroups, int step, float grad_scale, const int* skip_flag, int* skipped,
               sed_stream_t stream);
+int sed_guard_collect(const float* rank_flag, int* skip_flag, const int* skipped, int* err_host, int* status_host, sed_stream_t stream);
 int sed_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, long n, float* out_m, float* out_v,
                       sed_stream_t stream);
 

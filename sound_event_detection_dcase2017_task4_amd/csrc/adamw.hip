@@ -229,6 +229,17 @@ template <bool EIGHT> __global__ __launch_bounds__(256, 5) void adamw_kernel(Ada
     else adamw_chunk<__bf16, EIGHT>(a, row, c0);
 }
 
+// sed_guard_collect: one thread in front of a step
+__global__ void guard_collect_kernel(const float* rank_flag, int* skip_flag, const int* skipped, int* err_host, int* status_host) {
+    int bad = __hip_atomic_load(skip_flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+    if (rank_flag && !(rank_flag[0] == 0.f)) {
+        bad = 1;
+        __hip_atomic_store(skip_flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (err_host) __hip_atomic_store(err_host, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    if (status_host) __hip_atomic_store(status_host, __hip_atomic_load(skipped, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const char4* m, const float* ms, const uchar4* v, const float* vs, long n4,
                                                             float4* om, float4* ov) {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long)gridDim.x * 256) {
@@ -264,6 +275,13 @@ SED_API int sed_adamw(const long* rows, const int* chunks, long nchunks, void* m
     }
     if (state_bits == 8) hipLaunchKernelGGL(adamw_kernel<true>, dim3((unsigned)nchunks), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL(adamw_kernel<false>, dim3((unsigned)nchunks), dim3(256), 0, stream, a);
+    SED_LAUNCH_CHECK();
+    return 0;
+}
+
+SED_API int sed_guard_collect(const float* rank_flag, int* skip_flag, const int* skipped, int* err_host, int* status_host, sed_stream_t stream) {
+    if (!skip_flag || (status_host && !skipped)) return SED_EINVAL;
+    hipLaunchKernelGGL(guard_collect_kernel, dim3(1), dim3(1), 0, stream, rank_flag, skip_flag, skipped, err_host, status_host);
     SED_LAUNCH_CHECK();
     return 0;
 }

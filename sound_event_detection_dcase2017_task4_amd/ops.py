@@ -1935,6 +1935,13 @@ def guard_publish(flag_out):
     _call("sed_guard_publish", _sf16_err_dev_ptr(flag_out.device), _ptr(flag_out), _stream())
 
 
+def guard_collect(rank_flag, skipped, status_ptr):
+    """In front of adamw_: the ranks' summed flag (None: there are no others) raises this rank's found-non-finite words, and the refused
+    steps, the one that follows counted, go to the host-mapped status_ptr (None: nowhere); see include/sed_hip.h: sed_guard_collect."""
+    _call("sed_guard_collect", _ptr(rank_flag), _sf16_err_dev_ptr(skipped.device), _ptr(skipped), _sf16_err_ptr(),
+          ctypes.c_void_p(status_ptr) if status_ptr else None, _stream())
+
+
 # ------------------------------------------------------------------------------------------------------------
 # operators on float32 / float16 / bfloat16 tensors
 

@@ -114,7 +114,60 @@ def torch_adam_state_to_flat(sd, numels, trainable):
     return (steps.pop() if steps else 0), out[0], out[1], out[2], hyper
 
 
-class FusedAdamAmsgrad(object):
+class _LaggedPoll(object):
+    """The found-non-finite guard of an optimiser as the host sees it, `poll_lag` steps behind the newest one (see
+    FusedAdamAmsgrad).  The optimiser has `step_count`, `skipped_steps` and the device word `_skipped`."""
+
+    def _init_poll(self, poll_lag):
+        if poll_lag is not None and not (0 <= int(poll_lag) < POLL_RING - 1):
+            raise ValueError("poll_lag must be None or 0 .. %d" % (POLL_RING - 2))
+        self.poll_lag = poll_lag
+        self._status = torch.zeros((POLL_RING,), dtype=torch.int32).pin_memory()   # cumulative refused steps, written by the step's kernels
+        self._inflight = collections.deque()                                        # (issue number, event behind that step's kernels)
+        self._issued = 0
+
+    def _status_ptr(self):
+        """Where the step that is about to be issued leaves its status word."""
+        return self._status.data_ptr() + 4 * (self._issued % POLL_RING)
+
+    def _settle(self, lagged):
+        """Behind a step's launches: look at the steps that are due, or at whatever the host-mapped flag shows already."""
+        if lagged:
+            ev = torch.cuda.Event()
+            ev.record()
+            self._inflight.append((self._issued, ev))
+            self._issued += 1
+            self.poll(self.poll_lag)
+            ops.check_device_errors(nonfinite=False)       # the other run-time flags (fused GRU give-up)
+        else:
+            ops.check_device_errors()      # NonFiniteOperand: step_count / skipped_steps were already corrected there
+
+    def poll(self, lag=0):
+        """Deterministic poll of the found-non-finite guard: look at every optimiser step that is at least `lag` steps behind
+        the newest one (waiting for its event) and raise ops.NonFiniteOperand if the Adam kernel refused it -- together with
+        every step issued since, which the sticky device flag made it refuse too.  poll(0) drains: call it on ALL ranks
+        before anything that must not see a half-reported state (evaluation, checkpoints, the end of training)."""
+        while self._inflight and (self._issued - 1 - self._inflight[0][0]) >= lag:
+            n, ev = self._inflight.popleft()
+            ev.synchronize()
+            if int(self._status[n % POLL_RING]) > 0:
+                torch.cuda.synchronize()
+                k = int(self._skipped.item())              # == self._issued - n on every rank
+                self._skipped.zero_()
+                ops.clear_nonfinite_flags()
+                self._status.zero_()
+                self._inflight.clear()
+                self.step_count = max(0, self.step_count - k)
+                self.skipped_steps += k
+                raise ops.NonFiniteOperand(
+                    "sound_event_detection_dcase2017_task4_amd: a split-f16 convolution (or a BatchNorm statistic) of optimiser "
+                    "step %d met NaN / inf on some rank; the Adam kernel refused that step and the %d issued since (%d in all) "
+                    "on EVERY rank -- parameters, moments and BatchNorm running statistics are those from before it.  Re-run "
+                    "the last %d batches (the train CLI does so on the fp32 MFMA kernels, ops.USE_SF16 = False)."
+                    % (self.step_count + 1, k - 1, k, k), k)
+
+
+class FusedAdamAmsgrad(_LaggedPoll):
     """poll_lag: how the host learns that the Adam kernel refused a step (found-non-finite guard of the split-f16 path).
     None (default for one process): opportunistically -- ops.check_device_errors() raises at whatever call first sees the
     host-mapped flag.  k >= 0 (default 2 when world_size > 1; the train CLI always uses 2): DETERMINISTICALLY -- step() number
@@ -173,12 +226,7 @@ class FusedAdamAmsgrad(object):
         self._skipped = torch.zeros((1,), dtype=torch.int32, device=dev)    # ... counted here by the kernel itself
         ops._GUARDED.add(self)             # ops.check_device_errors() books them back, whoever happens to poll
         ops.invalidate_weight_caches()     # parameters moved into the flat buffer: operands derived from them are stale
-        self.poll_lag = (2 if world_size > 1 else None) if poll_lag == "auto" else poll_lag
-        if self.poll_lag is not None and not (0 <= int(self.poll_lag) < POLL_RING - 1):
-            raise ValueError("poll_lag must be None or 0 .. %d" % (POLL_RING - 2))
-        self._status = torch.zeros((POLL_RING,), dtype=torch.int32).pin_memory()   # cumulative refused steps, written by the Adam kernel
-        self._inflight = collections.deque()                                        # (issue number, event behind that step's Adam kernel)
-        self._issued = 0
+        self._init_poll((2 if world_size > 1 else None) if poll_lag == "auto" else poll_lag)
 
     def _publish_flag(self):
         """Called by the buckets right before the LAST one goes to the backend: this rank's found-non-finite word -> the flag
@@ -249,42 +297,10 @@ class FusedAdamAmsgrad(object):
         lagged = self.poll_lag is not None and ops.USE_SF16
         ops.adam_amsgrad_(self.flat, self.flat_grad, self.exp_avg, self.exp_avg_sq, self.max_exp_avg_sq, self.step_count,
                           self.lr, self.betas[0], self.betas[1], self.eps, 1.0 / float(self.world_size), skipped=self._skipped,
-                          status_ptr=(self._status.data_ptr() + 4 * (self._issued % POLL_RING)) if lagged else None,
+                          status_ptr=self._status_ptr() if lagged else None,
                           rank_flag=self._grad_store if self.world_size > 1 else None)
         ops.restore_bn_if_refused()        # a step refused after its forward pass takes the BatchNorm statistics back too
-        if lagged:
-            ev = torch.cuda.Event()
-            ev.record()
-            self._inflight.append((self._issued, ev))
-            self._issued += 1
-            self.poll(self.poll_lag)
-            ops.check_device_errors(nonfinite=False)       # the other run-time flags (fused GRU give-up)
-        else:
-            ops.check_device_errors()      # NonFiniteOperand: step_count / skipped_steps were already corrected there
-
-    def poll(self, lag=0):
-        """Deterministic poll of the found-non-finite guard: look at every optimiser step that is at least `lag` steps behind
-        the newest one (waiting for its event) and raise ops.NonFiniteOperand if the Adam kernel refused it -- together with
-        every step issued since, which the sticky device flag made it refuse too.  poll(0) drains: call it on ALL ranks
-        before anything that must not see a half-reported state (evaluation, checkpoints, the end of training)."""
-        while self._inflight and (self._issued - 1 - self._inflight[0][0]) >= lag:
-            n, ev = self._inflight.popleft()
-            ev.synchronize()
-            if int(self._status[n % POLL_RING]) > 0:
-                torch.cuda.synchronize()
-                k = int(self._skipped.item())              # == self._issued - n on every rank
-                self._skipped.zero_()
-                ops.clear_nonfinite_flags()
-                self._status.zero_()
-                self._inflight.clear()
-                self.step_count = max(0, self.step_count - k)
-                self.skipped_steps += k
-                raise ops.NonFiniteOperand(
-                    "sound_event_detection_dcase2017_task4_amd: a split-f16 convolution (or a BatchNorm statistic) of optimiser "
-                    "step %d met NaN / inf on some rank; the Adam kernel refused that step and the %d issued since (%d in all) "
-                    "on EVERY rank -- parameters, moments and BatchNorm running statistics are those from before it.  Re-run "
-                    "the last %d batches (the train CLI does so on the fp32 MFMA kernels, ops.USE_SF16 = False)."
-                    % (self.step_count + 1, k - 1, k, k), k)
+        self._settle(lagged)
 
     def state_dict(self):
         return {"step": self.step_count, "lr": self.lr, "betas": self.betas, "eps": self.eps,
@@ -335,7 +351,7 @@ class FusedAdamAmsgrad(object):
 STATE_BLOCK = 256      # elements that share one scale of an 8-bit moment; every tensor's moments begin at a multiple of it
 
 
-class FusedAdamW(object):
+class FusedAdamW(_LaggedPoll):
     """AdamW (decoupled weight decay) over many separate tensors in ONE launch (sed_adamw), float32 / float16 / bfloat16 ones together.
 
     params: a module, an iterable of tensors, or a list of groups {'params': [...], 'lr' / 'betas' / 'eps' / 'weight_decay': ...} as
@@ -349,8 +365,13 @@ class FusedAdamW(object):
     its copy (its model was loaded, it was clipped or broadcast), the step goes on from the parameter.
 
     `exp_avg`, `exp_avg_sq` (and `exp_avg_scale`, `exp_avg_sq_scale`) are flat buffers in which every tensor begins at a multiple of
-    256 elements (`offsets`).  In a data-parallel job reduce the gradients first and pass `step(grad_scale=1 / world_size)`.  The step
-    number is an argument of the launch, so step() refuses to be captured into a graph: it belongs behind the graph.
+    256 elements (`offsets`).  The step number is an argument of the launch, so step() refuses to be captured into a graph: it
+    belongs behind the graph.
+
+    In a data-parallel job reduce the gradients first and pass `step(grad_scale=1 / world_size)`.  step() is a collective call there:
+    the ranks add up their found-non-finite words, so that all of them refuse a step that one of them would, and with poll_lag (None: as
+    soon as this host sees it; k >= 0: k steps later; default 2 in such a job) all of them raise NonFiniteOperand from the same call,
+    as under FusedAdamAmsgrad.  world_size=1: an optimiser that only this rank steps.
 
     Found-non-finite guard: the kernel refuses a step behind a split-f16 kernel that reported a NaN / inf operand, and the BatchNorm
     statistics of the forward passes since the last step are taken back, as FusedAdamAmsgrad does.  Unlike there the gradients themselves
@@ -358,7 +379,7 @@ class FusedAdamW(object):
 
     DEFAULTS = ("lr", "betas", "eps", "weight_decay")
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, world_size=None, poll_lag="auto"):
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32, got %r" % (state_bits,))
         if hasattr(params, "parameters"):
@@ -401,6 +422,9 @@ class FusedAdamW(object):
         self.step_count = 0
         self.skipped_steps = 0
         self._skipped = zeros(1, torch.int32)
+        self.world_size = world_size
+        self._rank_flag = zeros(1, torch.float32)
+        self._init_poll((2 if self._shared() else None) if poll_lag == "auto" else poll_lag)
         ops._GUARDED.add(self)
         # the table of tensors: gradient addresses change from step to step, the rest only when a parameter moves
         self._rows = np.zeros((len(self.params), 6), dtype=np.int64)
@@ -487,6 +511,10 @@ class FusedAdamW(object):
         self._sent = at
         return grads
 
+    def _shared(self):
+        """Whether the ranks of a job agree on what they refuse."""
+        return self.world_size != 1 and parallel.collectives_on()
+
     @torch.no_grad()
     def step(self, grad_scale=1.0):
         """One update of every tensor that has a gradient, multiplied by grad_scale first."""
@@ -494,16 +522,23 @@ class FusedAdamW(object):
             raise RuntimeError("FusedAdamW.step() cannot be captured into a graph (the step number is an argument of the launch): "
                                "capture forward and backward, and call step() behind the replay")
         ops._there(self.exp_avg, self._update, self._hyper(), float(grad_scale))
-        ops.check_device_errors()
 
     def _update(self, hyper, grad_scale):
         grads = self._table()
         self.step_count += 1
+        lagged = self.poll_lag is not None and ops.USE_SF16
+        shared = self._shared() and ops.USE_SF16
+        if shared:
+            ops.guard_publish(self._rank_flag)
+            parallel.sum_words(self._rank_flag)
+        if shared or lagged:
+            ops.guard_collect(self._rank_flag if shared else None, self._skipped, self._status_ptr() if lagged else None)
         if len(self._chunks):
             ops.adamw_(self._dev_rows, self._chunks, len(self._chunks), self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
                        self.exp_avg_sq_scale, self.master, self.state_bits, hyper, self.step_count, grad_scale, skipped=self._skipped)
         del grads
         ops.restore_bn_if_refused()        # a step refused after its forward pass takes the BatchNorm statistics back too
+        self._settle(lagged)
 
     def moments(self):
         """(exp_avg, exp_avg_sq) as flat float32 buffers: the state itself with 32 bits, the values that the codes stand for with 8."""

@@ -130,6 +130,18 @@ def broadcast_rng_state(src=0):
         torch.set_rng_state(t.cpu())
 
 
+def sum_words(t):
+    """t (a few floats, in place) summed over the ranks, in the order of the current stream; over gloo through host memory."""
+    if not collectives_on():
+        return
+    if t.is_cuda and dist.get_backend() != "nccl":
+        h = t.cpu()
+        dist.all_reduce(h, op=dist.ReduceOp.SUM)
+        t.copy_(h)
+    else:
+        dist.all_reduce(t, op=dist.ReduceOp.SUM)
+
+
 def allreduce_flat_grad(flat_grad, buckets=1, async_op=False):
     """Sum the flat gradient buffer over ranks (the mean's 1/world is applied inside the optimiser kernel).
     `buckets` > 1 splits the buffer into contiguous chunks.  (The overlapped, readiness-driven form is GradBuckets.)"""

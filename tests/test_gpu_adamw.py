@@ -451,3 +451,28 @@ def test_a_refused_step_of_the_other_optimiser_leaves_the_statistics_of_settled_
         flat.step()
         ops.check_device_errors(synchronize=True)
     assert all(torch.equal(v, stats[k]) for k, v in _statistics(m).items())
+
+
+@gpu
+def test_lagged_poll_reports_a_refused_step_two_steps_later():
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = optim.FusedAdamW([p], poll_lag=2)
+    ops.check_device_errors(synchronize=True)
+    opt.step()
+    before = p.detach().clone()
+    _report()
+    opt.step()
+    opt.step()
+    with pytest.raises(ops.NonFiniteOperand) as e:
+        opt.step()
+    assert e.value.skipped_steps == 3 and opt.step_count == 1 and opt.skipped_steps == 3 and torch.equal(before, p.detach())
+    opt.step()
+    opt.poll(0)
+    assert opt.step_count == 2 and not torch.equal(before, p.detach())
+
+
+def test_guard_collect_refuses_bad_arguments():
+    from sound_event_detection_dcase2017_task4_amd import _lib
+    h = _lib.lib()
+    assert h.sed_guard_collect(16, None, 16, None, None, None) == -22 and h.sed_guard_collect(16, 16, None, None, 16, None) == -22

@@ -497,3 +497,68 @@ def test_train_cli_two_ranks_fall_back_together_when_one_capture_is_refused(tmp_
     assert any("another rank" in w for w in a["warns"]) and any("rank 1 (test)" in w for w in b["warns"])
     losses = [float(l.split()[1]) for l in r.stdout.splitlines() if len(l.split()) == 2 and l.split()[0].isdigit()]
     assert len(losses) == 7 and all(np.isfinite(losses))
+
+
+def _adamw_worker(rank, world, port, outdir, poll_lag):
+    """Four steps of a model under FusedAdamW; in the third one rank 0's split-f16 kernels report a NaN and its gradients hold one.
+    The gradients are summed over the ranks through host memory, as a caller of FusedAdamW does by itself."""
+    sys.path.insert(0, REPO)
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK="0", MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port),
+                      SED_SHARE_GPU="1", HSA_ENABLE_IPC_MODE_LEGACY="0")
+    from oracle import model as om
+    from sound_event_detection_dcase2017_task4_amd import ops, parallel
+    from sound_event_detection_dcase2017_task4_amd.optim import FusedAdamW
+    from sound_event_detection_dcase2017_task4_amd.pytorch import models
+    from sound_event_detection_dcase2017_task4_amd.pytorch.losses import clip_bce
+    parallel.init_from_env()
+    torch.cuda.set_device(0)
+    m = models.Cnn_9layers_FrameAvg(*CTOR)
+    m.load_state_dict(om.recipe_state("Cnn_9layers_FrameAvg", 3))
+    m = m.cuda().train()
+    opt = FusedAdamW(m, lr=1e-3, **({} if poll_lag == "default" else {"poll_lag": poll_lag}))
+    rs = np.random.RandomState(10 + rank)
+    x, y = torch.from_numpy((rs.randn(4, 32000) * 0.1).astype(np.float32)).cuda(), torch.from_numpy((rs.rand(4, 17) < 0.2).astype(np.float32)).cuda()
+    raised, skipped, held = [], [], None
+    for k in range(8):
+        opt.zero_grad()
+        clip_bce(m(x), {"target": y}).backward()
+        if k == 2:
+            torch.cuda.synchronize()
+            held = [p.detach().cpu().clone() for p in opt.params]
+            if rank == 0:
+                opt.params[0].grad.fill_(float("nan"))
+                ops._err_dev()[0] = 1
+                torch.cuda.synchronize()
+                ops._err_flag()[1] = 1
+        for p in opt.params:
+            if p.grad is not None:
+                h = p.grad.cpu()
+                torch.distributed.all_reduce(h)
+                p.grad.copy_(h)
+        try:
+            opt.step(grad_scale=1.0 / world)
+        except ops.NonFiniteOperand as e:
+            raised.append(k)
+            skipped.append(e.skipped_steps)
+            params = [p.detach().cpu().clone() for p in opt.params]
+    opt.poll(0)
+    torch.cuda.synchronize()
+    torch.save({"raised": raised, "skipped": skipped, "steps": opt.step_count, "refused": opt.skipped_steps, "held": held, "params": params,
+                "end": [p.detach().cpu() for p in opt.params]}, os.path.join(outdir, "rank%d.pt" % rank))
+    torch.distributed.barrier()
+    torch.distributed.destroy_process_group()
+
+
+@pytest.mark.parametrize("poll_lag", ["default", 0])
+def test_ranks_under_adamw_refuse_the_same_step(tmp_path, poll_lag):
+    """One rank's kernels report a NaN: every rank refuses that step (and those issued until it is reported), raises from the same call
+    with the same count, keeps its parameters, and goes on."""
+    from sound_event_detection_dcase2017_task4_amd import parallel
+    world, lag = 2, 2 if poll_lag == "default" else poll_lag
+    mp.spawn(_adamw_worker, args=(world, parallel.free_port(), str(tmp_path), poll_lag), nprocs=world, join=True)
+    rs = [torch.load(os.path.join(str(tmp_path), "rank%d.pt" % r)) for r in range(world)]
+    for r in rs:
+        assert r["raised"] == [2 + lag] and r["skipped"] == [lag + 1] and r["refused"] == lag + 1 and r["steps"] == 8 - (lag + 1)
+        assert all(torch.equal(a, b) for a, b in zip(r["held"], r["params"]))
+        assert all(torch.isfinite(v).all() for v in r["end"]) and not torch.equal(r["end"][-1], r["params"][-1])
+    assert all(torch.equal(a, b) for a, b in zip(rs[0]["end"], rs[1]["end"])), "ranks diverged"

@@ -388,3 +388,28 @@ def test_bench_strong_row_watchdog_keeps_the_headline_line():
              "w = bench.StrongRowWatchdog({'a': 1}, 0.5); w.cancel(); time.sleep(1.5); print('done')\n" % REPO)
     r = subprocess.run([sys.executable, "-c", code2], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip() == "done"
+
+
+def _sum_words_worker(rank, world, port, out):
+    sys.path.insert(0, REPO)
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank), MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    from sound_event_detection_dcase2017_task4_amd import parallel
+    parallel.init_from_env(backend="gloo")
+    for mine in (0.0, float("nan"), 0.0):
+        t = torch.tensor([mine if rank == 1 else 0.0])
+        parallel.sum_words(t)
+        assert bool(torch.isnan(t[0])) == (mine != mine) and (mine != mine or float(t) == 0.0)
+    dist.barrier()
+    if rank == 0:
+        open(out, "w").write("ok")
+    dist.destroy_process_group()
+
+
+def test_one_ranks_flag_reaches_the_others(tmp_path):
+    from sound_event_detection_dcase2017_task4_amd import parallel
+    t = torch.ones(1)
+    parallel.sum_words(t)                                          # no process group: left as it is
+    assert float(t) == 1.0
+    out = str(tmp_path / "ok")
+    mp.spawn(_sum_words_worker, args=(2, _free_port(), out), nprocs=2, join=True)
+    assert open(out).read() == "ok"
