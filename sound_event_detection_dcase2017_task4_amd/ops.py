@@ -11,6 +11,7 @@ import weakref
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -1958,6 +1959,9 @@ def _there(t, f, *args):
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}                  # SED_ACT_*; gelu is z Phi(z)
 
+# Calls that need no gradient launch without autograd.  Inside a forward-mode level (forward_ad.dual_level) they do not: the Function
+# refuses a tangent (NotImplementedError) that the bare launch would drop.
+
 
 def _act_code(activation):
     if activation not in ACTIVATIONS:
@@ -2066,7 +2070,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         for t in (x, weight, bias):                       # stays part of the graph, with gradients of zero
             y = y + t.sum().to(x.dtype) * 0 if grad and t is not None and t.requires_grad else y
         return y
-    if grad:
+    if grad or forward_ad._current_level >= 0:
         return GroupNormActFn.apply(x, weight, bias, groups, float(eps), act)
     return _there(x, _group_norm_fwd, _contiguous(x), _contiguous(weight), _contiguous(bias), groups, float(eps), act)[0]
 
@@ -2155,7 +2159,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         for t in (x, weight, bias, residual):             # stays part of the graph, with gradients of zero
             y = y + t.sum().to(dtype) * 0 if grad and t is not None and t.requires_grad else y
         return y
-    if grad:
+    if grad or forward_ad._current_level >= 0:
         return LinearActFn.apply(x, weight, bias, residual, act)
     return _there(x, _linear_fwd, _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), act, False)[0]
 

@@ -188,3 +188,18 @@ def test_a_model_of_the_package_under_adamw():
     fresh = fresh.cuda().eval()
     with torch.no_grad():
         assert torch.equal(model(x)["clipwise_output"], fresh(x)["clipwise_output"])
+
+
+@gpu
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor has a derivative that the operators do not carry on: they refuse it, with gradients switched on or off."""
+    from torch.autograd import forward_ad
+    x, w, b = torch.randn(6, 8, device="cuda"), torch.randn(8, 8, device="cuda"), torch.randn(8, device="cuda")
+    with forward_ad.dual_level():
+        for off in (False, True):
+            for call in (lambda t: ops.linear_act(t, w, b), lambda t: ops.linear_act(t, w, b, "silu", x), lambda t: ops.group_norm_act(t, 2, b, b),
+                         lambda t: ops.linear_act(x, w, b, "none", t)):
+                with torch.set_grad_enabled(not off), pytest.raises(NotImplementedError):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)))
+        y = ops.linear_act(x, w, b)                        # without a tangent the call is the usual one
+    assert torch.equal(y, ops.linear_act(x, w, b))
