@@ -70,7 +70,7 @@ def compile_cmd(src, obj, flags=None):
 def build(force=False, verbose=False):
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    hdrs = [os.path.join(CSRC, "common.h"), os.path.join(INCLUDE, "sed_hip.h")]
+    hdrs = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "act.h"), os.path.join(INCLUDE, "sed_hip.h")]
     # objects compiled with other flags (an experiment build) are never mixed with these: the stamp forces a full rebuild
     stamp = os.path.join(objdir, "flags.stamp")
     want = flags_hash(FLAGS + [f for s in SOURCES for f in SOURCE_FLAGS.get(s, [])])

@@ -11,6 +11,7 @@
 // A thread owns V channels (16 bytes) of every RT-th row of a chunk of rows, whatever the group width: sums are held per channel and
 // folded to groups afterwards.  A row that is not a multiple of V channels ends in a vector that overlaps its neighbour (the twice
 // computed channels are written twice with the same value, and counted once), and loads need no more than element alignment.
+#include "act.h"
 #include "common.h"
 #include "sed_hip.h"
 

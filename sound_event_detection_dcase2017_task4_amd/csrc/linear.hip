@@ -8,6 +8,7 @@
 // straight from memory, and read from there as the matrix instructions want it: 16 bytes of one row, or by transposing reads.
 // The matrix instruction takes P as its first operand: a lane then holds four consecutive n of one row m, which it can store together.
 // Products of 32-bit tensors run on the fp32 matrix instructions; sums are held in 32 bits for all types.
+#include "act.h"
 #include "common.h"
 #include "sed_hip.h"
 
