@@ -376,3 +376,22 @@ def test_gradients_at_the_ends_of_the_range(dtype):
             keep = torch.arange(len(a), device="cuda") != at
             assert torch.equal(a[keep], c[keep]) and not torch.isfinite(a[at]).any()
             assert torch.equal(a[at].double().nan_to_num(1.0, 2.0, 3.0), b[at].nan_to_num(1.0, 2.0, 3.0))
+
+
+@gpu
+@pytest.mark.parametrize("m", [50, 200001])
+def test_gelu_and_its_derivative_over_the_range(m):
+    """z Phi(z) with Phi(-|z|) right to a few roundings of itself: 16 H for the polynomial, the reciprocal and the products, and 1.5 z^2 H for
+    the exponential's argument z^2 / 2, which is rounded three times.  A positive z takes them of 1 - Phi and adds two of its own.  The
+    derivative has the same in Phi and in z phi."""
+    z = torch.linspace(-9.0, 9.0, m, device="cuda").view(-1, 1).requires_grad_(True)
+    one = torch.ones(1, 1, device="cuda")
+    y = ops.linear_act(z, one, activation="gelu")
+    g, = torch.autograd.grad(y.sum(), z)
+    zd = z.detach().double()
+    tail, phi = 0.5 * torch.erfc(zd.abs() / 2 ** 0.5), torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi)
+    cdf = torch.where(zd < 0, tail, 1 - tail)
+    near = (16 + 1.5 * zd * zd) * H
+    terr = tail * near + torch.where(zd < 0, 0.0, 2 * H)
+    assert ((y.detach().double() - zd * cdf).abs() <= zd.abs() * terr + 2.0 ** -126).all()
+    assert ((g.double() - (cdf + zd * phi)).abs() <= terr + zd.abs() * phi * near + 2 * H * (cdf + zd * phi).abs() + 2.0 ** -126).all()
