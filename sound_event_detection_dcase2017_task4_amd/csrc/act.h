@@ -27,7 +27,6 @@ template <int ACT> __device__ __forceinline__ float sed_act(float z) {
     return z;
 }
 template <int ACT> __device__ __forceinline__ float sed_act_grad(float z) {
-    if (ACT == 1) return z > 0.f ? 1.f : 0.f;
     if (ACT == 2) {
         const float s = sed_sigmoid(z);
         return s * fmaf(z, 1.f - s, 1.f);
@@ -37,4 +36,9 @@ template <int ACT> __device__ __forceinline__ float sed_act_grad(float z) {
         return fmaf(z * e, 0.39894228040143268f, sed_phi_cdf(z, e));
     }
     return 1.f;
+}
+// gy act'(z).  ReLU selects: an infinite gy is 0 where z is not positive, and passes where z is NaN, as in torch
+template <int ACT> __device__ __forceinline__ float sed_act_gz(float gy, float z) {
+    if (ACT == 1) return z <= 0.f ? 0.f : gy;
+    return gy * sed_act_grad<ACT>(z);
 }

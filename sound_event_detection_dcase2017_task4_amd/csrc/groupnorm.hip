@@ -384,7 +384,7 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
                         const float xh = ((float)v[u].v[j] - m[j]) * r[j];
-                        const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
+                        const float gz = sed_act_gz<ACT>((float)g[u].v[j], fmaf(xh, w[j], b[j]));
                         s1[j] += gz;
                         s2[j] = fmaf(gz, xh, s2[j]);
                     }
@@ -499,7 +499,7 @@ template <typename T, int V, int ACT> __global__ __launch_bounds__(THREADS) void
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float xh = ((float)v[u].v[j] - m[j]) * r[j];
-                    const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
+                    const float gz = sed_act_gz<ACT>((float)g[u].v[j], fmaf(xh, w[j], b[j]));
                     v[u].v[j] = (T)(r[j] * (fmaf(gz, w[j], -c1[j]) - xh * c2[j]));
                 }
                 store_vec<T, V>(gx + (s + (long)u * p.RT) * p.C, v[u]);
@@ -719,7 +719,7 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float xh = ((float)v[u].v[j] - m[j]) * r[j];
-                const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
+                const float gz = sed_act_gz<ACT>((float)g[u].v[j], fmaf(xh, w[j], b[j]));
                 s1[j] += gz;
                 s2[j] = fmaf(gz, xh, s2[j]);
             }
@@ -748,7 +748,7 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float xh = ((float)v[u].v[j] - m[j]) * r[j];
-                const float gz = (float)g[u].v[j] * sed_act_grad<ACT>(fmaf(xh, w[j], b[j]));
+                const float gz = sed_act_gz<ACT>((float)g[u].v[j], fmaf(xh, w[j], b[j]));
                 v[u].v[j] = (T)(r[j] * (fmaf(gz, w[j], -c1[j]) - xh * c2[j]));
             }
             store_vec<T, V>(gx + (long)(r0 + u * RT) * p.C, v[u]);

@@ -47,7 +47,7 @@ __device__ __forceinline__ void store_typed(void* p, int type, long i, float v) 
 
 // What is kept of z for the backward pass, which reads nothing but act'(z) from it: z in 32 bits, whatever the tensors' type.  (A z of
 // 16 bits puts |act''(z) z| 2^-12 into a float16 gradient, as much as its own rounding, and as much into a bias gradient of 32 bits.)
-// ReLU keeps 1 or 0, in 16 bits beside 16-bit tensors.
+// ReLU keeps 1 or 0, in 16 bits beside 16-bit tensors; a NaN counts as on, so that its gradient passes as in torch.
 template <typename T> struct Mask { typedef _Float16 type; };
 template <> struct Mask<float> { typedef float type; };
 template <typename T, int ACT> struct Kept { typedef float type; };
@@ -103,7 +103,7 @@ template <typename T, int V, int ACT> __device__ __forceinline__ void finish(con
             typedef typename Mask<T>::type Z;
             typename Wide<Z, V>::type k;
 #pragma unroll
-            for (int r = 0; r < V; ++r) k[r] = (Z)(v[r] > 0.f ? 1.f : 0.f);
+            for (int r = 0; r < V; ++r) k[r] = (Z)(v[r] <= 0.f ? 0.f : 1.f);
             *reinterpret_cast<typename Wide<Z, V>::type*>(reinterpret_cast<Z*>(e.z) + m * e.ldz + n) = k;
         } else {
             float* const z = reinterpret_cast<float*>(e.z) + m * e.ldz + n;

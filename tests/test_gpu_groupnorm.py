@@ -391,3 +391,22 @@ def test_a_row_far_from_the_others(shape, groups, where):
     want = ((xd - mean) / torch.sqrt(var + 1e-5)).reshape(shape)
     far = float((mean.abs() / var.sqrt()).max())
     assert ((y.double() - want).abs() <= 100 * H * want.abs() + 6 * H * far + 4 * H).all()
+
+
+@gpu
+@pytest.mark.parametrize("shape,groups", [((2, 130, 48), 6), ((2, 9000, 40), 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_relu_selects_its_gradient(shape, groups, dtype):
+    """As torch: an infinite gradient does not come through a unit that is off, and a unit whose z is NaN is on (in one pass and in two)."""
+    C = shape[-1]
+    x, w, b, gy = _inputs(shape, dtype, torch.float32, 19)
+    b = torch.where(torch.arange(C, device="cuda") % 2 == 0, 40.0, -40.0)
+    b[9] = float("nan")                                      # a bias enters no sum but its own channel's
+    gy[0, 3, 1], gy[1, 7, 5] = float("inf"), float("nan")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], activation="relu"), leaves, gy)
+    want = _reference(x, w, b, groups, 1e-5, "relu", gy)[1:]
+    assert all(torch.isfinite(t).all() for t in want)
+    for a, c in zip(got, want):
+        # normwise: sums of about a hundred H (as in _check) beside the output's own rounding
+        assert float((a.double().cpu() - c).norm()) <= (200 * H + HALF[a.dtype]) * float(c.norm())

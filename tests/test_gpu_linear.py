@@ -395,3 +395,29 @@ def test_gelu_and_its_derivative_over_the_range(m):
     terr = tail * near + torch.where(zd < 0, 0.0, 2 * H)
     assert ((y.detach().double() - zd * cdf).abs() <= zd.abs() * terr + 2.0 ** -126).all()
     assert ((g.double() - (cdf + zd * phi)).abs() <= terr + zd.abs() * phi * near + 2 * H * (cdf + zd * phi).abs() + 2.0 ** -126).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [6, 200])
+def test_relu_passes_the_gradient_of_a_nan(m, dtype):
+    """As torch: a unit whose z is NaN is on, and a gradient that is not finite does not come through one that is off."""
+    x, w, b, _, gy = _inputs(m, 40, 24, dtype, dtype, 51, residual=False)
+    b = torch.where(torch.arange(24, device="cuda") % 2 == 0, 30.0, -30.0).to(dtype)
+    b[3], gy[2, 5] = float("nan"), float("inf")              # unit 5 is off
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(ops.linear_act(*leaves, activation="relu"), leaves, gy)
+    d = [t.detach().double().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(F.relu(F.linear(*d)), d, gy.double())
+    on = (torch.arange(24, device="cuda") % 2 == 0) | (torch.arange(24, device="cuda") == 3)
+    gz = torch.where(on, gy.double(), 0.0)
+    terms = (_sum_err(24) * (gz.abs() @ d[1].abs()), _sum_err(m) * (gz.abs().t() @ d[0].abs()), _sum_err(m) * gz.abs().sum(0))
+    for a, c, t in zip(got, want, terms):
+        assert ((a.double() - c).abs() <= t.detach() + HALF[dtype] * 1.01 * c.abs() + TINY[dtype]).all()
+    w[3, 7] = float("nan")                                   # a NaN that comes in through W: rows of gx are NaN there and nowhere else
+    leaves[1] = w.clone().requires_grad_(True)
+    leaves[2] = torch.where(torch.isnan(b), torch.zeros_like(b), b).requires_grad_(True)
+    got = torch.autograd.grad(ops.linear_act(*leaves, activation="relu"), leaves, gy)
+    d = [t.detach().double().requires_grad_(True) for t in leaves]
+    want = torch.autograd.grad(F.relu(F.linear(*d)), d, gy.double())
+    assert all(torch.equal(torch.isnan(a), torch.isnan(c)) for a, c in zip(got, want))
