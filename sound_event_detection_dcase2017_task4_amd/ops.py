@@ -1981,6 +1981,12 @@ def _chk_operand(name, t, shape, dtype, other, device):
         raise ValueError("%s is on %s, the input on %s" % (name, t.device, device))
 
 
+def _chk_values(name, t):
+    """A ConvBlock's output with pairs_out=True is float32 by type, and holds split-f16 operand pairs."""
+    if getattr(t, "_sed_pairs", False):
+        raise ValueError("%s holds split-f16 operand pairs (a ConvBlock's output with pairs_out=True), not numbers: leave pairs_out False" % name)
+
+
 def _bytes(n, like):
     return like.new_empty(n, dtype=torch.uint8) if n else None
 
@@ -2052,6 +2058,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         raise ValueError("x must be float32, float16 or bfloat16, got %s" % x.dtype)
     if x.dim() < 2:
         raise ValueError("x must be (batch, ..., channels), got shape %s" % (tuple(x.shape),))
+    _chk_values("x", x)
     groups, C = int(groups), x.shape[-1]
     if groups < 1 or C < 1 or C % groups:
         raise ValueError("groups must divide the channels: %d channels, %d groups" % (C, groups))
@@ -2145,12 +2152,14 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         raise ValueError("x must be float32, float16 or bfloat16, got %s" % dtype)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError("x (..., K) and weight (N, K) do not fit: %s and %s" % (tuple(x.shape), tuple(weight.shape)))
+    _chk_values("x", x)
     N = weight.shape[0]
     _chk_operand("weight", weight, weight.shape, dtype, dtype, device)
     if bias is not None:
         _chk_operand("bias", bias, (N,), dtype, torch.float32, device)
     if residual is not None:
         _chk_operand("residual", residual, x.shape[:-1] + (N,), dtype, dtype, device)
+        _chk_values("residual", residual)
     _chk_dev(x)
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad))

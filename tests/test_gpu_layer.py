@@ -203,3 +203,12 @@ def test_forward_mode_tangents_are_refused():
                     call(forward_ad.make_dual(x, torch.ones_like(x)))
         y = ops.linear_act(x, w, b)                        # without a tangent the call is the usual one
     assert torch.equal(y, ops.linear_act(x, w, b))
+
+
+def test_operand_pairs_are_refused():
+    """They are marked on the tensor that a ConvBlock returns, and look like float32."""
+    x, w, pairs = torch.zeros(3, 8), torch.zeros(8, 8), torch.zeros(3, 8)
+    pairs._sed_pairs = True
+    for call in (lambda: ops.linear_act(pairs, w), lambda: ops.linear_act(x, w, residual=pairs), lambda: ops.group_norm_act(pairs, 2)):
+        with pytest.raises(ValueError, match="pairs"):
+            call()
