@@ -262,7 +262,7 @@ SED_API int sed_adamw(const long* rows, const int* chunks, long nchunks, void* m
         return SED_EINVAL;
     if (state_bits != 32 && (state_bits != 8 || !m_scale || !v_scale)) return SED_EINVAL;
     if (skip_flag && !skipped) return SED_EINVAL;
-    AdamwP a;
+    AdamwP a{};
     a.rows = rows; a.chunks = reinterpret_cast<const int2*>(chunks);
     a.m = m; a.v = v; a.ms = m_scale; a.vs = v_scale; a.master = master;
     a.skip_flag = skip_flag; a.skipped = skipped; a.grad_scale = grad_scale;

@@ -15,6 +15,8 @@ several backward passes into one step needs `direct_grads=False` (plain autograd
 """
 import array
 import collections
+import itertools
+import operator
 
 import numpy as np
 import torch
@@ -355,7 +357,8 @@ class FusedAdamW(_LaggedPoll):
     """AdamW (decoupled weight decay) over many separate tensors in ONE launch (sed_adamw), float32 / float16 / bfloat16 ones together.
 
     params: a module, an iterable of tensors, or a list of groups {'params': [...], 'lr' / 'betas' / 'eps' / 'weight_decay': ...} as
-    torch.optim.AdamW takes them (at most 16 groups); `param_groups` may be changed between steps.  Gradients are read from `p.grad`
+    torch.optim.AdamW takes them (at most 16 groups); the options in `param_groups` may be changed between steps, the groups and their
+    tensors may not (ValueError at the next step).  Gradients are read from `p.grad`
     wherever they lie; a tensor whose gradient is None is left as it is in that step (weight decay and moments too).  One step
     counter serves all tensors, as in FusedAdamAmsgrad.
 
@@ -400,6 +403,7 @@ class FusedAdamW(_LaggedPoll):
             raise ValueError("no trainable parameters")
         if len(self.param_groups) > 16:
             raise ValueError("at most 16 parameter groups, got %d" % len(self.param_groups))
+        self._group_sizes = [len(g["params"]) for g in self.param_groups]
         self._hyper()                                       # refuses bad values now, not at the first step
         self._check_params()
         dev = self.params[0].device
@@ -443,7 +447,12 @@ class FusedAdamW(_LaggedPoll):
         torch.cuda.current_stream(dev).synchronize()        # the buffers are complete when this returns: any stream may use them
 
     def _hyper(self):
-        """lr, beta1, beta2, eps, weight_decay of every group as one array of doubles, which the launch copies."""
+        """lr, beta1, beta2, eps, weight_decay of every group as one array of doubles, which the launch copies.  The table of tensors holds
+        group numbers: the groups must be those that it was made of."""
+        if [len(g["params"]) for g in self.param_groups] != self._group_sizes or not all(
+                map(operator.is_, itertools.chain.from_iterable(g["params"] for g in self.param_groups), self.params)):
+            raise ValueError("FusedAdamW: the parameter groups or their tensors changed since the optimiser was made (the options may, "
+                             "the tensors may not)")
         rows = []
         for g in self.param_groups:
             lr, (b1, b2), eps, wd = float(g["lr"]), g["betas"], float(g["eps"]), float(g["weight_decay"])
