@@ -490,7 +490,7 @@ int sed_guard_publish(const int* err_dev, float* flag_out, sed_stream_t stream);
  *   gz = gy act'(z);  gweight = sum gz xhat;  gbias = sum gz  ([C] of wdtype, nullable)
  *   gx = rstd (gz weight - mean_g(gz weight) - xhat mean_g(gz weight xhat))  (nullable)
  * ws: sed_group_norm_ws_floats(..) floats of scratch (0: null will do).  No pointer needs more than its element's alignment; results
- * do not overlap operands.  N, S, C >= 1, C % G == 0, N G < 2^22, N times the workgroups of a sample (one up to 16 KB) below 2^24. */
+ * do not overlap operands.  N, S, C >= 1, C < 2^26 - 16, C % G == 0, N G < 2^22, N times the workgroups of a sample (one up to 16 KB) below 2^24. */
 long sed_group_norm_ws_floats(int dtype, long N, long S, int C, int G, int backward);
 int sed_group_norm_fwd(const void* x, const void* weight, const void* bias, int dtype, int wdtype, long N, long S, int C, int G,
                        float eps, int act, void* y, float* mean, float* rstd, float* ws, sed_stream_t stream);

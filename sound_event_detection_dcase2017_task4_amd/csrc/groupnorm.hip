@@ -963,7 +963,8 @@ __global__ __launch_bounds__(256) void norm_zero_kernel(int* p, long n) {
 int esize_of(int dtype) { return dtype == SED_F32 ? 4 : 2; }
 bool bad_shape(int dtype, int wdtype, long N, long S, int C, int G, int act) {
     return dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2 || N < 1 || S < 1 || C < 1 || G < 1 || C % G || act < 0 || act > 3 ||
-           N * G >= 1L << 22 || cut_of(N, S, C, esize_of(dtype)).blocks + C / 16 + 1 >= 1L << 24;         // a launch takes fewer than 2^32 threads
+           // a launch takes fewer than 2^32 threads: 1024 a workgroup for the joins and the parameters' sums, 256 for the passes
+           N * G >= 1L << 22 || C / 16 + 1 >= 1L << 22 || cut_of(N, S, C, esize_of(dtype)).blocks + C / 16 + 1 >= 1L << 24;
 }
 // How the one-pass kernels cut: bundles of whole groups with at least 128 bytes of a row (or all of it), a workgroup of so many threads
 // that each holds up to R vectors.  threads = 0: the rows do not fit, or a row has fewer channels than a vector.

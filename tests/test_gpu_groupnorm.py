@@ -410,3 +410,30 @@ def test_relu_selects_its_gradient(shape, groups, dtype):
     for a, c in zip(got, want):
         # normwise: sums of about a hundred H (as in _check) beside the output's own rounding
         assert float((a.double().cpu() - c).norm()) <= (200 * H + HALF[a.dtype]) * float(c.norm())
+
+
+def test_c_entries_refuse_more_channels_than_the_parameter_sums_hold():
+    from sound_event_detection_dcase2017_task4_amd import _lib
+    h = _lib.lib()
+    for t in (0, 1, 2):
+        for n, s, c, g in ((1, 1, 1 << 26, 1 << 20), (1, 1, 1 << 26, 1 << 21), (1, 3, (1 << 26) + 4096, 1 << 12)):
+            for backward in (0, 1):
+                assert h.sed_group_norm_ws_floats(t, n, s, c, g, backward) == 0
+            assert h.sed_group_norm_fwd(16, None, None, t, 0, n, s, c, g, 1e-5, 0, 16, 16, 16, 16, None) == -22
+            assert h.sed_group_norm_bwd(16, 16, None, None, t, 0, n, s, c, g, 0, 16, 16, None, 16, 16, 16, None) == -22
+
+
+@gpu
+@pytest.mark.parametrize("shape,groups", [((2, 9000, 40), 5), ((3, 40001, 24), 3), ((2, 6001, 51), 17)])
+def test_only_wanted_gradients_in_two_passes(shape, groups):
+    """Rows that a workgroup cannot hold: the parameters' sums have a launch of their own where x needs no gradient.  They are the sums of the
+    same numbers as beside gx, added in another order: a hundred H of them in the norm, as in _check."""
+    x, w, b, gy = _inputs(shape, torch.float32, torch.float32, 15)
+    full = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    every = torch.autograd.grad(ops.group_norm_act(full[0], groups, full[1], full[2], activation="gelu"), full, gy)
+    want = _reference(x, w, b, groups, 1e-5, "gelu", gy)[1:]
+    for wanted in ((0,), (1,), (2,), (1, 2), (0, 2)):
+        leaves = [t.clone().requires_grad_(j in wanted) for j, t in enumerate((x, w, b))]
+        got = torch.autograd.grad(ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], activation="gelu"), [leaves[j] for j in wanted], gy)
+        for j, t in zip(wanted, got):
+            assert float((t.double().cpu() - want[j]).norm()) <= 200 * H * float(want[j].norm()) and float((t - every[j]).norm()) <= 100 * H * float(every[j].norm())
