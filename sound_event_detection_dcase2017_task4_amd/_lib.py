@@ -108,9 +108,11 @@ def verify_flags(h):
 
 
 class SedHipError(RuntimeError):
-    pass
+    code = 0
 
 
 def check(rc, what):
     if rc != 0:
-        raise SedHipError("%s failed with code %d%s" % (what, rc, " (invalid argument)" if rc == -22 else " (hipError_t)"))
+        err = SedHipError("%s failed with code %d%s" % (what, rc, " (invalid argument)" if rc == -22 else " (hipError_t)"))
+        err.code = rc
+        raise err

@@ -1987,6 +1987,13 @@ def _chk_values(name, t):
         raise ValueError("%s holds split-f16 operand pairs (a ConvBlock's output with pairs_out=True), not numbers: leave pairs_out False" % name)
 
 
+def _too_large(error, sizes, limits):
+    """What a call raises whose arguments were all checked but for their sizes: those that no launch holds are refused by name."""
+    if error.code != -22:
+        raise error
+    raise ValueError("%s: too large for a launch, which takes %s" % (sizes, limits)) from None
+
+
 def _bytes(n, like):
     return like.new_empty(n, dtype=torch.uint8) if n else None
 
@@ -2004,8 +2011,12 @@ def _group_norm_fwd(x, weight, bias, groups, eps, act):
     at, dt = stats.data_ptr(), DTYPE_CODES[x.dtype]
     ws = _bytes(4 * _lib.lib().sed_group_norm_ws_floats(dt, N, S, C, groups, 0), x)
     par = weight if weight is not None else bias
-    _call("sed_group_norm_fwd", x.data_ptr(), _ptr(weight), _ptr(bias), dt, DTYPE_CODES[par.dtype] if par is not None else 0,
-          N, S, C, groups, eps, act, y.data_ptr(), at, at + 4 * N * groups, _ptr(ws), _stream())
+    try:
+        _call("sed_group_norm_fwd", x.data_ptr(), _ptr(weight), _ptr(bias), dt, DTYPE_CODES[par.dtype] if par is not None else 0,
+              N, S, C, groups, eps, act, y.data_ptr(), at, at + 4 * N * groups, _ptr(ws), _stream())
+    except _lib.SedHipError as e:
+        _too_large(e, "x %s in %d groups" % (tuple(x.shape), groups), "batch x groups below 2^22, channels below 2^26 - 16, batch x the "
+                   "workgroups of a sample (one up to 16 KB) below 2^24")
     return y, stats
 
 
@@ -2094,8 +2105,12 @@ def _linear_fwd(x, weight, bias, residual, act, keep):
     px, pw = x.data_ptr(), weight.data_ptr()
     need = h.sed_linear_fwd_ws_bytes(px, pw, dt, M, N, K)
     ws = _bytes(need, x)
-    _call("sed_linear_fwd", px, pw, _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt, M, N, K, act,
-          y.data_ptr(), _ptr(z), _ptr(ws), need, _stream())
+    try:
+        _call("sed_linear_fwd", px, pw, _ptr(bias), _ptr(residual), dt, DTYPE_CODES[bias.dtype] if bias is not None else dt, M, N, K, act,
+              y.data_ptr(), _ptr(z), _ptr(ws), need, _stream())
+    except _lib.SedHipError as e:
+        _too_large(e, "x %s and weight %s" % (tuple(x.shape), (N, K)), "less than 2^31 - 256 rows, at most 2^21 columns, and x, weight and y "
+                   "below 2^38 elements")
     return y, z
 
 

@@ -212,3 +212,17 @@ def test_operand_pairs_are_refused():
     for call in (lambda: ops.linear_act(pairs, w), lambda: ops.linear_act(x, w, residual=pairs), lambda: ops.group_norm_act(pairs, 2)):
         with pytest.raises(ValueError, match="pairs"):
             call()
+
+
+@gpu
+def test_sizes_that_no_launch_holds_are_refused_by_name():
+    for x, groups in ((torch.zeros(2 ** 22, 1, 1, device="cuda"), 1), (torch.zeros(2 ** 12, 1, 2 ** 10, device="cuda"), 2 ** 10)):
+        for t in (x, x.requires_grad_(True)):
+            with pytest.raises(ValueError, match="too large"):
+                ops.group_norm_act(t, groups)
+    w = torch.zeros(2 ** 21 + 1, 1, device="cuda")
+    for t in (torch.zeros(3, 1, device="cuda"), torch.zeros(3, 1, device="cuda", requires_grad=True)):
+        with pytest.raises(ValueError, match="too large"):
+            ops.linear_act(t, w)
+    with pytest.raises(ValueError, match="too large"):
+        ops.linear_act(torch.zeros(3, 2 ** 21 + 1, device="cuda"), w.t())
