@@ -27,7 +27,7 @@ FLAGS = BASE_FLAGS + os.environ.get("SED_HIPCC_FLAGS", "").split()
 
 
 def flags_hash(flags=None):
-    """Identity of a set of hipcc flags (the include PATH is machine-specific and left out)."""
+    """Identity of a set of hipcc flags and of those that single sources get besides (the include PATH is machine-specific and left out)."""
     flags = list(BASE_FLAGS if flags is None else flags)
     keep, skip = [], False
     for f in flags:
@@ -40,6 +40,8 @@ def flags_hash(flags=None):
         if f.startswith("-DSED_BUILD_FLAGS_HASH"):
             continue
         keep.append(f)
+    for s in sorted(SOURCE_FLAGS):
+        keep += [s + ":"] + SOURCE_FLAGS[s]
     return hashlib.sha1(" ".join(keep).encode()).hexdigest()[:12]
 
 
@@ -73,7 +75,7 @@ def build(force=False, verbose=False):
     hdrs = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "act.h"), os.path.join(INCLUDE, "sed_hip.h")]
     # objects compiled with other flags (an experiment build) are never mixed with these: the stamp forces a full rebuild
     stamp = os.path.join(objdir, "flags.stamp")
-    want = flags_hash(FLAGS + [f for s in SOURCES for f in SOURCE_FLAGS.get(s, [])])
+    want = flags_hash(FLAGS)
     if not os.path.exists(stamp) or open(stamp).read().strip() != want:
         force = True
     jobs = []
