@@ -566,8 +566,8 @@ class FusedAdamW(_LaggedPoll):
 
     def load_state_dict(self, sd):
         """Takes over the step counter, the moments and the 32-bit copies of a state_dict() of the same tensors and state_bits; a
-        'master' of None (or none at all) takes the copies from the parameters, as does one that they are not the rounding of.  lr / betas / eps / weight_decay stay those of this
-        optimiser.  Anything that does not fit is refused (ValueError) before anything is changed."""
+        'master' of None (or none at all) takes the copies from the parameters, as does one that they are not the rounding of.  lr / betas /
+        eps / weight_decay stay those of this optimiser, as in FusedAdamAmsgrad.  Anything that does not fit is refused (ValueError) before anything is changed."""
         if "step" not in sd or "exp_avg" not in sd or "exp_avg_sq" not in sd:
             raise ValueError("unknown optimiser state layout (keys: %s): expected a FusedAdamW.state_dict()" % sorted(sd.keys()))
         if sd.get("state_bits", 32) != self.state_bits:
@@ -589,4 +589,8 @@ class FusedAdamW(_LaggedPoll):
         with torch.no_grad():
             for k, have in new.items():
                 getattr(self, k).copy_(have.reshape(-1))
+            if self.master is not None and "master" not in new:
+                for at, p in zip(self._copy_at, self.params):
+                    if p.dtype != torch.float32:
+                        self.master[at:at + p.numel()].copy_(p.detach().reshape(-1))
         self.step_count = step

@@ -497,3 +497,21 @@ def test_changed_groups_are_refused():
     opt.param_groups = groups
     opt.step()
     assert opt.step_count == 2 and float((ps[1].detach() - before[1]).abs().min()) > 0.1
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_without_copies_takes_them_from_the_parameters(bits):
+    ps = _tensors([1000, 257], (torch.bfloat16, torch.float32, torch.float16), 5)
+    opt = optim.FusedAdamW(ps, state_bits=bits)
+    for _ in range(3):
+        opt.step()
+    p = ps[0].detach().float().reshape(-1)
+    assert not torch.equal(opt.master[:1000], p)                  # the copy has bits that its rounding has not
+    sd = opt.state_dict()
+    for state in (dict(sd, master=None), {k: v for k, v in sd.items() if k != "master"}):
+        kept = opt.master.clone()
+        opt.load_state_dict(state)
+        assert torch.equal(opt.master[:1000], p)
+        opt.load_state_dict(dict(sd, master=kept))
+        assert torch.equal(opt.master, kept)
