@@ -14,9 +14,12 @@
 // is what the update sees:
 //   m = sign(q) (|q| / 127)^2 scale, q = rint(127 sqrt(|m| / scale))       half a step = 0.8 % at the scale, 8 % at a hundredth of it
 //   v = (q / 255)^4 scale,           q = rint(255 (v / scale)^(1/4))       half a step of sqrt(v) = 0.4 % at the scale
-// A positive v never decodes to 0 (its code is at least 1): m / (0 + eps) would be a step of any size.  The update itself uses the
-// new moments in 32 bits; only what the next step reads is rounded.  A NaN or an infinity in a block makes its scale NaN or infinite,
-// and the block reads back as NaN: as with 32-bit moments, nothing hides it.
+// A positive v does not decode to 0 (its code is at least 1, which stands for 2.4e-10 of the scale): m / (0 + eps) would be a step of any
+// size.  Below a scale of 3e-36 -- gradients of 1e-18 -- the product underflows to 0 all the same, and eps has to hold.  The update itself
+// uses the new moments in 32 bits; only what the next step reads is rounded.  A NaN in a block makes its scale NaN, and the block reads back
+// as NaN.  An infinite m (or a gradient beyond 1.8e19, whose square is) makes it infinite: the codes are then 0 for m, which reads back as
+// NaN; and 1 for a positive v, which reads back as infinity (0 as NaN): where only v overflowed, the block's updates are 0 from there on, as
+// a 32-bit element's are.
 #include "common.h"
 #include "sed_hip.h"
 

@@ -142,7 +142,7 @@ template <int V, typename F> __device__ __forceinline__ void fold_rows(const Nor
 
 // Statistics of a column of numbers in one reading: the sums run over d = x - k0, k0 the column's first number.  A column is what one
 // thread reads of a channel, 64 rows at most: whatever k0 is -- a padded row, an outlier -- the squares that cancel are at most 64 times
-// what k0 itself adds to the group's squares, and the variance keeps 32 - 6 bits' worth of it.
+// what k0 itself adds to the group's squares, and the variance keeps 24 - 6 bits of it.
 template <int V> __device__ __forceinline__ void column_stats(int count, const float (&k0)[V], float (&s1)[V], float (&s2)[V]) {      // -> mean, squared deviations
     const float inv = count ? 1.f / (float)count : 0.f;
 #pragma unroll
