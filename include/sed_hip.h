@@ -513,6 +513,9 @@ int sed_group_norm_bwd(const void* x, const void* gy, const void* weight, const 
  * with lines of up to 1 KB, 32 rows with 4 KB, 16 rows with 16 KB). */
 long sed_linear_kept_elements(long M, long N);
 long sed_linear_fwd_ws_bytes(const void* x, const void* weight, int dtype, long M, long N, long K);
+/* How a product is cut: its tile's edge (64, 128, 256; 1: a pass over the weight for a few rows) + 1024 times the slices along k that
+ * a second pass adds.  which: 0 y, 1 gx, 2 gweight.  0: sizes that are refused. */
+int sed_linear_plan(int dtype, long M, long N, long K, int act, int which);
 int sed_linear_fwd(const void* x, const void* weight, const void* bias, const void* residual, int dtype, int bdtype, long M, long N,
                    long K, int act, void* y, void* z, void* ws, long ws_bytes, sed_stream_t stream);
 long sed_linear_bwd_ws_bytes(const void* x, const void* weight, const void* gy, int dtype, long M, long N, long K, int act, int gx,

@@ -138,7 +138,7 @@ template <typename T> __device__ __forceinline__ void split(float f, T& large, T
     small = rest - rest == 0.f ? (T)(rest * (1.f / Split<T>::LOW)) : (T)0.f;
 }
 // SiLU and GELU beside 16-bit tensors: their gz has more bits than the tensors
-template <typename T> bool in_parts(int act) { return sizeof(T) == 2 && (act == SED_ACT_SILU || act == SED_ACT_GELU); }
+bool in_parts(int esize, int act) { return esize == 2 && (act == SED_ACT_SILU || act == SED_ACT_GELU); }
 
 // ---- 16 bytes of k of every row: one instruction in 16 bits, four in 32 (they take the k of a lane in any order, as long as P and Q agree)
 template <typename T> struct Frag;
@@ -838,6 +838,9 @@ long fwd_ws(const void* x, const void* w, int esize, long M, long N, long K) {
     return (needs_pad(x, K, esize) ? up256(M * ld * esize) : 0) + (needs_pad(w, K, esize) ? up256(N * ld * esize) : 0) + plan_of(M, N, ld, esize).part_bytes;
 }
 
+Plan plan_gx(long M, long N, long K, int esize, bool parts) { return plan_of(M, K, parts ? 2 * whole_steps(N, esize) : padded(N, esize), esize); }
+Plan plan_gw(long M, long N, long K, int esize, bool parts) { return plan_of(N, K, parts ? 2 * whole_steps(M, esize) : M, esize); }
+
 struct BwdNeeds {
     bool gz, px, pw;
 };
@@ -847,10 +850,10 @@ BwdNeeds bwd_needs(const void* x, const void* w, const void* gy, int esize, long
 long bwd_ws(const void* x, const void* w, const void* gy, int esize, long M, long N, long K, int act, bool gx, bool gw, bool gb) {
     const BwdNeeds d = bwd_needs(x, w, gy, esize, N, K, act, gx, gw);
     const long ldn = padded(N, esize), ldk = padded(K, esize);
-    const bool parts = esize == 2 && in_parts<_Float16>(act);
+    const bool parts = in_parts(esize, act);
     long b = (d.gz ? up256((parts ? 2 : 1) * M * ldn * esize) : 0) + (d.px ? up256(M * ldk * esize) : 0) + (d.pw ? up256(N * ldk * esize) : 0);
     if (gb) b += up256(grad_cut(M, ldn, esize).chunks * ldn * 4);
-    const Plan px = gx ? plan_of(M, K, parts ? 2 * whole_steps(N, esize) : ldn, esize) : Plan{}, pw = gw ? plan_of(N, K, parts ? 2 * whole_steps(M, esize) : M, esize) : Plan{};
+    const Plan px = gx ? plan_gx(M, N, K, esize, parts) : Plan{}, pw = gw ? plan_gw(M, N, K, esize, parts) : Plan{};
     if (gx && gw && pairs(pw, px)) return b + pw.part_bytes + px.part_bytes;
     return b + (px.part_bytes > pw.part_bytes ? px.part_bytes : pw.part_bytes);
 }
@@ -862,7 +865,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
     const BwdNeeds d = bwd_needs(x, w, gy, es, N, K, act, gx != nullptr, gw != nullptr);
     const long ldn = padded(N, es), ldk = padded(K, es);
     const GradCut c = grad_cut(M, ldn, es);
-    const bool parts = in_parts<T>(act);
+    const bool parts = in_parts(es, act);
     T* gz = nullptr;
     if (d.gz) {
         gz = reinterpret_cast<T*>(ws);
@@ -892,7 +895,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         x_.p = {w, ldk, (int)ldk, 0};
         // gz has zeros behind its N-th column, W has no line there: k ends at N for W's lines and at ldn for gz's pieces
         set_k<T>(x_, N, parts);
-        px = plan_of(M, K, parts ? x_.end : ldn, es);
+        px = plan_gx(M, N, K, es, parts);
     }
     if (gw) {
         w_.M = (int)N; w_.N = (int)K;
@@ -900,7 +903,7 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
         w_.e.y = gw; w_.e.wide = wide && aligned16(gw);
         w_.q = {dz, ldn, (int)ldn, M * ldn};
         w_.p = {x, ldk, (int)ldk, 0};
-        pw = plan_of(N, K, w_.end, es);
+        pw = plan_gw(M, N, K, es, parts);
     }
     float* const part = reinterpret_cast<float*>(ws);
     ColumnsP columns{sums, c.chunks, (int)ldn, (int)N, gb, btype, gb && c.chunks > 1 ? sed_cdiv(N, 16) : 0};
@@ -917,6 +920,14 @@ int linear_bwd(const void* x, const void* w, const void* gy, const void* z, int 
 }  // namespace
 
 SED_API long sed_linear_kept_elements(long M, long N) { return M < 1 || N < 1 ? 0 : M * padded(N, 2); }
+
+SED_API int sed_linear_plan(int dtype, long M, long N, long K, int act, int which) {
+    if (bad_shape(dtype, M, N, K, act) || which < 0 || which > 2) return 0;
+    const int es = esize_of(dtype);
+    if (which == 0 && few_rows(M, K, es)) return 1 + 1024;
+    const Plan p = which == 0 ? plan_of(M, N, padded(K, es), es) : which == 1 ? plan_gx(M, N, K, es, in_parts(es, act)) : plan_gw(M, N, K, es, in_parts(es, act));
+    return p.edge + 1024 * p.slices;
+}
 
 SED_API long sed_linear_fwd_ws_bytes(const void* x, const void* w, int dtype, long M, long N, long K) {
     return bad_shape(dtype, M, N, K, 0) ? 0 : fwd_ws(x, w, esize_of(dtype), M, N, K);

@@ -421,3 +421,124 @@ def test_relu_passes_the_gradient_of_a_nan(m, dtype):
     d = [t.detach().double().requires_grad_(True) for t in leaves]
     want = torch.autograd.grad(F.relu(F.linear(*d)), d, gy.double())
     assert all(torch.equal(torch.isnan(a), torch.isnan(c)) for a, c in zip(got, want))
+
+
+# Shapes whose products are cut into tiles of 128 and 256: (which product, edge, cut along k), rows, K, N.  No size is a multiple of 64, so that
+# every one ends inside a tile and inside a step; the second shape of each pair has lines that are not aligned.
+WIDE16 = [(0, 128, False, 33772, 40, 72), (0, 128, False, 37109, 40, 67), (0, 128, True, 67, 5224, 4312), (0, 128, True, 3074, 5501, 65),
+          (0, 256, False, 26822, 1064, 408), (0, 256, False, 19870, 1033, 540)]
+BACK16 = [(1, 128, False, 33035, 72, 40), (1, 128, False, 33885, 68, 46), (1, 128, True, 73, 3384, 5968), (1, 128, True, 4297, 66, 4609),
+          (1, 256, False, 25665, 400, 1104), (1, 256, False, 19738, 522, 1061), (2, 128, False, 65, 880, 4704), (2, 128, False, 66, 3590, 1115),
+          (2, 128, True, 4365, 4248, 72), (2, 128, True, 5554, 3077, 65), (2, 256, False, 1050, 3352, 3656), (2, 256, False, 1031, 3245, 3836),
+          (2, 256, True, 38925, 392, 3144), (2, 256, True, 38748, 3106, 386)]
+WIDE32 = [(0, 28623, 40, 144), (0, 21371, 42, 206), (0, 66, 2072, 4640), (0, 4153, 2061, 66), (1, 28303, 144, 40), (1, 27290, 130, 49),
+          (1, 4294, 80, 2120), (1, 67, 4227, 2093), (2, 67, 4904, 1080), (2, 67, 2638, 1933), (2, 2218, 80, 4272), (2, 2227, 4119, 66)]
+
+
+def _plan(dtype, m, k, n, act, which):
+    """(edge, slices) of one product of a call."""
+    from sound_event_detection_dcase2017_task4_amd import _lib
+    p = _lib.lib().sed_linear_plan(ops.DTYPE_CODES[dtype], m, n, k, ops.ACTIVATIONS[act], which)
+    return p % 1024, p // 1024
+
+
+def _poison(dtype):
+    """LDS and scratch hold NaN when the case begins: what is read beside the matrices shows."""
+    ops.linear_act(*[torch.full((4000, 1000), float("nan"), dtype=dtype, device="cuda")] * 2)
+
+
+@gpu
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("which,edge,cut,m,k,n", WIDE16)
+def test_forward_in_larger_tiles(which, edge, cut, m, k, n, dtype, act):
+    got = _plan(dtype, m, k, n, act, which)
+    assert got[0] == edge and (got[1] > 1) == cut
+    x, w, b, r, _ = _inputs(m, k, n, dtype, dtype, 61)
+    _poison(dtype)
+    for bias, res in ((b, r), (b.float(), None), (None, r)):
+        leaf = x.clone().requires_grad_(True)              # z is kept, or its mask
+        y = ops.linear_act(leaf, w, bias, act, res)
+        z = x.double() @ w.double().t() + (0 if bias is None else bias.double())
+        want = ACTS[act](z) + (0 if res is None else res.double())
+        # as in _check
+        zerr = _sum_err(k) * (x.double().abs() @ w.double().abs().t() + (0 if bias is None else bias.double().abs())) + 4 * H
+        tol = 1.2 * zerr + 12 * H * (1 + want.abs()) + HALF[dtype] * 1.01 * want.abs() + TINY[dtype]
+        assert ((y.detach().double() - want).abs() <= tol).all()
+        with torch.no_grad():
+            assert torch.equal(ops.linear_act(x, w, bias, act, res), y)
+        gy = torch.ones_like(y)                            # what was kept gives the derivative: a bias gradient that is a plain sum of it
+        if bias is not None and bias.dtype == torch.float32 and act != "relu":
+            lb = bias.clone().requires_grad_(True)
+            gb, = torch.autograd.grad(ops.linear_act(x, w, lb, act, res), lb, gy)
+            zl = z.clone().requires_grad_(True)
+            da, = torch.autograd.grad(ACTS[act](zl).sum(), zl)
+            assert ((gb.double() - da.sum(0)).abs() <= (1.2 * zerr + 16 * H).sum(0) + _sum_err(m) * da.abs().sum(0)).all()
+
+
+@gpu
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("which,edge,cut,m,k,n", BACK16)
+def test_gradients_in_larger_tiles(which, edge, cut, m, k, n, dtype, act):
+    got = _plan(dtype, m, k, n, act, which)
+    assert got[0] == edge and (got[1] > 1) == cut
+    x, w, b, _, gy = _inputs(m, k, n, dtype, torch.float32, 67, residual=False)
+    _poison(dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(ops.linear_act(*leaves, activation=act), leaves, gy)
+    z = (x.double() @ w.double().t() + b.double()).requires_grad_(True)
+    gz = gy.double() * torch.autograd.grad(ACTS[act](z).sum(), z)[0]
+    e, tiny = HALF[dtype], TINY[dtype]
+    zerr = _sum_err(k) * (x.double().abs() @ w.double().abs().t() + b.double().abs()) + 4 * H
+    gzerr = gy.double().abs() * (1.2 * zerr + 16 * H) + e * e * gz.abs() + (2.0 ** -36 if dtype == torch.float16 else 0)
+    want, terms = (gz @ w.double(), gz.t() @ x.double()), (_sum_err(2 * n) * (gz.abs() @ w.double().abs()), _sum_err(2 * m) * (gz.abs().t() @ x.double().abs()))
+    for a, c, err, t in zip(got, want, (gzerr @ w.double().abs(), gzerr.t() @ x.double().abs()), terms):
+        assert ((a.double() - c).abs() <= err + t + e * 1.01 * c.abs() + tiny).all()
+        assert (a.double() - c).norm() <= 1.05 * (c.to(dtype).double() - c).norm()
+    assert ((got[2].double() - gz.sum(0)).abs() <= (gy.double().abs() * (1.2 * zerr + 16 * H)).sum(0) + _sum_err(m) * gz.abs().sum(0)).all()
+    only, = torch.autograd.grad(ops.linear_act(*leaves, activation=act), [leaves[which - 1]], gy)
+    assert torch.equal(only, got[which - 1])               # the product by itself
+
+
+@gpu
+@pytest.mark.parametrize("which,m,k,n", WIDE32)
+def test_32_bit_products_in_larger_tiles(which, m, k, n):
+    act = ("silu", "gelu", "none")[(m + k) % 3]
+    assert _plan(torch.float32, m, k, n, act, which)[0] == 128
+    _poison(torch.float32)
+    _check(*_inputs(m, k, n, torch.float32, torch.float32, 71, residual=m % 2 == 0), act)
+
+
+def test_plans_cover_every_edge():
+    """What the tests above run: every edge whole and cut, but for 256 in the forward product and gx, which the rule does not cut."""
+    for dtype in (torch.float16, torch.bfloat16):
+        assert {c[:3] for c in WIDE16} == {(0, 128, False), (0, 128, True), (0, 256, False)}
+        assert {c[:3] for c in BACK16} == {(w, e, c) for w in (1, 2) for e in (128, 256) for c in (False, True)} - {(1, 256, True)}
+        for which, edge, cut, m, k, n in WIDE16 + BACK16:
+            assert all(s % 64 for s in (m, k, n))
+            for act in ("none", "silu"):
+                p = _plan(dtype, m, k, n, act, which)
+                assert p[0] == edge and (p[1] > 1) == cut
+    for which in range(3):
+        assert {(_plan(torch.float32, m, k, n, "none", w)[1] > 1) for w, m, k, n in WIDE32 if w == which} == {False, True}
+    assert _plan(torch.float16, 3, 64, 64, "none", 0) == (1, 1) and _plan(torch.float16, 0, 64, 64, "none", 0) == (0, 0)
+
+
+@gpu
+def test_parts_of_more_than_two_to_the_31_elements():
+    """gz in two parts of 2.7e9 elements each: rows at both ends of it, all others without a gradient."""
+    M, K, N, dtype = 2 ** 26 + 70, 8, 40, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ends = torch.cat([torch.arange(200), torch.arange(M - 200, M)]).cuda()
+    x = torch.zeros((M, K), dtype=dtype, device="cuda")
+    x[ends] = torch.randn((400, K), generator=g, device="cuda").to(dtype)
+    w = torch.randn((N, K), generator=g, device="cuda").to(dtype)
+    gy = torch.zeros((M, N), dtype=dtype, device="cuda")
+    gy[ends] = torch.randn((400, N), generator=g, device="cuda").to(dtype)
+    leaves = [x.requires_grad_(True), w.clone().requires_grad_(True)]
+    gx, gw = torch.autograd.grad(ops.linear_act(*leaves, activation="silu"), leaves, gy)
+    _, want, _ = _gradients(x.detach()[ends], w, gy[ends], "silu")
+    for a, c in ((gx[ends], want[0]), (gw, want[1])):
+        assert (a.double() - c).norm() <= 1.05 * (c.to(dtype).double() - c).norm()
+    assert not gx[200:100000].any() and not gx[-100000:-200].any()
