@@ -79,7 +79,7 @@ template <typename T> __device__ __forceinline__ void store4(T* p, long e, long 
 }
 
 // largest of non-negative floats over the wave, compared as bits: a NaN is the largest of all and is not lost.  Lanes trade within quads,
-// rows of 16 and across rows by DPP moves, which need no LDS (958 -> 828 us at 240 M elements, now 797); lane 63 ends with the largest.
+// rows of 16 and across rows by DPP moves, which need no LDS (958 -> 828 us at 240 M elements, now 820); lane 63 ends with the largest.
 template <int CTRL> __device__ __forceinline__ int max_dpp(int m) { return max(m, __builtin_amdgcn_update_dpp(m, m, CTRL, 0xf, 0xf, false)); }
 __device__ __forceinline__ float wave_max_bits(float a, float b, float c, float d) {
     int m = max(max(__float_as_int(a), __float_as_int(b)), max(__float_as_int(c), __float_as_int(d)));       // no sign bit: int order is float order

@@ -762,8 +762,9 @@ template <typename T, int V, int ACT, int R> __global__ __launch_bounds__(ONE_TH
 // what was left, from memory.  The results are the same bits either way.
 // Taken from 384 MB on: below 256 MB the caches serve the second reading of the two passes.  256 x 64064 x 64 float16 (2.1 GB) takes
 // 1062 us, in two passes 1255; 64 x 64064 x 64 float32 459 and 667; 262 MB of either type 149 to 201 and 163 to 179; 131 MB 85 and 80.
-// (Backward, with x and gy in registers, it lost: 65 M bfloat16 elements 190 us, in two passes 146 -- a sample then has twice the workgroups,
-// and the last one adds up a row of channels from each.)
+// (Backward, with x and gy in registers, the form that was built lost: 65 M bfloat16 elements 190 us, in two passes 146.  A sample then has
+// twice the workgroups, and each published a row of channels for the last one to add up; what the waiting ones need is two numbers a
+// group and chunk, which was not built.)
 constexpr long SHARED_LEAST = 384l << 20;          // bytes of x
 constexpr int SHARED_MOST = 128;                   // workgroups of a sample, of the 512 that are resident
 constexpr long WAIT_TICKS = 200000;                // of the 100 MHz clock: 2 ms

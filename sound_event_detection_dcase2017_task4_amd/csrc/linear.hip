@@ -302,7 +302,7 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
     SQ::offsets(a.q, m0, qoff);
     // For the epilogue a wave passes 32 rows of its results at a time through LDS: a lane then has V consecutive n of row
     // 32 i + PASS it + lane / LINE, and its neighbours have the rest of the line.  (Stored from where the instructions leave them, 32 bytes
-    // a line, a bf16 product of 32000 x 2048 x 2048 with silu, residual and kept z took 402 us, now 330.)
+    // a line, a bf16 product of 32000 x 2048 x 2048 with silu, residual and kept z took 402 us, now 335.)
     constexpr int W = BN / WN, LINE = W / V, PASS = 64 / LINE, PASSES = 32 / PASS, PITCH = 4 * W + 16;
     static_assert(4 * 32 * PITCH <= 5 * SLOT, "the waves' rows fit the ring");
     const int n = n0 + wn + lane % LINE * V;
@@ -457,8 +457,9 @@ template <int ROWS> __device__ __forceinline__ void column_sums(const ColumnsP& 
 
 // both products of a backward pass, and the bias gradient's last sums, in one launch, where both are cut into tiles of 64: the first
 // c.blocks workgroups take the sums, the next `first` gz^T x, whose tiles are the longer ones where there are more rows than columns,
-// the others gz W.  Forward and backward of 4000 x 512 x 512 bf16
-// 44.9 -> 39.8 us, of 4000 x 512 x 2048 86 -> 72, of 500 x 96 x 136 fp32 29.1 -> 24.3.
+// the others gz W.  Forward and backward of 4000 x 512 x 512 bf16 take 27.3 us so and 35.7 in two launches (with gelu, gz in two
+// parts, 42.6 and 49.9), of 4000 x 512 x 2048 58.7 and 76.9 (with gelu gW is cut into tiles of 128, and the launches are two: 113), of
+// 500 x 96 x 136 fp32 16.7 and 23.1.
 template <typename T, bool CUTW, bool CUTX> __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(GemmP w, GemmP x, int first, ColumnsP c) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[5 * 64 * 128];
     const int bid = (int)blockIdx.x - c.blocks;
