@@ -128,7 +128,7 @@ template <typename T, int V, int ACT> __device__ __forceinline__ void finish(con
 
 // One number as the sum of two of a 16-bit type: what is lost is 2^-18 of it in bfloat16, 2^-24 of it or 2^-36 in float16, which holds half of it
 // and the small part times 2^11.  An infinity or NaN is in the large part alone.
-template <typename T> struct Split;
+template <typename T> struct Split { static constexpr float UNIT = 1.f, LOW = 1.f; };
 template <> struct Split<__bf16> { static constexpr float UNIT = 1.f, LOW = 1.f; };
 template <> struct Split<_Float16> { static constexpr float UNIT = 0.5f, LOW = 0x1p-11f; };
 template <typename T> __device__ __forceinline__ void split(float f, T& large, T& small) {
@@ -170,7 +170,7 @@ __device__ __forceinline__ floatx16 mma(floatx4 p, floatx4 q, floatx16 c) {
 // what it leaves: gx and gW then carry their own rounding only (gz rounded once put as much again into them, and in float16 lost what is
 // below 6e-8).  k runs over the small parts first and over the large ones behind them, 0 .. K and half .. half + K, half the next
 // multiple of the step.  float16 holds gz / 2, which cannot overflow, and the small part times 2^11, which does not underflow: the sums are
-// multiplied by `low` between the parts and by `scale` at the end, powers of two (the float16 kernels of edge 256 spill there, outside the
+// multiplied by 2^-11 between the parts and by 2 at the end (the float16 kernels of edge 256 spill there, outside the
 // loop).  It doubles the two products: forward and backward of 32000 x 2048 x 2048 bf16 take 1302 us, for 848 with gz and z in 16
 // bits, of 4000 x 512 x 2048 125 for 116; the error against 64 bits is 1.7e-3 for 2.4e-3, that of the output's rounding.
 struct Operand {
@@ -185,7 +185,6 @@ struct GemmP {
     int M, N;
     long K;
     long half, end;                                // first k of the second part, end of the last one
-    float low, scale;
     long kslice;                                   // k of one slice, a multiple of the step
     int tm, tn;                                    // tiles
     float* part;                                   // [slices][M][ldp] where the product is cut along k
@@ -280,7 +279,7 @@ template <int LATER> __device__ __forceinline__ void arrived() {
 // all of it (a wave that issues sixteen at once waits for the address unit: 57 % of the matrix rate against 72 %), and have at least
 // three quarters to arrive.  Steps behind the end are requested and read like any other, as zeros: the loop has no other branch.
 // `bid` of `blocks` workgroups; lds: 5 slots.
-template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT, int ACT>
+template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT, int ACT, bool PARTS>
 __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, unsigned char* lds) {
     constexpr int THREADS = 64 * WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, V = 16 / sizeof(T);
     typedef Stage<T, BN, PROWS, THREADS, V == 8> SP;
@@ -293,7 +292,7 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
     // tiles in groups of eight rows of tiles: the 32 that an XCD works on share 8 + 4 operand tiles, not 32 + 1
     const int group = tile / (8 * a.tn), gm = min(8, a.tm - 8 * group), in = tile - group * 8 * a.tn;
     const int m0 = (8 * group + in % gm) * BM, n0 = in / gm * BN;
-    constexpr bool PARTS = PROWS && sizeof(T) == 2;          // the backward products
+    static_assert(!PARTS || (PROWS && sizeof(T) == 2), "the backward products of 16-bit tensors");
     const long end = PARTS ? a.end : a.K, k0 = CUT ? slice * a.kslice : 0, k1 = CUT ? min(end, k0 + a.kslice) : end;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
@@ -373,9 +372,9 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
             const long stop = min(k1, k < a.half ? a.half : k1);
             for (; k < stop; k += SP::STEP) step(k);
             if constexpr (Split<T>::LOW != 1.f)
-                if (a.low != 1.f && k <= a.half)
+                if (k <= a.half)
 #pragma unroll
-                    for (int f = 0; f < MFMAS; ++f) acc[f / NI][f % NI] *= a.low;
+                    for (int f = 0; f < MFMAS; ++f) acc[f / NI][f % NI] *= Split<T>::LOW;
         } while (k < k1);
     } else {
         for (long k = k0; k < k1; k += SP::STEP) step(k);
@@ -404,7 +403,7 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
             for (int h = 0; h < V / 4; ++h) {
                 const floatx4 q = *reinterpret_cast<const floatx4*>(mine + (PASS * it + lane / LINE) * PITCH + place(lane % LINE * (V / 4) + h));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * h + j] = PARTS ? q[j] * a.scale : q[j];
+                for (int j = 0; j < 4; ++j) v[4 * h + j] = PARTS ? q[j] * (1.f / Split<T>::UNIT) : q[j];
             }
             const int m = row(i, it);
             if (m >= a.M || n >= a.N) continue;
@@ -426,10 +425,10 @@ __device__ __forceinline__ void gemm_tile(const GemmP& a, int bid, int blocks, u
     }
 }
 
-template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT, int ACT>
+template <typename T, bool PROWS, bool QROWS, int BM, int BN, int WM, int WN, bool CUT, int ACT, bool PARTS>
 __global__ __launch_bounds__(64 * WM * WN, BM * BN > 128 * 128 ? 1 : 2) void gemm_kernel(GemmP a) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[5 * BM * 128];
-    gemm_tile<T, PROWS, QROWS, BM, BN, WM, WN, CUT, ACT>(a, blockIdx.x, gridDim.x, lds);
+    gemm_tile<T, PROWS, QROWS, BM, BN, WM, WN, CUT, ACT, PARTS>(a, blockIdx.x, gridDim.x, lds);
 }
 // gb [N] of `type` = the column sums of sums [chunks][ld]: 16 columns x ROWS lanes, a power of two
 struct ColumnsP {
@@ -460,12 +459,12 @@ template <int ROWS> __device__ __forceinline__ void column_sums(const ColumnsP& 
 // the others gz W.  Forward and backward of 4000 x 512 x 512 bf16 take 27.3 us so and 35.7 in two launches (with gelu, gz in two
 // parts, 42.6 and 49.9), of 4000 x 512 x 2048 58.7 and 76.9 (with gelu gW is cut into tiles of 128, and the launches are two: 113), of
 // 500 x 96 x 136 fp32 16.7 and 23.1.
-template <typename T, bool CUTW, bool CUTX> __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(GemmP w, GemmP x, int first, ColumnsP c) {
+template <typename T, bool CUTW, bool CUTX, bool PARTS> __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(GemmP w, GemmP x, int first, ColumnsP c) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[5 * 64 * 128];
     const int bid = (int)blockIdx.x - c.blocks;
     if (bid < 0) column_sums<16>(c, blockIdx.x, reinterpret_cast<float*>(lds));
-    else if (bid < first) gemm_tile<T, true, true, 64, 64, 2, 2, CUTW, 0>(w, bid, first, lds);
-    else gemm_tile<T, true, false, 64, 64, 2, 2, CUTX, 0>(x, bid - first, gridDim.x - c.blocks - first, lds);
+    else if (bid < first) gemm_tile<T, true, true, 64, 64, 2, 2, CUTW, 0, PARTS>(w, bid, first, lds);
+    else gemm_tile<T, true, false, 64, 64, 2, 2, CUTX, 0, PARTS>(x, bid - first, gridDim.x - c.blocks - first, lds);
 }
 
 // the slices of a cut product, added in order, and the epilogue
@@ -675,9 +674,6 @@ template <typename T> void set_k(GemmP& a, long K, bool parts) {
     a.K = K;
     a.half = parts ? whole_steps(K, sizeof(T)) : ONE_PART;
     a.end = parts ? 2 * a.half : K;
-    a.low = a.scale = 1.f;
-    if constexpr (sizeof(T) == 2)
-        if (parts) { a.low = Split<T>::LOW; a.scale = 1.f / Split<T>::UNIT; }
 }
 
 // How a product is cut: tile edge, and slices along k that a second pass adds.  The cut with the least time by what was measured on an
@@ -718,17 +714,22 @@ Plan plan_of(long M, long N, long K, int esize) {
 // rows 10.1, 64 rows 24.7 against 15.2 in tiles; (64, 2048, 512) 5.1 against 5.5, (64, 512, 2048) 13.4 against 8.1.
 bool few_rows(long M, long K, int esize) { return M <= 64 && K * esize <= (M <= 16 ? 16384 : M <= 32 ? 4096 : 1024); }
 
-template <typename T, bool PROWS, bool QROWS, int EDGE> void launch_edge(const GemmP& a, const Plan& q, hipStream_t stream) {
+template <typename T, bool PROWS, bool QROWS, int EDGE, bool PARTS> void launch_edge(const GemmP& a, const Plan& q, hipStream_t stream) {
     const dim3 grid((unsigned)((long)q.tm * q.tn * q.slices));
-    if (q.slices > 1) { hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, true, 0>), grid, dim3(256), 0, stream, a); return; }
+    if (q.slices > 1) { hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, true, 0, PARTS>), grid, dim3(256), 0, stream, a); return; }
     if constexpr (!PROWS) {                        // only the forward product has an epilogue
         switch (a.e.act) {
-            case SED_ACT_RELU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 1>), grid, dim3(256), 0, stream, a); return;
-            case SED_ACT_SILU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 2>), grid, dim3(256), 0, stream, a); return;
-            case SED_ACT_GELU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 3>), grid, dim3(256), 0, stream, a); return;
+            case SED_ACT_RELU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 1, PARTS>), grid, dim3(256), 0, stream, a); return;
+            case SED_ACT_SILU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 2, PARTS>), grid, dim3(256), 0, stream, a); return;
+            case SED_ACT_GELU: hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 3, PARTS>), grid, dim3(256), 0, stream, a); return;
         }
     }
-    hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 0>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((gemm_kernel<T, PROWS, QROWS, EDGE, EDGE, 2, 2, false, 0, PARTS>), grid, dim3(256), 0, stream, a);
+}
+template <typename T, bool PROWS, bool QROWS, bool PARTS> void launch_edges(const GemmP& a, const Plan& q, hipStream_t stream) {
+    if (q.edge == 64) launch_edge<T, PROWS, QROWS, 64, PARTS>(a, q, stream);
+    else if (q.edge == 128 || sizeof(T) == 4) launch_edge<T, PROWS, QROWS, 128, PARTS>(a, q, stream);
+    else if constexpr (sizeof(T) == 2) launch_edge<T, PROWS, QROWS, 256, PARTS>(a, q, stream);
 }
 void place(GemmP& a, const Plan& q, float* part) { a.tm = q.tm; a.tn = q.tn; a.kslice = q.kslice; a.part = part; a.ldp = q.ldp; }
 template <typename T> void launch_join(const GemmP& a, const Plan& q, hipStream_t stream) {
@@ -738,24 +739,24 @@ template <typename T> void launch_join(const GemmP& a, const Plan& q, hipStream_
 }
 template <typename T, bool PROWS, bool QROWS> void launch_gemm(GemmP a, const Plan& q, float* part, hipStream_t stream) {
     place(a, q, part);
-    if (q.edge == 64) launch_edge<T, PROWS, QROWS, 64>(a, q, stream);
-    else if (q.edge == 128 || sizeof(T) == 4) launch_edge<T, PROWS, QROWS, 128>(a, q, stream);
-    else if constexpr (sizeof(T) == 2) launch_edge<T, PROWS, QROWS, 256>(a, q, stream);
+    if (a.half == ONE_PART) launch_edges<T, PROWS, QROWS, false>(a, q, stream);
+    else if constexpr (PROWS && sizeof(T) == 2) launch_edges<T, PROWS, QROWS, true>(a, q, stream);
     launch_join<T>(a, q, stream);
 }
 bool pairs(const Plan& w, const Plan& x) { return w.edge == 64 && x.edge == 64 && (long)w.tm * w.tn * w.slices + (long)x.tm * x.tn * x.slices < (1L << 24) - (1L << 17); }
+template <typename T, bool PARTS> void launch_pair(const GemmP& w, bool cutw, const GemmP& x, bool cutx, int first, const ColumnsP& c, dim3 grid, hipStream_t stream) {
+    if (cutw && cutx) hipLaunchKernelGGL((gemm_pair_kernel<T, true, true, PARTS>), grid, dim3(256), 0, stream, w, x, first, c);
+    else if (cutw) hipLaunchKernelGGL((gemm_pair_kernel<T, true, false, PARTS>), grid, dim3(256), 0, stream, w, x, first, c);
+    else if (cutx) hipLaunchKernelGGL((gemm_pair_kernel<T, false, true, PARTS>), grid, dim3(256), 0, stream, w, x, first, c);
+    else hipLaunchKernelGGL((gemm_pair_kernel<T, false, false, PARTS>), grid, dim3(256), 0, stream, w, x, first, c);
+}
 template <typename T> void launch_pair(GemmP w, const Plan& qw, GemmP x, const Plan& qx, const ColumnsP& c, float* part, hipStream_t stream) {
     place(w, qw, part);
     place(x, qx, part + qw.part_bytes / 4);
     const int first = qw.tm * qw.tn * qw.slices;
     const dim3 grid((unsigned)(c.blocks + first + qx.tm * qx.tn * qx.slices));
-    if (qw.slices > 1) {
-        if (qx.slices > 1) hipLaunchKernelGGL((gemm_pair_kernel<T, true, true>), grid, dim3(256), 0, stream, w, x, first, c);
-        else hipLaunchKernelGGL((gemm_pair_kernel<T, true, false>), grid, dim3(256), 0, stream, w, x, first, c);
-    } else {
-        if (qx.slices > 1) hipLaunchKernelGGL((gemm_pair_kernel<T, false, true>), grid, dim3(256), 0, stream, w, x, first, c);
-        else hipLaunchKernelGGL((gemm_pair_kernel<T, false, false>), grid, dim3(256), 0, stream, w, x, first, c);
-    }
+    if (w.half == ONE_PART) launch_pair<T, false>(w, qw.slices > 1, x, qx.slices > 1, first, c, grid, stream);
+    else if constexpr (sizeof(T) == 2) launch_pair<T, true>(w, qw.slices > 1, x, qx.slices > 1, first, c, grid, stream);
     launch_join<T>(w, qw, stream);
     launch_join<T>(x, qx, stream);
 }
