@@ -937,7 +937,7 @@ SED_API long sed_linear_fwd_ws_bytes(const void* x, const void* w, int dtype, lo
 
 SED_API int sed_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, int dtype, int bdtype, long M, long N,
                            long K, int act, void* y, void* z, void* ws, long ws_bytes, sed_stream_t stream) {
-    if (!x || !w || !y || bdtype < 0 || bdtype > 2 || bad_shape(dtype, M, N, K, act)) return SED_EINVAL;
+    if (!x || !w || !y || !aligned16(z) || bdtype < 0 || bdtype > 2 || bad_shape(dtype, M, N, K, act)) return SED_EINVAL;
     const long need = fwd_ws(x, w, esize_of(dtype), M, N, K);
     if (need && (!ws || ws_bytes < need || !aligned16(ws))) return SED_EINVAL;
     char* const s = reinterpret_cast<char*>(ws);

@@ -542,3 +542,10 @@ def test_parts_of_more_than_two_to_the_31_elements():
     for a, c in ((gx[ends], want[0]), (gw, want[1])):
         assert (a.double() - c).norm() <= 1.05 * (c.to(dtype).double() - c).norm()
     assert not gx[200:100000].any() and not gx[-100000:-200].any()
+
+
+def test_c_entry_refuses_a_kept_z_that_is_not_aligned():
+    """It is written 16 bytes at a time."""
+    from sound_event_detection_dcase2017_task4_amd import _lib
+    for z in (2, 4, 24):
+        assert _lib.lib().sed_linear_fwd(16, 16, None, None, 1, 1, 100, 8, 8, 2, 16, z, None, 0, None) == -22
